@@ -1,0 +1,167 @@
+// Values into e4m3 with a float32 scale for each block: 128 of a row (activations), or 128 x 128 of a matrix (weights).
+//
+//   a = max(amax of the block, 2^-100),  scale = a / 448,  code = e4m3 nearest to 448 x / a  (448 is the largest e4m3)
+//
+// The quotient is rounded once to float32 and once to e4m3: a quotient of two bfloat16 numbers often lies right between two e4m3, and a product with a
+// rounded reciprocal would take one or the other by chance (2 to 3 of 1,000 codes).  2^-100 keeps a block of zeros, or of nothing that counts, free of
+// divisions by zero.  A block that holds a NaN has NaN as its scale and codes; one that holds an infinity an infinite scale and, there, a NaN.
+//
+// Both read their input once and keep it in registers while the block's largest value is found; they are bound by memory.
+#include "common.cuh"
+#include <cuda_fp8.h>
+
+namespace {
+constexpr int QB = 128;                              // a block's edge
+constexpr unsigned LEAST_BITS = 0x0D800000u;         // 2^-100
+constexpr unsigned LARGE_BITS = 0x71800000u;         // 2^100
+
+// What a block's values are turned to codes with: x -> (x * mul) / div.  (Above 2^100 both by 2^-20 less, so that 448 x stays finite.)
+struct Coding {
+    float mul, div, scale;
+};
+__device__ __forceinline__ Coding coding_of(unsigned amax_bits) {
+    const unsigned bits = max(amax_bits, LEAST_BITS);        // (a NaN's bits are above all others)
+    const float a = __uint_as_float(bits);
+    Coding c;
+    c.mul = bits > LARGE_BITS ? 448.f * 0x1p-20f : 448.f;
+    c.div = bits > LARGE_BITS ? a * 0x1p-20f : a;
+    c.scale = a / 448.f;
+    return c;
+}
+__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t codes4(const float* v, const Coding& c) {
+    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[0] * c.mul, c.div), __fdiv_rn(v[1] * c.mul, c.div)), __NV_SATFINITE, __NV_E4M3);
+    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[2] * c.mul, c.div), __fdiv_rn(v[3] * c.mul, c.div)), __NV_SATFINITE, __NV_E4M3);
+    return (uint32_t)lo | ((uint32_t)hi << 16);
+}
+
+// Eight consecutive values of a row of K, zeros past its end.
+template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* row, int k, int K, float (&v)[8]) {
+    if (VEC && k + 8 <= K) {
+#pragma unroll
+        for (int i = 0; i < 8; i += Vec16<T>::N) load16<T>(row + k + i, v + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f<T>(row[k + i]) : 0.f;
+    }
+}
+// Their codes, into a row that starts at a multiple of 16 bytes and has room for K rounded up to 16.
+__device__ __forceinline__ void store8(unsigned char* row, int k, int K, const float (&v)[8], const Coding& c) {
+    if (k < K) *reinterpret_cast<uint2*>(row + k) = make_uint2(codes4(v, c), codes4(v + 4, c));
+}
+
+// Sixteen lanes take a block of a row, eight values each; a group of lanes takes UNITS blocks, all of whose loads are asked for first.
+constexpr int ROWS_THREADS = 256, UNITS = 2;
+template <typename T, bool VEC>
+__global__ __launch_bounds__(ROWS_THREADS) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, unsigned char* __restrict__ codes, long long ldc,
+                                                                     float* __restrict__ scales, int n_tokens, int K, int k_blocks) {
+    pdl_wait_and_trigger();
+    const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
+    const long long total = (long long)n_tokens * k_blocks;
+    const long long first = (long long)blockIdx.x * (ROWS_THREADS / 16 * UNITS) + group;
+    float v[UNITS][8];
+    int row[UNITS], kb[UNITS];
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const long long unit = first + u * (ROWS_THREADS / 16);
+        row[u] = unit < total ? (int)(unit / k_blocks) : -1;
+        kb[u] = unit < total ? (int)(unit - (long long)row[u] * k_blocks) : 0;
+        if (row[u] >= 0) {
+            load8<T, VEC>(x + row[u] * ldx, kb[u] * QB + lane * 8, K, v[u]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        unsigned amax = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(v[u][i]));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));      // within the sixteen lanes
+        if (row[u] < 0) continue;
+        const Coding c = coding_of(amax);
+        store8(codes + row[u] * ldc, kb[u] * QB + lane * 8, K, v[u], c);
+        if (lane == 0) scales[(long long)kb[u] * n_tokens + row[u]] = c.scale;
+    }
+}
+
+// A CTA takes a block of 128 x 128: sixteen lanes a row, sixteen rows at a time.
+constexpr int MATRIX_THREADS = 256, MATRIX_ROWS = QB / (MATRIX_THREADS / 16);
+template <typename T, bool VEC>
+__global__ __launch_bounds__(MATRIX_THREADS) void quantize_matrix_kernel(const T* __restrict__ w, long long ldw, long long stack_w, unsigned char* __restrict__ codes,
+                                                                         long long ldc, float* __restrict__ scales, int N, int K) {
+    pdl_wait_and_trigger();
+    __shared__ unsigned part[MATRIX_THREADS / 32];
+    const int kb = blockIdx.x, nb = blockIdx.y, e = blockIdx.z;
+    const int r0 = nb * QB + (threadIdx.x >> 4), k = kb * QB + (threadIdx.x & 15) * 8;
+    w += e * stack_w;
+    codes += (long long)e * N * ldc;
+    float v[MATRIX_ROWS][8];
+    unsigned amax = 0;
+#pragma unroll
+    for (int i = 0; i < MATRIX_ROWS; ++i) {
+        const int r = r0 + i * (MATRIX_THREADS / 16);
+        if (r < N) {
+            load8<T, VEC>(w + r * ldw, k, K, v[i]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MATRIX_ROWS; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = max(amax, abs_bits(v[i][j]));
+    amax = __reduce_max_sync(0xffffffffu, amax);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < MATRIX_THREADS / 32; ++i) amax = max(amax, part[i]);
+    const Coding c = coding_of(amax);
+#pragma unroll
+    for (int i = 0; i < MATRIX_ROWS; ++i) {
+        const int r = r0 + i * (MATRIX_THREADS / 16);
+        if (r < N) store8(codes + r * ldc, k, K, v[i], c);
+    }
+    if (threadIdx.x == 0) scales[((long long)e * gridDim.y + nb) * gridDim.x + kb] = c.scale;
+}
+
+bool in_vectors(const void* p, long long ld, int size) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && (ld * size) % 16 == 0; }
+}  // namespace
+
+// x [T, K] (rows ldx elements apart) -> codes [T, K] (rows ldc bytes apart, a multiple of 16) and scales float32 [ceil(K / 128), T].
+extern "C" int rlis_quantize_rows(const void* x, long long ldx, void* codes, long long ldc, float* scales, int n_tokens, int K, int dtype, cudaStream_t stream) {
+    if (n_tokens <= 0 || K <= 0) return 0;
+    if ((dtype != RLIS_F32 && dtype != RLIS_BF16) || ldc < ((K + 15) & ~15) || ldc % 16 != 0 || (reinterpret_cast<uintptr_t>(codes) & 15) != 0) return RLIS_ERR_UNSUPPORTED;
+    const int k_blocks = (K + QB - 1) / QB, per = ROWS_THREADS / 16 * UNITS;
+    const long long ctas = ((long long)n_tokens * k_blocks + per - 1) / per;
+    if (ctas > 0x7fffffffLL) return RLIS_ERR_UNSUPPORTED;
+    const bool vec = in_vectors(x, n_tokens > 1 ? ldx : 0, dtype == RLIS_F32 ? 4 : 2);
+    const dim3 grid((unsigned)ctas);
+    unsigned char* c = static_cast<unsigned char*>(codes);
+    if (dtype == RLIS_F32)
+        rlis_launch(vec ? quantize_rows_kernel<float, true> : quantize_rows_kernel<float, false>, grid, ROWS_THREADS, 0, stream, (const float*)x, ldx, c, ldc, scales, n_tokens, K, k_blocks);
+    else
+        rlis_launch(vec ? quantize_rows_kernel<bf16, true> : quantize_rows_kernel<bf16, false>, grid, ROWS_THREADS, 0, stream, (const bf16*)x, ldx, c, ldc, scales, n_tokens, K, k_blocks);
+    return RLIS_LAUNCH_CHECK();
+}
+
+// w [E, N, K] (rows ldw and matrices stack_w elements apart) -> codes [E, N, K] (rows ldc bytes apart) and scales float32 [E, ceil(N / 128), ceil(K / 128)].
+extern "C" int rlis_quantize_matrix(const void* w, long long ldw, long long stack_w, void* codes, long long ldc, float* scales, int E, int N, int K, int dtype,
+                                    cudaStream_t stream) {
+    if (E <= 0 || N <= 0 || K <= 0) return 0;
+    const int k_blocks = (K + QB - 1) / QB, n_blocks = (N + QB - 1) / QB;
+    if ((dtype != RLIS_F32 && dtype != RLIS_BF16) || ldc < ((K + 15) & ~15) || ldc % 16 != 0 || (reinterpret_cast<uintptr_t>(codes) & 15) != 0 || n_blocks > 65535 || E > 65535)
+        return RLIS_ERR_UNSUPPORTED;
+    const int size = dtype == RLIS_F32 ? 4 : 2;
+    const bool vec = in_vectors(w, N > 1 ? ldw : 0, size) && (E == 1 || (stack_w * size) % 16 == 0);
+    const dim3 grid((unsigned)k_blocks, (unsigned)n_blocks, (unsigned)E);
+    unsigned char* c = static_cast<unsigned char*>(codes);
+    if (dtype == RLIS_F32)
+        rlis_launch(vec ? quantize_matrix_kernel<float, true> : quantize_matrix_kernel<float, false>, grid, MATRIX_THREADS, 0, stream, (const float*)w, ldw, stack_w, c, ldc, scales, N, K);
+    else
+        rlis_launch(vec ? quantize_matrix_kernel<bf16, true> : quantize_matrix_kernel<bf16, false>, grid, MATRIX_THREADS, 0, stream, (const bf16*)w, ldw, stack_w, c, ldc, scales, N, K);
+    return RLIS_LAUNCH_CHECK();
+}

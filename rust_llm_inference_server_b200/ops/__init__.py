@@ -2385,3 +2385,6 @@ def nll_rows(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
                               logits.stride(0), _stream()), "nll_rows")
     _count("nll_rows")
     return out
+
+
+from .blocks import BlockMatrix, BlockRows, linear_blocks, quantize_matrix, quantize_rows  # noqa: E402,F401  (at the end: it takes helpers of this file)
