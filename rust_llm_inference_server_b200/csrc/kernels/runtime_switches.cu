@@ -64,9 +64,10 @@ extern "C" int* rlis_attention_prefill_tc_error_addr(void);
 extern "C" int* rlis_attention_decode_error_addr(void);
 extern "C" int* rlis_attention_difference_decode_error_addr(void);
 extern "C" int* rlis_gemm_f32_split_error_addr(void);
+extern "C" int* rlis_blocks_gemm_error_addr(void);
 
 namespace {
-constexpr int kWords = 6;
+constexpr int kWords = 7;
 struct ErrorWords { int* w[kWords]; };
 
 __global__ void take_errors_kernel(ErrorWords words, int* __restrict__ out) {
@@ -89,7 +90,8 @@ extern "C" int rlis_take_errors(int* out, cudaStream_t stream) {
     if (!g_words_known[dev]) {
         ErrorWords w = {{rlis_gemm_tcgen05_error_addr(), rlis_stream_gemm_error_addr(),
                          rlis_attention_prefill_tc_error_addr(), rlis_attention_decode_error_addr(),
-                         rlis_attention_difference_decode_error_addr(), rlis_gemm_f32_split_error_addr()}};
+                         rlis_attention_difference_decode_error_addr(), rlis_gemm_f32_split_error_addr(),
+                         rlis_blocks_gemm_error_addr()}};
         for (int i = 0; i < kWords; ++i)
             if (w.w[i] == nullptr) return RLIS_ERR_UNSUPPORTED;
         g_words[dev] = w;

@@ -1377,7 +1377,8 @@ def check_device_errors() -> None:
     """Raises if a bounded wait inside a kernel ever ran out on this device (the kernel then
     finished without its data; results since are not to be trusted).  Synchronises the device."""
     code = (lib().rlis_gemm_tcgen05_error() or lib().rlis_stream_gemm_error() or lib().rlis_attention_prefill_tc_error()
-            or lib().rlis_attention_decode_error() or lib().rlis_attention_difference_decode_error() or lib().rlis_gemm_f32_split_error())
+            or lib().rlis_attention_decode_error() or lib().rlis_attention_difference_decode_error() or lib().rlis_gemm_f32_split_error()
+            or lib().rlis_blocks_gemm_error())
     if code != 0:
         raise KernelError(f"a bounded mbarrier wait of a tcgen05 kernel ran out on the device (code {code})")
 

@@ -159,7 +159,7 @@ def lib():
             fn.argtypes = args
             fn.restype = c_int
         for name in ("rlis_gemm_tcgen05_error", "rlis_stream_gemm_error", "rlis_attention_prefill_tc_error",
-                     "rlis_attention_decode_error", "rlis_attention_difference_decode_error", "rlis_gemm_f32_split_error"):
+                     "rlis_attention_decode_error", "rlis_attention_difference_decode_error", "rlis_gemm_f32_split_error", "rlis_blocks_gemm_error"):
             fn = getattr(handle, name)
             fn.argtypes = []
             fn.restype = c_int
