@@ -27,13 +27,20 @@ constexpr int BG_THREADS = 384, BG_WARPS = 8;           // three groups of four 
 // Registers a thread: 168 at launch for every group; the epilogue's 128 sums a thread and two sets of loads want more, the first group gives them up.
 constexpr int BG_REGS_LAUNCH = 168, BG_REGS_FIRST = 56, BG_REGS_EPILOGUE = 224;
 static_assert(BG_REGS_FIRST + 2 * BG_REGS_EPILOGUE <= 3 * BG_REGS_LAUNCH && BG_THREADS * BG_REGS_LAUNCH <= 65536, "a split above what the launch holds waits for good");
-constexpr int BG_TURN = 32 * 128;                       // bytes in which an epilogue warp turns 128 bytes of its 32 rows
-constexpr int BG_MAX_STAGES = 8, BG_MAX_BUFFERS = 4;
+constexpr int BG_MAX_STAGES = 6, BG_MAX_BUFFERS = 4;
+constexpr int BG_STAGING = 8192;                        // bytes of results that an epilogue warp keeps for its stores at most
 
 template <int BN> __host__ __device__ constexpr int bg_stage_bytes() { return BG_A_BYTES + BN / 2 * QB; }
-template <int BN> __host__ __device__ constexpr int bg_stages() { return BN == 256 ? 6 : BN == 192 ? 6 : 8; }
+template <int BN> __host__ __device__ constexpr int bg_stages() { return BN == 128 ? 6 : 5; }
 template <int BN> __host__ __device__ constexpr int bg_buffers() { return BN == 128 ? 4 : 2; }
-template <int BN> constexpr size_t bg_smem() { return (size_t)bg_stages<BN>() * bg_stage_bytes<BN>() + BG_WARPS * BG_TURN + 1024 /* alignment */ + 256; }
+// Columns that one store takes: 128 bytes of a row, or 64 where a warp's 96 columns are no multiple of that.
+template <int BN, typename OutT> __host__ __device__ constexpr int bg_store_cols() { return BN == 192 ? 32 : 128 / (int)sizeof(OutT); }
+template <int BN, typename OutT> __host__ __device__ constexpr int bg_staging() {
+    return BN / 2 * 32 * (int)sizeof(OutT) < BG_STAGING ? BN / 2 * 32 * (int)sizeof(OutT) : BG_STAGING;
+}
+template <int BN, typename OutT> constexpr size_t bg_smem() {
+    return (size_t)bg_stages<BN>() * bg_stage_bytes<BN>() + BG_WARPS * bg_staging<BN, OutT>() + 1024 /* alignment */ + 256;
+}
 
 struct BgCtrl {
     uint64_t full[BG_MAX_STAGES];           // CTA 0's: both CTAs' bytes of a stage have arrived
@@ -94,18 +101,24 @@ __device__ __forceinline__ void bg_commit_pair(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(smem_u32(bar)), "h"(both) : "memory");
 }
+// (Relaxed: what it hands over is tensor memory, whose loads have been waited for and fenced; a release would also wait for the next block's scales, which are on
+// their way from memory: 1,050 to 1,300 cycles a block.)
 __device__ __forceinline__ void bg_arrive_cluster(uint32_t bar_cluster_addr) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster_addr) : "memory");
 }
 
-// Sixteen columns of a lane's row without the wait: the registers may be read only after tmem_ld_wait().
-__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
+// 32 columns of a lane's row; the registers pass through the statements behind the wait, so that nothing that reads them is moved ahead of it.
+__device__ __forceinline__ void tmem_ld32_pinned(uint32_t taddr, uint32_t (&r)[32]) {
+    tmem_ld32(taddr, r);
+#pragma unroll
+    for (int i = 0; i < 32; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
+}
+__device__ __forceinline__ void tmem_ld16_pinned(uint32_t taddr, uint32_t (&r)[16]) {
+    tmem_ld16(taddr, r);
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+        asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]), "+r"(r[i + 6]), "+r"(r[i + 7]));
 }
 // Two sums at once: acc += s * r.
 __device__ __forceinline__ void fma2(unsigned long long& acc, uint32_t r0, uint32_t r1, unsigned long long s2) {
@@ -124,16 +137,18 @@ __device__ __forceinline__ float2 two_of(unsigned long long v) {
     return make_float2(__uint_as_float(a), __uint_as_float(b));
 }
 
-// 128 bytes of each of a warp's 32 rows (64 bfloat16 or 32 float32 sums of columns col .., a row a lane), by way of shared memory: rows in 16-byte pieces whose
-// places are swapped by the row, so that neither side meets in a bank, and an instruction writes the 128 bytes of four rows.
-template <typename OutT> constexpr int BG_STORE = 128 / (int)sizeof(OutT);
-template <typename OutT>
-__device__ __forceinline__ void store_turned(const unsigned long long* acc, uint4* turn, OutT* __restrict__ y, int row0, int col, int M, int end, int N, bool aligned) {
-    constexpr int PER = 16 / (int)sizeof(OutT);             // values in a piece
+// COLS sums of each of a warp's 32 rows (a row a lane) on their way out, in the layout that a bulk tensor copy of 32 rows reads: rows of 128 bytes in 16-byte pieces,
+// piece c of row r at c ^ (r % 8), or rows of 64 bytes, piece c at c ^ (r / 2 % 4); a quarter of a warp's lanes meet in no bank either way.
+template <int COLS, typename OutT>
+__device__ __forceinline__ int staged_piece(int row, int piece) {
+    if constexpr (COLS * sizeof(OutT) == 128) return row * 8 + (piece ^ (row & 7));
+    else return row * 4 + (piece ^ ((row >> 1) & 3));
+}
+template <int COLS, typename OutT>
+__device__ __forceinline__ void stage_sums(const unsigned long long* acc, uint4* to) {
     const int lane = threadIdx.x & 31;
-    __syncwarp();
 #pragma unroll
-    for (int v = 0; v < 8; ++v) {
+    for (int v = 0; v < COLS * (int)sizeof(OutT) / 16; ++v) {
         uint4 pk;
         if constexpr (sizeof(OutT) == 2) {
             const float2 a = two_of(acc[4 * v]), b = two_of(acc[4 * v + 1]), c = two_of(acc[4 * v + 2]), d = two_of(acc[4 * v + 3]);
@@ -142,38 +157,37 @@ __device__ __forceinline__ void store_turned(const unsigned long long* acc, uint
             const float2 a = two_of(acc[2 * v]), b = two_of(acc[2 * v + 1]);
             pk = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
         }
-        turn[lane * 8 + (v ^ (lane & 7))] = pk;
+        to[staged_piece<COLS, OutT>(lane, v)] = pk;
     }
-    __syncwarp();
-    if (aligned) {
-        const int piece = lane & 7, at = col + piece * PER;
+}
+// The same for results whose rows start anywhere: value by value.
+template <int COLS, typename OutT>
+__device__ __forceinline__ void store_staged(const uint4* from, OutT* __restrict__ y, int row0, int col, int M, int N) {
+    constexpr int PER = 16 / (int)sizeof(OutT);
+    const int lane = threadIdx.x & 31;
+    for (int r = 0; r < 32 && row0 + r < M; ++r)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int lr = j * 4 + (lane >> 3);
-            if (row0 + lr < M && at < end) *reinterpret_cast<uint4*>(y + (size_t)(row0 + lr) * N + at) = turn[lr * 8 + (piece ^ (lr & 7))];
-        }
-    } else {
-        // rows that start anywhere: value by value
-        for (int lr = 0; lr < 32 && row0 + lr < M; ++lr)
-            for (int c = lane; c < BG_STORE<OutT> && col + c < end; c += 32)
-                y[(size_t)(row0 + lr) * N + col + c] = reinterpret_cast<const OutT*>(turn)[(lr * 8 + ((c / PER) ^ (lr & 7))) * PER + c % PER];
-    }
+        for (int c = lane; c < COLS; c += 32)
+            if (col + c < N) y[(size_t)(row0 + r) * N + col + c] = reinterpret_cast<const OutT*>(from)[staged_piece<COLS, OutT>(r, c / PER) * PER + c % PER];
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
 }
 
 // Persistent: pair p works on tiles p, p + pairs, ...; tile t -> (n tile t / m_tiles, m tile t % m_tiles), so that the pairs that run together share a few
 // rows of w and all of x in L2.
 template <int BN, typename OutT>
 __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
-                                                                 const float* __restrict__ sx, const float* __restrict__ sw, OutT* __restrict__ y, int M, int N,
-                                                                 int k_blocks, int m_tiles, int num_tiles) {
+                                                                    const __grid_constant__ CUtensorMap map_y, const float* __restrict__ sx,
+                                                                    const float* __restrict__ sw, OutT* __restrict__ y, int M, int N, int k_blocks, int m_tiles,
+                                                                    int num_tiles, int bulk_stores, int early) {
     constexpr int STAGES = bg_stages<BN>(), BUFFERS = bg_buffers<BN>(), B_BYTES = BN / 2 * QB, HALF = BN / 2;
     constexpr uint32_t IDESC = idesc_e4m3(2 * BG_M, BN);
-    pdl_wait();
     extern __shared__ unsigned char bg_smem_raw[];
     // the same offset in both CTAs (their dynamic arrays start at the same address): the instruction reads both CTAs' tiles through one descriptor
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(bg_smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *a_tiles = base, *b_tiles = base + STAGES * BG_A_BYTES, *turns = b_tiles + STAGES * B_BYTES;
-    BgCtrl* ctrl = reinterpret_cast<BgCtrl*>(turns + BG_WARPS * BG_TURN);
+    unsigned char *a_tiles = base, *b_tiles = base + STAGES * BG_A_BYTES, *staging = b_tiles + STAGES * B_BYTES;
+    BgCtrl* ctrl = reinterpret_cast<BgCtrl*>(staging + BG_WARPS * bg_staging<BN, OutT>());
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = bg_cta_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -204,16 +218,22 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(BG_REGS_FIRST));
         if (warp == 0) {
             if (lane == 0) {
+                // the first stages' tiles of w before the kernel before this one has finished, where the caller says that it does not write them
+                const int first = early ? min(STAGES, k_blocks) : 0;
+                auto ask_w = [&](int s, int n0, int kb) {
+                    if (rank == 0) bar_expect_tx(&ctrl->full[s], 2 * (BG_A_BYTES + B_BYTES));
+                    bg_load_pair(b_tiles + s * B_BYTES, &map_w, kb * QB, n0 + (int)rank * HALF, bg_in_cta(&ctrl->full[s], 0));
+                };
+                for (int kb = 0; kb < first; ++kb) ask_w(kb, (pair / m_tiles) * BN, kb);
+                pdl_wait();
                 int it = 0;
                 for (int tile = pair; tile < num_tiles && !ctrl->abort; tile += pairs) {
                     const int n0 = (tile / m_tiles) * BN, m0 = (tile % m_tiles) * 2 * BG_M;
                     for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                         const int s = it % STAGES;
                         if (it >= STAGES && !bar_wait(&ctrl->empty[s], ((it / STAGES) - 1) & 1, &ctrl->abort)) break;
-                        const uint32_t full0 = bg_in_cta(&ctrl->full[s], 0);
-                        if (rank == 0) bar_expect_tx(&ctrl->full[s], 2 * (BG_A_BYTES + B_BYTES));
-                        bg_load_pair(a_tiles + s * BG_A_BYTES, &map_x, kb * QB, m0 + (int)rank * BG_M, full0);
-                        bg_load_pair(b_tiles + s * B_BYTES, &map_w, kb * QB, n0 + (int)rank * HALF, full0);
+                        if (it >= first) ask_w(s, n0, kb);
+                        bg_load_pair(a_tiles + s * BG_A_BYTES, &map_x, kb * QB, m0 + (int)rank * BG_M, bg_in_cta(&ctrl->full[s], 0));
                     }
                 }
             }
@@ -225,11 +245,11 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
                 for (int tile = pair; tile < num_tiles && fine; tile += pairs) {
                     for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                         const int s = it % STAGES, buf = it % BUFFERS;
-                        if (it >= BUFFERS && !bar_wait_warp(&ctrl->acc_empty[buf], ((it / BUFFERS) - 1) & 1, &ctrl->abort)) { fine = false; break; }
                         if (!bar_wait_warp(&ctrl->full[s], (it / STAGES) & 1, &ctrl->abort)) { fine = false; break; }
+                        const uint64_t adesc = smem_desc_sw128(a_tiles + s * BG_A_BYTES), bdesc = smem_desc_sw128(b_tiles + s * B_BYTES);
+                        if (it >= BUFFERS && !bar_wait_warp(&ctrl->acc_empty[buf], ((it / BUFFERS) - 1) & 1, &ctrl->abort)) { fine = false; break; }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         if (elect_one()) {
-                            const uint64_t adesc = smem_desc_sw128(a_tiles + s * BG_A_BYTES), bdesc = smem_desc_sw128(b_tiles + s * B_BYTES);
     #pragma unroll
                             for (int k = 0; k < QB / 32; ++k)          // 32 codes further along the swizzled row
                                 umma_e4m3_pair(tmem_base + (uint32_t)(buf * BN), adesc + (uint64_t)(k * 32 >> 4), bdesc + (uint64_t)(k * 32 >> 4), IDESC, k != 0 ? 1u : 0u);
@@ -243,11 +263,13 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BG_REGS_EPILOGUE));
+        pdl_wait();
         // epilogue: warp w may touch TMEM lanes 32 * (w % 4) .. + 31; two warps share them, half of the columns each
         const int q = warp & 3, half = (warp - 4) / 4;
         const int n_blocks = (N + QB - 1) / QB;
-        const bool aligned = (N * (int)sizeof(OutT)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
-        uint4* turn = reinterpret_cast<uint4*>(turns + (warp - 4) * BG_TURN);
+        constexpr int COLS = bg_store_cols<BN, OutT>(), STORE_BYTES = COLS * 32 * (int)sizeof(OutT), STAGED = bg_staging<BN, OutT>() / STORE_BYTES;
+        unsigned char* mine = staging + (warp - 4) * bg_staging<BN, OutT>();
+        const uint32_t released = bg_in_cta(&ctrl->acc_empty[0], 0);
         int it = 0;
         bool fine = true;
         for (int tile = pair; tile < num_tiles && fine; tile += pairs) {
@@ -259,48 +281,67 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
             unsigned long long acc[HALF / 2];
 #pragma unroll
             for (int i = 0; i < HALF / 2; ++i) acc[i] = 0ull;
-            float a = *px, b = *pw, b1 = BN == 192 ? *pw1 : 0.f;           // the next block's scales are asked for before this one's sums are awaited
+            // the scales of two blocks ahead are on their way: a block takes less time than a load from memory
+            float a[2], b[2], b1[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int kb = min(i, k_blocks - 1);
+                a[i] = px[(size_t)kb * M];
+                b[i] = pw[kb];
+                b1[i] = BN == 192 ? pw1[kb] : 0.f;
+            }
+#pragma unroll 2
             for (int kb = 0; kb < k_blocks; ++kb, ++it) {
                 const int buf = it % BUFFERS;
-                const unsigned long long s2 = twice(a * b), s2b = BN == 192 ? twice(a * b1) : 0ull;
-                if (kb + 1 < k_blocks) {
-                    a = px[(size_t)(kb + 1) * M];
-                    b = pw[kb + 1];
-                    if (BN == 192) b1 = pw1[kb + 1];
+                const unsigned long long s2 = twice(a[kb & 1] * b[kb & 1]), s2b = BN == 192 ? twice(a[kb & 1] * b1[kb & 1]) : 0ull;
+                if (kb + 2 < k_blocks) {
+                    a[kb & 1] = px[(size_t)(kb + 2) * M];
+                    b[kb & 1] = pw[kb + 2];
+                    if (BN == 192) b1[kb & 1] = pw1[kb + 2];
                 }
                 if (!bar_wait_warp(&ctrl->acc_full[buf], (it / BUFFERS) & 1, &ctrl->abort)) { fine = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const uint32_t from = tmem_base + (uint32_t)(buf * BN + half * HALF) + ((uint32_t)(q * 32) << 16);
-                uint32_t r[2][16];
-                tmem_ld16_nowait(from, r[0]);
 #pragma unroll
-                for (int c = 0; c < HALF / 16; ++c) {
-                    tmem_ld_wait();
-                    if (c + 1 < HALF / 16) tmem_ld16_nowait(from + (uint32_t)((c + 1) * 16), r[(c + 1) & 1]);
-                    const unsigned long long s = BN == 192 && c * 16 >= border ? s2b : s2;
+                for (int c = 0; c < HALF / 32; ++c) {
+                    uint32_t r[32];
+                    tmem_ld32_pinned(from + (uint32_t)(c * 32), r);
+                    const unsigned long long s = BN == 192 && c * 32 >= border ? s2b : s2;
+                    if (c + 1 == HALF / 32) {
+                        // this warp has read its lanes of the accumulator: CTA 0's product warp may write it again
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) bg_arrive_cluster(released + (uint32_t)buf * 8u);
+                    }
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) fma2(acc[c * 8 + i], r[c & 1][2 * i], r[c & 1][2 * i + 1], s);
+                    for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], r[2 * i], r[2 * i + 1], s);
                 }
-                // this warp has read its lanes of the accumulator: CTA 0's product warp may write it again
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) bg_arrive_cluster(bg_in_cta(&ctrl->acc_empty[buf], 0));
             }
             if (!fine) break;
 #pragma unroll
-            for (int c = 0; c < HALF; c += BG_STORE<OutT>) {
-                if constexpr (HALF % BG_STORE<OutT> != 0) {                // bfloat16, 96 columns: 64 and 32
-                    if (c + BG_STORE<OutT> > HALF) {
-                        unsigned long long rest[BG_STORE<OutT> / 2];
-#pragma unroll
-                        for (int i = 0; i < BG_STORE<OutT> / 2; ++i) rest[i] = c / 2 + i < HALF / 2 ? acc[(c / 2 + i) % (HALF / 2)] : 0ull;
-                        store_turned<OutT>(rest, turn, y, row0, col0 + c, M, min(N, col0 + HALF), N, aligned);
-                        continue;
-                    }
+            for (int c = 0; c < HALF / COLS; ++c) {
+                if (c % STAGED == 0) {
+                    // what the last stores read has to be read before it is written over
+                    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+                    __syncwarp();
                 }
-                store_turned<OutT>(acc + c / 2, turn, y, row0, col0 + c, M, N, N, aligned);
+                unsigned char* to = mine + (c % STAGED) * STORE_BYTES;
+                stage_sums<COLS, OutT>(acc + c * (COLS / 2), reinterpret_cast<uint4*>(to));
+                if (bulk_stores) {
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0 && row0 < M && col0 + c * COLS < N) {
+                        tma_store_2d(&map_y, to, col0 + c * COLS, row0);
+                        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    }
+                } else {
+                    __syncwarp();
+                    store_staged<COLS, OutT>(reinterpret_cast<const uint4*>(to), y, row0, col0 + c * COLS, M, N);
+                    __syncwarp();
+                }
             }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     // nobody leaves, and no tensor memory is freed, while the other CTA may still use this one's
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -313,41 +354,94 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
     pdl_trigger();
 }
 
+// The result [M, N] as a tensor map with boxes of 32 rows x cols columns, in the layout of stage_sums.
+template <typename OutT> bool make_result_map(CUtensorMap* map, void* y, int M, int N, int cols) {
+    EncodeTiledFn fn = encode_fn();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+    const cuuint64_t strides[1] = {(cuuint64_t)N * sizeof(OutT)};
+    const cuuint32_t box[2] = {(cuuint32_t)cols, 32u};
+    const cuuint32_t estr[2] = {1, 1};
+    return fn(map, sizeof(OutT) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              cols * sizeof(OutT) == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int BN, typename OutT>
-int launch_blocks_gemm(const void* x, long long ldx, const float* sx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int sms,
+int launch_blocks_gemm(const void* x, long long ldx, const float* sx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int early, int sms,
                        cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed{0};
-    const cudaError_t e = rlis_allow_smem(blocks_gemm_kernel<BN, OutT>, (int)bg_smem<BN>(), allowed);
+    const cudaError_t e = rlis_allow_smem(blocks_gemm_kernel<BN, OutT>, (int)bg_smem<BN, OutT>(), allowed);
     if (e != cudaSuccess) return (int)e;
-    CUtensorMap map_x, map_w;
+    CUtensorMap map_x, map_w, map_y;
     if (!make_code_map(&map_x, x, M, K, BG_M, ldx) || !make_code_map(&map_w, w, N, K, BN / 2, ldw)) return RLIS_ERR_UNSUPPORTED;
+    // rows of the result that start at multiples of 16 bytes leave by bulk tensor copies
+    const bool bulk = ((long long)N * (int)sizeof(OutT)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+    map_y = map_x;
+    if (bulk && !make_result_map<OutT>(&map_y, y, M, N, bg_store_cols<BN, OutT>())) return RLIS_ERR_UNSUPPORTED;
     const int m_tiles = (M + 2 * BG_M - 1) / (2 * BG_M), num_tiles = m_tiles * ((N + BN - 1) / BN), pairs = num_tiles < sms / 2 ? num_tiles : sms / 2;
-    rlis_launch_cluster(blocks_gemm_kernel<BN, OutT>, dim3((unsigned)(2 * pairs)), dim3(BG_THREADS), bg_smem<BN>(), stream, dim3(2, 1, 1), map_x, map_w, sx, sw, (OutT*)y,
-                        M, N, (K + QB - 1) / QB, m_tiles, num_tiles);
+    rlis_launch_cluster(blocks_gemm_kernel<BN, OutT>, dim3((unsigned)(2 * pairs)), dim3(BG_THREADS), bg_smem<BN, OutT>(), stream, dim3(2, 1, 1), map_x, map_w, map_y, sx,
+                        sw, (OutT*)y, M, N, (K + QB - 1) / QB, m_tiles, num_tiles, bulk ? 1 : 0, early);
     return RLIS_LAUNCH_CHECK();
 }
 }  // namespace
+
+#include "blocks_few.cuh"
 
 // 0 if no bounded wait of these products ever ran out on the current device.
 extern "C" int rlis_blocks_gemm_error(void) { return tc::read_error_word(); }
 extern "C" int* rlis_blocks_gemm_error_addr(void) { return tc::error_word_addr(); }
 
-// x [M, K] (rows ldx bytes apart), sx [ceil(K / 128), M]; w [N, K] (rows ldw bytes apart), sw [ceil(N / 128), ceil(K / 128)]; y [M, N].  Codes on 16-byte
-// boundaries, their rows multiples of 16 bytes apart.
-extern "C" int rlis_blocks_gemm(const void* x, long long ldx, const float* sx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int out_dtype,
-                                cudaStream_t stream) {
-    if (M <= 0 || N <= 0) return 0;
-    if (K <= 0 || (out_dtype != RLIS_F32 && out_dtype != RLIS_BF16) || ldx < K || ldw < K || ldx % 16 != 0 || ldw % 16 != 0 ||
-        ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(w)) & 15) != 0)
-        return RLIS_ERR_UNSUPPORTED;
+namespace {
+int sms_of_device() {
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+constexpr int FEW_ROWS = 128;           // rows up to which a product is a stream of w
+bool codes_fit(const void* p, long long ld, int K) { return ld >= K && ld % 16 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+}  // namespace
+
+// x [M, K] (rows ldx bytes apart), sx [ceil(K / 128), M]; w [N, K] (rows ldw bytes apart), sw [ceil(N / 128), ceil(K / 128)]; y [M, N].  Codes on 16-byte
+// boundaries, their rows multiples of 16 bytes apart.  early: no kernel still in flight writes w, so that its first tiles may be read before the kernel before
+// this one has finished.
+extern "C" int rlis_blocks_gemm(const void* x, long long ldx, const float* sx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int out_dtype,
+                                int early, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (K <= 0 || (out_dtype != RLIS_F32 && out_dtype != RLIS_BF16) || !codes_fit(x, ldx, K) || !codes_fit(w, ldw, K)) return RLIS_ERR_UNSUPPORTED;
+    const int sms = sms_of_device();
+    const bool f32 = out_dtype == RLIS_F32;
+    if (M <= FEW_ROWS) {
+        const FewPlan p = few_plan(N, (K + QB - 1) / QB, sms);
+        const PlainRows none{nullptr, 0, 0};
+#define RLIS_BF(NT) (f32 ? launch_blocks_few<NT, 0, float>(none, x, ldx, sx, w, ldw, sw, y, M, N, K, early, p, stream) \
+                         : launch_blocks_few<NT, 0, bf16>(none, x, ldx, sx, w, ldw, sw, y, M, N, K, early, p, stream))
+        return M <= 16 ? RLIS_BF(16) : M <= 32 ? RLIS_BF(32) : M <= 64 ? RLIS_BF(64) : RLIS_BF(128);
+#undef RLIS_BF
+    }
     // The width of a tile: the one whose rounds over the pairs of SMs come to the fewest columns (a round of narrow tiles is shorter), the widest of equals.
     const long long m_tiles = (M + 2 * BG_M - 1) / (2 * BG_M);
     auto columns = [&](int bn) { const long long tiles = m_tiles * ((N + bn - 1) / bn); return (tiles + sms / 2 - 1) / (sms / 2) * bn; };
     const int bn = columns(256) <= columns(192) && columns(256) <= columns(128) ? 256 : columns(192) <= columns(128) ? 192 : 128;
-    const bool f32 = out_dtype == RLIS_F32;
-#define RLIS_BG(BN) (f32 ? launch_blocks_gemm<BN, float>(x, ldx, sx, w, ldw, sw, y, M, N, K, sms, stream) : launch_blocks_gemm<BN, bf16>(x, ldx, sx, w, ldw, sw, y, M, N, K, sms, stream))
+#define RLIS_BG(BN) (f32 ? launch_blocks_gemm<BN, float>(x, ldx, sx, w, ldw, sw, y, M, N, K, early, sms, stream) \
+                         : launch_blocks_gemm<BN, bf16>(x, ldx, sx, w, ldw, sw, y, M, N, K, early, sms, stream))
     return bn == 256 ? RLIS_BG(256) : bn == 192 ? RLIS_BG(192) : RLIS_BG(128);
 #undef RLIS_BG
+}
+
+// The same for up to 16 plain rows x [M, K] of `dtype` (ldx elements apart), which the product puts into blocks itself.  RLIS_ERR_UNSUPPORTED where a CTA's part of
+// them does not fit its shared memory.
+extern "C" int rlis_blocks_gemm_rows(const void* x, long long ldx, int dtype, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int out_dtype,
+                                     int early, cudaStream_t stream) {
+    if (M <= 0 || N <= 0) return 0;
+    if (M > 16 || K <= 0 || (out_dtype != RLIS_F32 && out_dtype != RLIS_BF16) || (dtype != RLIS_F32 && dtype != RLIS_BF16) || !codes_fit(w, ldw, K)) return RLIS_ERR_UNSUPPORTED;
+    const FewPlan p = few_plan(N, (K + QB - 1) / QB, sms_of_device());
+    if (p.per > BF_FUSED_BLOCKS) return RLIS_ERR_UNSUPPORTED;
+    const int size = dtype == RLIS_F32 ? 4 : 2;
+    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (M == 1 || (ldx * size) % 16 == 0), f32 = out_dtype == RLIS_F32;
+    const PlainRows rows{x, ldx, K};
+#define RLIS_BF(HOW) (f32 ? launch_blocks_few<16, HOW, float>(rows, nullptr, 0, nullptr, w, ldw, sw, y, M, N, K, early, p, stream) \
+                          : launch_blocks_few<16, HOW, bf16>(rows, nullptr, 0, nullptr, w, ldw, sw, y, M, N, K, early, p, stream))
+    return dtype == RLIS_BF16 ? (vec ? RLIS_BF(3) : RLIS_BF(1)) : (vec ? RLIS_BF(4) : RLIS_BF(2));
+#undef RLIS_BF
 }

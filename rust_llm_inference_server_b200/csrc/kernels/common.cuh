@@ -148,6 +148,19 @@ static inline cudaError_t rlis_allow_smem(void (*kernel)(KArgs...), int bytes, s
     return e;
 }
 
+// Clusters of more than eight CTAs, allowed in the same way.
+template <typename... KArgs>
+static inline cudaError_t rlis_allow_wide_cluster(void (*kernel)(KArgs...), std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+    if (bit & done.load(std::memory_order_acquire)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+
 // The same for a grid of thread-block clusters of `cluster` CTAs.
 template <typename... KArgs, typename... Args>
 static inline void rlis_launch_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,

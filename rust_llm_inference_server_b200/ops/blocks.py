@@ -13,6 +13,7 @@ from .library import KernelError, check, lib
 
 BLOCK = 128                     # a block's edge
 CODES = torch.float8_e4m3fn
+FUSED_ROWS = 16                 # rows up to which a product puts them into blocks itself
 
 _device = torch._C._cuda_getDevice
 
@@ -111,10 +112,11 @@ def quantize_matrix(w: torch.Tensor) -> BlockMatrix:
     return matrix
 
 
-def linear_blocks(x, w: BlockMatrix, out_dtype=None) -> torch.Tensor:
+def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> torch.Tensor:
     """y = x @ w^T for a weight in blocks.  x [T, K]: plain rows (bfloat16 or float32; may be a column slice of wider rows), which are put into blocks as
     `quantize_rows` does, or BlockRows, for rows that several products read.  Every block of 128 k is summed on its own, scaled by both scales and added in
-    float32; the result is rounded once, to `out_dtype` (bfloat16 or float32; None: x's, bfloat16 for BlockRows)."""
+    float32; the result is rounded once, to `out_dtype` (bfloat16 or float32; None: x's, bfloat16 for BlockRows).
+    `early`: w is a weight that no kernel still in flight writes, so that its first tiles may be asked for before the kernels before have finished."""
     if not isinstance(w, BlockMatrix) or w.values.dim() != 2:
         raise KernelError("linear_blocks: expected a BlockMatrix [N, K]")
     plain = not isinstance(x, BlockRows)
@@ -126,12 +128,20 @@ def linear_blocks(x, w: BlockMatrix, out_dtype=None) -> torch.Tensor:
     out_code = _code(out_dtype or (x.dtype if plain else torch.bfloat16))
     if w.values.get_device() != _device():
         with torch.cuda.device(w.device):
-            return linear_blocks(x, w, out_dtype)
-    if plain:
-        x = quantize_rows(x)
-    T = x.values.shape[0]
+            return linear_blocks(x, w, out_dtype, early=early)
+    T = x.shape[0]
     out = torch.empty((T, N), dtype=torch.bfloat16 if out_code else torch.float32, device=w.values.device)
+    if plain and T <= FUSED_ROWS:
+        code = lib().rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), _code(x.dtype), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K, out_code,
+                                           int(early), _stream())
+        if code != -1:              # (a matrix of so many features and k that a CTA has no room for its part of the rows)
+            check(code, "linear_blocks")
+            _count("linear_blocks.rows")
+            return out
+    if plain:
+        # (the kernel that quantises starts the next one when all kernels before itself have finished: none but itself is in flight, and it does not write w)
+        x, early = quantize_rows(x), True
     check(lib().rlis_blocks_gemm(x.values.data_ptr(), x.stride, x.scales.data_ptr(), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
-                                 out_code, _stream()), "linear_blocks")
+                                 out_code, int(early), _stream()), "linear_blocks")
     _count("linear_blocks")
     return out
