@@ -2,35 +2,32 @@
 //
 // The weights are the M side of the instruction: a CTA owns 128 features and a range of the blocks of k; a block of w (128 x 128 codes, 16 KB) arrives by one
 // bulk tensor copy into a ring of stages, with the NT x 128 tile of x (NT: rows rounded up to 16, 32, 64 or 128).  Warp 0 asks for the tiles, warp 1 issues
-// tcgen05.mma (128 x NT x 32, four a block) into one of several accumulators of NT columns, warps 2-5 take a block's sums from there (a lane a feature, a
-// column a row of x), multiply them by sx[row] sw and add them in registers, where a block's products of scales lie in shared memory.
-// w has one scale for the CTA's 128 features and a block, so a thread needs no scale of its own.
+// tcgen05.mma (128 x NT x 32, four a block) into one of four accumulators of NT columns, the other warps take a block's sums from there (a lane a feature, a
+// column a row of x; groups of four warps share the columns, since the way from a block's sums to the next is a chain of waits, as long as a block of w takes
+// to arrive), multiply them by sx[row] sw and add them in registers.  w has one scale for the CTA's 128 features and a block; the products of scales lie in
+// shared memory.
 //
 // Matrices with few features would fill few SMs, so k is split over the CTAs of a thread-block cluster (any number up to 16).  Their sums go to shared memory, and
 // after a cluster barrier CTA r adds the rows r, r + splits, .. of all CTAs in the order of the splits: the result does not depend on timing.  The number of
-// splits depends on N and K alone, so a row has the same bits whatever other rows there are, up to 128.
-//
-// FUSED (up to 16 rows, not yet in blocks): the CTA puts its part of x into blocks itself, as quantize_rows does, straight into the swizzled layout that the
-// instruction reads, while its first tiles of w are on their way; a launch and a round trip of the codes less.
+// splits depends on N and K alone up to 64 rows (few_splits), so a row has the same bits whatever other rows there are.
 // (Included by blocks_gemm.cu, whose error word it shares.)
 #pragma once
 
 namespace {
 constexpr int BF_F = 128;                               // features of a CTA
-constexpr int BF_THREADS = 192;
 constexpr int BF_W_BYTES = BF_F * QB;
-constexpr int BF_MAX_STAGES = 6, BF_MAX_BUFFERS = 4, BF_MAX_SPLITS = 16;
+constexpr int BF_MAX_STAGES = 6, BF_BUFFERS = 4, BF_MAX_SPLITS = 16;
 constexpr int BF_SCALES = 4096;                         // products of scales that shared memory holds at a time
-constexpr int BF_FUSED_BLOCKS = 32;                     // blocks of k up to which a CTA holds its rows of x itself
 
-template <int NT> __host__ __device__ constexpr int bf_stages() { return NT == 16 ? 6 : NT == 32 ? 5 : NT == 64 ? 4 : 3; }
-template <int NT> __host__ __device__ constexpr int bf_buffers() { return NT <= 32 ? 4 : 2; }
+template <int NT> __host__ __device__ constexpr int bf_groups() { return NT == 128 ? 4 : NT == 16 ? 1 : 2; }      // of four warps, NT / groups columns each
+template <int NT> __host__ __device__ constexpr int bf_threads() { return 64 + 128 * bf_groups<NT>(); }
+template <int NT> __host__ __device__ constexpr int bf_ctas() { return NT == 128 ? 1 : 2; }                       // that fit an SM
 
 struct BfCtrl {
     uint64_t full[BF_MAX_STAGES];
     uint64_t empty[BF_MAX_STAGES];
-    uint64_t acc_full[BF_MAX_BUFFERS];
-    uint64_t acc_empty[BF_MAX_BUFFERS];
+    uint64_t acc_full[BF_BUFFERS];
+    uint64_t acc_empty[BF_BUFFERS];
     uint32_t tmem_base;
     int abort;
 };
@@ -47,61 +44,16 @@ __device__ __forceinline__ void umma_e4m3(uint32_t tmem_d, uint64_t adesc, uint6
         : "memory");
 }
 
-// The rows of x that a FUSED launch puts into blocks.
-struct PlainRows {
-    const void* x;
-    long long ld;
-    int K;
-};
-
-// This CTA's blocks kb0 .. kb1 of x's rows: codes into the tiles [block][16 rows of 128 bytes, 128-byte swizzle], scales times w's into sc [block][16].
-template <typename T, bool VEC>
-__device__ __forceinline__ void blocks_of_rows(const PlainRows& p, int M, int kb0, int n_kb, const float* __restrict__ sw, unsigned char* tiles, float* sc) {
-    constexpr int GROUPS = BF_THREADS / 16, AHEAD = 4;
-    const T* x = reinterpret_cast<const T*>(p.x);
-    const int group = threadIdx.x >> 4, lane = threadIdx.x & 15, total = M * n_kb;
-    for (int first = group; first - group < total; first += GROUPS * AHEAD) {          // (the same number of rounds for all: shuffles are whole warps')
-        float v[AHEAD][8];
-        int row[AHEAD], kb[AHEAD];
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int unit = first + u * GROUPS;
-            row[u] = unit < total ? unit / n_kb : -1;
-            kb[u] = unit < total ? unit - row[u] * n_kb : 0;
-            if (row[u] >= 0) {
-                load8<T, VEC>(x + row[u] * p.ld, (kb0 + kb[u]) * QB + lane * 8, p.K, v[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            unsigned amax = 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(v[u][i]));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-            if (row[u] < 0) continue;
-            const Coding c = coding_of(amax);
-            unsigned char* to = tiles + kb[u] * (16 * QB) + row[u] * QB + (((lane >> 1) ^ (row[u] & 7)) << 4) + (lane & 1) * 8;
-            *reinterpret_cast<uint2*>(to) = make_uint2(codes4(v[u], c), codes4(v[u] + 4, c));
-            if (lane == 0) sc[kb[u] * 16 + row[u]] = c.scale * sw[kb0 + kb[u]];
-        }
-    }
-}
-
-template <int NT, int FUSED /* 0: x in blocks; 1: bfloat16 rows, 2: float32; 3, 4: the same in vectors */, typename OutT>
-__global__ __launch_bounds__(BF_THREADS) void blocks_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const PlainRows rows,
-                                                                const float* __restrict__ sx, const float* __restrict__ sw, OutT* __restrict__ y, int M, int N,
-                                                                int k_blocks, int per, int n_stages, int early) {
-    static_assert(!FUSED || NT == 16, "rows that a CTA puts into blocks itself are few");
-    constexpr int X_BYTES = NT * QB, BUFFERS = bf_buffers<NT>();
-    constexpr uint32_t COLS = BUFFERS * NT, IDESC = idesc_e4m3(BF_F, NT);
+template <int NT, typename OutT>
+__global__ __launch_bounds__(bf_threads<NT>(), bf_ctas<NT>()) void blocks_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
+                                                                                     const float* __restrict__ sx, const float* __restrict__ sw, OutT* __restrict__ y, int M,
+                                                                                     int N, int k_blocks, int per, int n_stages, int early) {
+    constexpr int X_BYTES = NT * QB, GROUPS = bf_groups<NT>(), C = NT / GROUPS, TAKERS = 128 * GROUPS;
+    constexpr uint32_t COLS = BF_BUFFERS * NT, IDESC = idesc_e4m3(BF_F, NT);
     extern __shared__ unsigned char bf_smem_raw[];
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(bf_smem_raw) + 1023) & ~(uintptr_t)1023);
-    unsigned char *w_tiles = base, *x_tiles = base + n_stages * BF_W_BYTES;         // x: a tile a stage, or (FUSED) a tile a block
-    float* sc = reinterpret_cast<float*>(x_tiles + (FUSED ? per : n_stages) * X_BYTES);
+    unsigned char *w_tiles = base, *x_tiles = base + n_stages * BF_W_BYTES;
+    float* sc = reinterpret_cast<float*>(x_tiles + n_stages * X_BYTES);
     const int chunk = min(per, BF_SCALES / NT);                                       // blocks whose products of scales are held
     BfCtrl* ctrl = reinterpret_cast<BfCtrl*>(sc + chunk * NT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -115,9 +67,9 @@ __global__ __launch_bounds__(BF_THREADS) void blocks_few_kernel(const __grid_con
             bar_init(&ctrl->full[s], 1);
             bar_init(&ctrl->empty[s], 1);
         }
-        for (int i = 0; i < BUFFERS; ++i) {
+        for (int i = 0; i < BF_BUFFERS; ++i) {
             bar_init(&ctrl->acc_full[i], 1);
-            bar_init(&ctrl->acc_empty[i], 4);
+            bar_init(&ctrl->acc_empty[i], 4 * GROUPS);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
@@ -133,44 +85,33 @@ __global__ __launch_bounds__(BF_THREADS) void blocks_few_kernel(const __grid_con
 
     const int first = min(n_stages, n_kb);
     auto ask_w = [&](int s, int it) {
-        bar_expect_tx(&ctrl->full[s], BF_W_BYTES + (FUSED ? 0 : X_BYTES));
+        bar_expect_tx(&ctrl->full[s], BF_W_BYTES + X_BYTES);
         tma_load_2d(w_tiles + s * BF_W_BYTES, &map_w, (kb0 + it) * QB, n0, &ctrl->full[s]);
     };
-    if (threadIdx.x == 0 && early)
-        for (int it = 0; it < first; ++it) ask_w(it, it);
-    pdl_wait();
-    if (threadIdx.x == 0 && !early)
-        for (int it = 0; it < first; ++it) ask_w(it, it);
-    if constexpr (FUSED != 0) {
-        __syncwarp();
-        if constexpr (FUSED == 1 || FUSED == 3) blocks_of_rows<bf16, FUSED == 3>(rows, M, kb0, n_kb, my_sw, x_tiles, sc);
-        else blocks_of_rows<float, FUSED == 4>(rows, M, kb0, n_kb, my_sw, x_tiles, sc);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
-    }
-
-    unsigned long long acc[NT / 2];
+    // (128-byte rows of zeros where x has no row; every wait below that fails ends its loop, so that all threads come to the barriers at the end)
+    unsigned long long acc[C / 2];
     bool fine = true;
     if (warp == 0) {
         if (lane == 0) {
-            for (int it = 0; it < n_kb; ++it) {
-                const int s = it % n_stages;
-                if (it >= first) {
-                    if (!bar_wait(&ctrl->empty[s], ((it / n_stages) - 1) & 1, &ctrl->abort)) break;
-                    ask_w(s, it);
-                }
-                if (!FUSED) tma_load_2d(x_tiles + s * X_BYTES, &map_x, (kb0 + it) * QB, 0, &ctrl->full[s]);
+            if (early)
+                for (int it = 0; it < first; ++it) ask_w(it, it);
+            pdl_wait();
+            for (int it = 0, s = 0, phase = 1; it < n_kb; ++it) {
+                if (it >= first && !bar_wait(&ctrl->empty[s], phase, &ctrl->abort)) break;
+                if (it >= first || !early) ask_w(s, it);
+                tma_load_2d(x_tiles + s * X_BYTES, &map_x, (kb0 + it) * QB, 0, &ctrl->full[s]);
+                if (++s == n_stages) s = 0, phase ^= 1;
             }
             pdl_trigger();     // everything this CTA reads is asked for: the next kernel may start its own
         }
     } else if (warp == 1) {
         // the whole warp walks the loop and waits, and leaves it together; one lane issues
-        for (int it = 0; it < n_kb; ++it) {
-            const int s = it % n_stages, buf = it % BUFFERS;
-            if (!bar_wait_warp(&ctrl->full[s], (it / n_stages) & 1, &ctrl->abort)) break;
-            if (it >= BUFFERS && !bar_wait_warp(&ctrl->acc_empty[buf], ((it / BUFFERS) - 1) & 1, &ctrl->abort)) break;
+        for (int it = 0, s = 0, phase = 0; it < n_kb; ++it) {
+            const int buf = it % BF_BUFFERS;
+            if (!bar_wait_warp(&ctrl->full[s], phase, &ctrl->abort)) break;
+            const uint64_t adesc = smem_desc_sw128(w_tiles + s * BF_W_BYTES), bdesc = smem_desc_sw128(x_tiles + s * X_BYTES);
+            if (it >= BF_BUFFERS && !bar_wait_warp(&ctrl->acc_empty[buf], ((it / BF_BUFFERS) - 1) & 1, &ctrl->abort)) break;
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint64_t adesc = smem_desc_sw128(w_tiles + s * BF_W_BYTES), bdesc = smem_desc_sw128(x_tiles + (FUSED ? it : s) * X_BYTES);
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < QB / 32; ++k)          // 32 codes further along the swizzled row
@@ -179,56 +120,50 @@ __global__ __launch_bounds__(BF_THREADS) void blocks_few_kernel(const __grid_con
                 umma_commit(&ctrl->acc_full[buf]);
             }
             __syncwarp();
+            if (++s == n_stages) s = 0, phase ^= 1;
         }
     } else {
-        const int q = warp & 3, mine = (warp - 2) * 32 + lane;
+        pdl_wait();
+        const int q = warp & 3, group = (warp - 2) / 4, mine = (int)threadIdx.x - 64;
 #pragma unroll
-        for (int i = 0; i < NT / 2; ++i) acc[i] = 0ull;
-        for (int it = 0; it < n_kb; ++it) {
-            const int at = it % chunk;
-            if (!FUSED && at == 0) {
-                asm volatile("bar.sync 1, 128;" ::: "memory");         // the last chunk's have been read
-                const int n = min(chunk, n_kb - it) * NT;
-                for (int i = mine; i < n; i += 128) {
-                    const int kb = kb0 + it + i / NT, t = i % NT;
-                    sc[i] = t < M ? sx[(size_t)kb * M + t] * my_sw[kb] : 0.f;
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int i = 0; i < C / 2; ++i) acc[i] = 0ull;
+        for (int it0 = 0; it0 < n_kb; it0 += chunk) {
+            const int n = min(chunk, n_kb - it0);
+            asm volatile("bar.sync 1, %0;" ::"n"(TAKERS) : "memory");         // the last chunk's have been read
+            for (int i = mine; i < n * NT; i += TAKERS) {
+                const int kb = kb0 + it0 + i / NT, t = i % NT;
+                sc[i] = t < M ? sx[(size_t)kb * M + t] * my_sw[kb] : 0.f;
             }
-            const int buf = it % BUFFERS;
-            if (fine) fine = bar_wait_warp(&ctrl->acc_full[buf], (it / BUFFERS) & 1, &ctrl->abort);
-            if (!fine) continue;                                         // (to the barriers above, which all four warps meet at)
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t from = tmem_base + (uint32_t)(buf * NT) + ((uint32_t)(q * 32) << 16);
-            const ulonglong2* scale = reinterpret_cast<const ulonglong2*>(sc + at * NT);
-            constexpr int LW = NT < 32 ? NT : 32;
-#pragma unroll
-            for (int c = 0; c < NT / LW; ++c) {
-                uint32_t r[LW];
-                if constexpr (LW == 32) tmem_ld32_pinned(from + (uint32_t)(c * LW), r);
+            asm volatile("bar.sync 1, %0;" ::"n"(TAKERS) : "memory");
+            const ulonglong2* scale = reinterpret_cast<const ulonglong2*>(sc + group * C);
+            for (int i = 0; i < n && fine; ++i, scale += NT / 4) {
+                const int it = it0 + i, buf = it % BF_BUFFERS;
+                fine = bar_wait_warp(&ctrl->acc_full[buf], (it / BF_BUFFERS) & 1, &ctrl->abort);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t from = tmem_base + (uint32_t)(buf * NT + group * C) + ((uint32_t)(q * 32) << 16);
+                uint32_t r[C];
+                if constexpr (C == 32) tmem_ld32_pinned(from, r);
                 else tmem_ld16_pinned(from, r);
-                if (c + 1 == NT / LW) {
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                    __syncwarp();
-                    if (lane == 0) bar_arrive(&ctrl->acc_empty[buf]);
-                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) bar_arrive(&ctrl->acc_empty[buf]);
 #pragma unroll
-                for (int i = 0; i < LW / 4; ++i) {
-                    const ulonglong2 s = scale[c * (LW / 4) + i];
-                    fma2(acc[c * (LW / 2) + 2 * i], r[4 * i], r[4 * i + 1], s.x);
-                    fma2(acc[c * (LW / 2) + 2 * i + 1], r[4 * i + 2], r[4 * i + 3], s.y);
+                for (int j = 0; j < C / 4; ++j) {
+                    const ulonglong2 s2 = scale[j];
+                    fma2(acc[2 * j], r[4 * j], r[4 * j + 1], s2.x);
+                    fma2(acc[2 * j + 1], r[4 * j + 2], r[4 * j + 3], s2.y);
                 }
             }
         }
     }
-    const int f_local = (warp & 3) * 32 + lane, f = n0 + f_local;
+    const int f_local = (warp & 3) * 32 + lane, f = n0 + f_local, group = (warp - 2) / 4, t0 = group * C;
     if (splits == 1) {
         if (warp >= 2 && fine && f < N) {
 #pragma unroll
-            for (int i = 0; i < NT / 2; ++i) {
+            for (int i = 0; i < C / 2; ++i) {
                 const float2 v = two_of(acc[i]);
-                if (2 * i < M) y[(size_t)(2 * i) * N + f] = from_f<OutT>(v.x);
-                if (2 * i + 1 < M) y[(size_t)(2 * i + 1) * N + f] = from_f<OutT>(v.y);
+                if (t0 + 2 * i < M) y[(size_t)(t0 + 2 * i) * N + f] = from_f<OutT>(v.x);
+                if (t0 + 2 * i + 1 < M) y[(size_t)(t0 + 2 * i + 1) * N + f] = from_f<OutT>(v.y);
             }
         }
     } else {
@@ -237,15 +172,15 @@ __global__ __launch_bounds__(BF_THREADS) void blocks_few_kernel(const __grid_con
         __syncwarp();
         if (warp >= 2) {
 #pragma unroll
-            for (int i = 0; i < NT / 2; ++i) {
+            for (int i = 0; i < C / 2; ++i) {
                 const float2 v = two_of(acc[i]);
-                if (2 * i < M) part[(2 * i) * BF_F + f_local] = v.x;
-                if (2 * i + 1 < M) part[(2 * i + 1) * BF_F + f_local] = v.y;
+                if (t0 + 2 * i < M) part[(t0 + 2 * i) * BF_F + f_local] = v.x;
+                if (t0 + 2 * i + 1 < M) part[(t0 + 2 * i + 1) * BF_F + f_local] = v.y;
             }
         }
         cluster_sync_all();
         if (warp >= 2) {
-            for (int t = split; t < M; t += splits) {
+            for (int t = split + group * splits; t < M; t += GROUPS * splits) {
                 float v = 0.f;
 #pragma unroll 4
                 for (int s = 0; s < splits; ++s) v += ld_dsmem(part + t * BF_F + f_local, (uint32_t)s);
@@ -262,40 +197,46 @@ __global__ __launch_bounds__(BF_THREADS) void blocks_few_kernel(const __grid_con
     }
 }
 
-// How a product is cut: CTAs that share a tile's k, and blocks of k for each.
-struct FewPlan {
-    int tiles, splits, per;
-};
-FewPlan few_plan(int N, int k_blocks, int sms) {
-    FewPlan p;
-    p.tiles = (N + BF_F - 1) / BF_F;
-    int splits = (2 * sms + p.tiles - 1) / p.tiles;
-    if (splits > BF_MAX_SPLITS) splits = BF_MAX_SPLITS;
-    if (splits > k_blocks / 2) splits = k_blocks / 2;
-    if (splits < 1) splits = 1;
-    p.per = (k_blocks + splits - 1) / splits;
-    p.splits = (k_blocks + p.per - 1) / p.per;
-    return p;
+// CTAs that share a tile's k: a power of two (such clusters leave no SMs of a group of them idle), the smallest that gives work to three quarters of the SMs.  A CTA
+// streams a block in 0.4 us at the fastest, so fewer leave memory idle; more share the same stream, and one that finds no place costs a second round.  8 rows, us:
+// 4,096 of K 14336 (32 tiles) in 2, 4, 8, 9 splits 19.9, 12.8, 12.7, 13.0 (a cluster of 9 too many: 18.3); 6,144 of K 4096 (48) in 2, 4, 6, 8 8.8, 7.8, 12.6, 7.8;
+// 16,384 of K 2048 (128) in 1, 2, 3 8.3, 9.1, 9.3 to 15.1.  With 128 rows a CTA fills an SM, and clusters of more than 4 find too few places.
+template <int NT> int few_splits(int tiles, int k_blocks, int sms) {
+    int s = 1;
+    if (NT == 128)
+        while (s < 4 && 2 * s * tiles * 10 <= 9 * sms) s *= 2;
+    else
+        while (s < BF_MAX_SPLITS && 4 * s * tiles < 3 * sms) s *= 2;
+    const int most = k_blocks / 2;
+    return s < most ? s : most < 1 ? 1 : most;
+}
+// Stages of the ring: six for a CTA that has an SM to itself; four so that two CTAs fit, for clusters and where there are more CTAs than SMs; and as few as keep
+// tensor memory enough for many CTAs an SM where there are several for each (128,256 features of K 2048: 40.2, 41.4 and 45.2 us with 2, 4 and 6).
+template <int NT> int few_stages(int tiles, int splits, int sms) {
+    if (NT == 128 || (splits == 1 && tiles <= sms)) return 6;
+    return splits > 1 || tiles <= 4 * sms || NT == 64 ? 4 : NT == 16 ? 2 : 3;
 }
 
-template <int NT, int FUSED, typename OutT>
-int launch_blocks_few(const PlainRows& rows, const void* x, long long ldx, const float* sx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K,
-                      int early, const FewPlan& p, cudaStream_t stream) {
-    CUtensorMap map_w, map_x;
-    if (!make_code_map(&map_w, w, N, K, BF_F, ldw)) return RLIS_ERR_UNSUPPORTED;
-    map_x = map_w;
-    if (!FUSED && !make_code_map(&map_x, x, M, K, NT, ldx)) return RLIS_ERR_UNSUPPORTED;
-    int stages = p.per < bf_stages<NT>() ? p.per : bf_stages<NT>();
-    // (the stages also hold a CTA's sums for the cluster)
-    while (p.splits > 1 && stages * (BF_W_BYTES + (FUSED ? 0 : NT * QB)) < NT * BF_F * 4) ++stages;
-    const int chunk = p.per < BF_SCALES / NT ? p.per : BF_SCALES / NT;
-    const size_t smem = (size_t)stages * BF_W_BYTES + (size_t)(FUSED ? p.per : stages) * NT * QB + (size_t)chunk * NT * 4 + 1024 /* alignment */ + 256;
+template <int NT, typename OutT>
+int launch_blocks_few(const void* x, long long ldx, const float* sx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int early, int sms,
+                      cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed{0}, wide{0};
-    cudaError_t e = rlis_allow_smem(blocks_few_kernel<NT, FUSED, OutT>, (int)(BF_MAX_STAGES * (BF_W_BYTES + 32 * QB) + BF_FUSED_BLOCKS * 16 * QB + BF_SCALES * 4 + 1280), allowed);
-    if (e == cudaSuccess) e = rlis_allow_wide_cluster(blocks_few_kernel<NT, FUSED, OutT>, wide);
+    constexpr int STAGE_BYTES = BF_W_BYTES + NT * QB;
+    cudaError_t e = rlis_allow_smem(blocks_few_kernel<NT, OutT>, BF_MAX_STAGES * STAGE_BYTES + BF_SCALES * 4 + 1280, allowed);
+    if (e == cudaSuccess) e = rlis_allow_wide_cluster(blocks_few_kernel<NT, OutT>, wide);
     if (e != cudaSuccess) return (int)e;
-    rlis_launch_cluster(blocks_few_kernel<NT, FUSED, OutT>, dim3((unsigned)p.tiles, (unsigned)p.splits), BF_THREADS, smem, stream, dim3(1, (unsigned)p.splits, 1), map_w,
-                        map_x, rows, sx, sw, (OutT*)y, M, N, (K + QB - 1) / QB, p.per, stages, early);
+    CUtensorMap map_w, map_x;
+    if (!make_code_map(&map_w, w, N, K, BF_F, ldw) || !make_code_map(&map_x, x, M, K, NT, ldx)) return RLIS_ERR_UNSUPPORTED;
+    const int tiles = (N + BF_F - 1) / BF_F, k_blocks = (K + QB - 1) / QB;
+    int splits = few_splits<NT>(tiles, k_blocks, sms);
+    const int per = (k_blocks + splits - 1) / splits;
+    splits = (k_blocks + per - 1) / per;
+    int stages = few_stages<NT>(tiles, splits, sms);
+    if (stages > per) stages = per;
+    while (splits > 1 && stages * STAGE_BYTES < NT * BF_F * 4) ++stages;         // (they also hold a CTA's sums for the cluster)
+    const int chunk = per < BF_SCALES / NT ? per : BF_SCALES / NT;
+    rlis_launch_cluster(blocks_few_kernel<NT, OutT>, dim3((unsigned)tiles, (unsigned)splits), bf_threads<NT>(), (size_t)stages * STAGE_BYTES + (size_t)chunk * NT * 4 + 1280,
+                        stream, dim3(1, (unsigned)splits, 1), map_w, map_x, sx, sw, (OutT*)y, M, N, k_blocks, per, stages, early);
     return RLIS_LAUNCH_CHECK();
 }
 }  // namespace

@@ -412,10 +412,8 @@ extern "C" int rlis_blocks_gemm(const void* x, long long ldx, const float* sx, c
     const int sms = sms_of_device();
     const bool f32 = out_dtype == RLIS_F32;
     if (M <= FEW_ROWS) {
-        const FewPlan p = few_plan(N, (K + QB - 1) / QB, sms);
-        const PlainRows none{nullptr, 0, 0};
-#define RLIS_BF(NT) (f32 ? launch_blocks_few<NT, 0, float>(none, x, ldx, sx, w, ldw, sw, y, M, N, K, early, p, stream) \
-                         : launch_blocks_few<NT, 0, bf16>(none, x, ldx, sx, w, ldw, sw, y, M, N, K, early, p, stream))
+#define RLIS_BF(NT) (f32 ? launch_blocks_few<NT, float>(x, ldx, sx, w, ldw, sw, y, M, N, K, early, sms, stream) \
+                         : launch_blocks_few<NT, bf16>(x, ldx, sx, w, ldw, sw, y, M, N, K, early, sms, stream))
         return M <= 16 ? RLIS_BF(16) : M <= 32 ? RLIS_BF(32) : M <= 64 ? RLIS_BF(64) : RLIS_BF(128);
 #undef RLIS_BF
     }
@@ -429,19 +427,16 @@ extern "C" int rlis_blocks_gemm(const void* x, long long ldx, const float* sx, c
 #undef RLIS_BG
 }
 
-// The same for up to 16 plain rows x [M, K] of `dtype` (ldx elements apart), which the product puts into blocks itself.  RLIS_ERR_UNSUPPORTED where a CTA's part of
-// them does not fit its shared memory.
-extern "C" int rlis_blocks_gemm_rows(const void* x, long long ldx, int dtype, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int out_dtype,
-                                     int early, cudaStream_t stream) {
+extern "C" int rlis_quantize_rows(const void* x, long long ldx, void* codes, long long ldc, float* scales, int n_tokens, int K, int dtype, cudaStream_t stream);
+
+// The same for plain rows x [M, K] of `dtype` (ldx elements apart): rlis_quantize_rows and the product.  scratch: M * ceil(K / 16) * 16 bytes of codes and behind them
+// M * ceil(K / 128) floats, 16-byte aligned.  (The first kernel lets the second start once all kernels before itself have finished; none but itself is in
+// flight then, and it does not write w: w's first tiles are always read early.)
+extern "C" int rlis_blocks_gemm_rows(const void* x, long long ldx, int dtype, void* scratch, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K,
+                                     int out_dtype, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
-    if (M > 16 || K <= 0 || (out_dtype != RLIS_F32 && out_dtype != RLIS_BF16) || (dtype != RLIS_F32 && dtype != RLIS_BF16) || !codes_fit(w, ldw, K)) return RLIS_ERR_UNSUPPORTED;
-    const FewPlan p = few_plan(N, (K + QB - 1) / QB, sms_of_device());
-    if (p.per > BF_FUSED_BLOCKS) return RLIS_ERR_UNSUPPORTED;
-    const int size = dtype == RLIS_F32 ? 4 : 2;
-    const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (M == 1 || (ldx * size) % 16 == 0), f32 = out_dtype == RLIS_F32;
-    const PlainRows rows{x, ldx, K};
-#define RLIS_BF(HOW) (f32 ? launch_blocks_few<16, HOW, float>(rows, nullptr, 0, nullptr, w, ldw, sw, y, M, N, K, early, p, stream) \
-                          : launch_blocks_few<16, HOW, bf16>(rows, nullptr, 0, nullptr, w, ldw, sw, y, M, N, K, early, p, stream))
-    return dtype == RLIS_BF16 ? (vec ? RLIS_BF(3) : RLIS_BF(1)) : (vec ? RLIS_BF(4) : RLIS_BF(2));
-#undef RLIS_BF
+    const long long ldc = (K + 15LL) / 16 * 16;
+    float* sx = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + M * ldc);
+    const int e = rlis_quantize_rows(x, ldx, scratch, ldc, sx, M, K, dtype, stream);
+    return e != 0 ? e : rlis_blocks_gemm(scratch, ldc, sx, w, ldw, sw, y, M, N, K, out_dtype, 1, stream);
 }

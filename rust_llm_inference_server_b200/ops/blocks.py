@@ -13,7 +13,6 @@ from .library import KernelError, check, lib
 
 BLOCK = 128                     # a block's edge
 CODES = torch.float8_e4m3fn
-FUSED_ROWS = 16                 # rows up to which a product puts them into blocks itself
 
 _device = torch._C._cuda_getDevice
 
@@ -131,17 +130,13 @@ def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> 
             return linear_blocks(x, w, out_dtype, early=early)
     T = x.shape[0]
     out = torch.empty((T, N), dtype=torch.bfloat16 if out_code else torch.float32, device=w.values.device)
-    if plain and T <= FUSED_ROWS:
-        code = lib().rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), _code(x.dtype), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K, out_code,
-                                           int(early), _stream())
-        if code != -1:              # (a matrix of so many features and k that a CTA has no room for its part of the rows)
-            check(code, "linear_blocks")
-            _count("linear_blocks.rows")
-            return out
     if plain:
-        # (the kernel that quantises starts the next one when all kernels before itself have finished: none but itself is in flight, and it does not write w)
-        x, early = quantize_rows(x), True
-    check(lib().rlis_blocks_gemm(x.values.data_ptr(), x.stride, x.scales.data_ptr(), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
-                                 out_code, int(early), _stream()), "linear_blocks")
+        scratch = torch.empty((T * (-(-K // 16) * 16 + 4 * -(-K // BLOCK)),), dtype=torch.uint8, device=w.values.device)
+        check(lib().rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), _code(x.dtype), scratch.data_ptr(), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(),
+                                          T, N, K, out_code, _stream()), "linear_blocks")
+        _count("quantize_rows")
+    else:
+        check(lib().rlis_blocks_gemm(x.values.data_ptr(), x.stride, x.scales.data_ptr(), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
+                                     out_code, int(early), _stream()), "linear_blocks")
     _count("linear_blocks")
     return out

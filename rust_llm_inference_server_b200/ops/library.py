@@ -117,7 +117,7 @@ SIGNATURES = {
     "rlis_attention_decode_last_variant": [],
     "rlis_quantize_rows": [P, LL, P, LL, P, I, I, I, P],
     "rlis_quantize_matrix": [P, LL, LL, P, LL, P, I, I, I, I, P],
-    "rlis_blocks_gemm_rows": [P, LL, I, P, LL, P, P, I, I, I, I, I, P],
+    "rlis_blocks_gemm_rows": [P, LL, I, P, P, LL, P, P, I, I, I, I, P],
     "rlis_blocks_gemm": [P, LL, P, P, LL, P, P, I, I, I, I, I, P],
 }
 
