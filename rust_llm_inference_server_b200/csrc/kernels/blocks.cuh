@@ -2,9 +2,14 @@
 //
 //   a = max(amax of the block, 2^-100),  scale = a / 448,  code = e4m3 nearest to 448 x / a  (448 is the largest e4m3)
 //
-// The quotient is rounded once to float32 and once to e4m3: a quotient of two bfloat16 numbers often lies right between two e4m3, and a product with a
-// rounded reciprocal would take one or the other by chance (2 to 3 of 1,000 codes).  2^-100 keeps a block of zeros, or of nothing that counts, free of
-// divisions by zero.  A block that holds a NaN has NaN as its scale and codes; one that holds an infinity an infinite scale and, there, a NaN.
+// 2^-100 keeps a block of zeros, or of nothing that counts, free of divisions by zero.  A block that holds a NaN has NaN as its scale and codes; one that holds an
+// infinity an infinite scale and, there, a NaN.
+//
+// The quotient of two bfloat16 numbers often lies right between two e4m3 (2 to 3 of 1,000 codes), and p = x * fl(448 / a) is off by up to 2^-23 of it, to
+// either side: p alone would take one code or the other by chance.  A point between two codes has five significant bits at most, and a quotient 7 X / A of
+// integers of eight bits that is none of them is at least 2^-13 of it away.  So p rounded to 16 bits (off by 2^-17 at most) is that point where the quotient is,
+// and stays on its side where it is not: for bfloat16 its e4m3 is the quotient's.  A float32 x may come closer: where the 16 bits end in eleven zeros (one
+// of 2,048), the quotient is formed by a division.  (As divisions, all of them, the codes of 2,048 rows of 14,336 took 5 us more: the kernels are nearly bound by instructions.)
 #pragma once
 #include "common.cuh"
 #include <cuda_fp8.h>
@@ -14,38 +19,94 @@ constexpr int QB = 128;                              // a block's edge
 constexpr unsigned LEAST_BITS = 0x0D800000u;         // 2^-100
 constexpr unsigned LARGE_BITS = 0x71800000u;         // 2^100
 
-// What a block's values are turned to codes with: x -> (x * mul) / div.  (Above 2^100 both by 2^-20 less, so that 448 x stays finite.)
+// What a block's values are turned to codes with.
 struct Coding {
-    float mul, div, scale;
+    float a, factor, scale;
 };
 __device__ __forceinline__ Coding coding_of(unsigned amax_bits) {
-    const unsigned bits = max(amax_bits, LEAST_BITS);        // (a NaN's bits are above all others)
-    const float a = __uint_as_float(bits);
     Coding c;
-    c.mul = bits > LARGE_BITS ? 448.f * 0x1p-20f : 448.f;
-    c.div = bits > LARGE_BITS ? a * 0x1p-20f : a;
-    c.scale = a / 448.f;
+    c.a = __uint_as_float(max(amax_bits, LEAST_BITS));          // (a NaN's bits are above all others)
+    c.factor = 448.f / c.a;
+    c.scale = c.a / 448.f;
     return c;
 }
-__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-__device__ __forceinline__ uint32_t codes4(const float* v, const Coding& c) {
-    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[0] * c.mul, c.div), __fdiv_rn(v[1] * c.mul, c.div)), __NV_SATFINITE, __NV_E4M3);
-    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[2] * c.mul, c.div), __fdiv_rn(v[3] * c.mul, c.div)), __NV_SATFINITE, __NV_E4M3);
+// p rounded to 16 significant bits (T. J. Dekker's splitting; a NaN stays one).
+__device__ __forceinline__ float of_16_bits(float p) {
+    const float c = __fmul_rn(p, 257.f);
+    return __fsub_rn(c, __fsub_rn(c, p));
+}
+__device__ __forceinline__ uint32_t pack_codes(const float* q) {
+    const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+    const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
     return (uint32_t)lo | ((uint32_t)hi << 16);
 }
-
-// Eight consecutive values of a row of K, zeros past its end.
-template <typename T, bool VEC> __device__ __forceinline__ void load8(const T* row, int k, int K, float (&v)[8]) {
+// Eight consecutive values of a row of K as they lie in memory, zeros past the row's end.
+template <typename T> struct Eight {
+    static constexpr int WORDS = 2 * (int)sizeof(T);
+    uint32_t w[WORDS];
+};
+template <typename T> __device__ __forceinline__ Eight<T> nothing8() {
+    Eight<T> e;
+#pragma unroll
+    for (int i = 0; i < Eight<T>::WORDS; ++i) e.w[i] = 0u;
+    return e;
+}
+template <typename T, bool VEC> __device__ __forceinline__ Eight<T> load8(const T* row, int k, int K) {
+    Eight<T> e = nothing8<T>();
     if (VEC && k + 8 <= K) {
 #pragma unroll
-        for (int i = 0; i < 8; i += Vec16<T>::N) load16<T>(row + k + i, v + i);
+        for (int i = 0; i < Eight<T>::WORDS; i += 4) *reinterpret_cast<uint4*>(e.w + i) = *reinterpret_cast<const uint4*>(row + k + i * 4 / (int)sizeof(T));
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f<T>(row[k + i]) : 0.f;
+        for (int i = 0; i < 8; ++i)
+            if (k + i < K) {
+                if constexpr (sizeof(T) == 4) e.w[i] = reinterpret_cast<const uint32_t*>(row)[k + i];
+                else e.w[i >> 1] |= (uint32_t) reinterpret_cast<const unsigned short*>(row)[k + i] << (i & 1) * 16;
+            }
+    }
+    return e;
+}
+// The bits of the largest of their absolute values as a float (a NaN's are above all others).
+template <typename T> __device__ __forceinline__ unsigned amax_bits(const Eight<T>& e) {
+    unsigned m = 0;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, e.w[i] & 0x7fffffffu);
+        return m;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = __vmaxu2(m, e.w[i] & 0x7fff7fffu);
+        return max(m << 16, m & 0xffff0000u);
     }
 }
+template <typename T> __device__ __forceinline__ void widen(const Eight<T>& e, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = __uint_as_float(e.w[i]);
+        else v[i] = __uint_as_float((i & 1) ? e.w[i >> 1] & 0xffff0000u : e.w[i >> 1] << 16);
+    }
+}
+template <typename T> __device__ __forceinline__ uint2 codes8(const Eight<T>& e, const Coding& c) {
+    float v[8], q[8];
+    widen(e, v);
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        q[i] = of_16_bits(__fmul_rn(v[i], c.factor));
+        near |= (__float_as_uint(q[i]) & 0x7ffffu) == 0u && q[i] != 0.f;
+    }
+    if (sizeof(T) == 4 && near) {
+        // (above 2^100 both by 2^-20 less, so that 448 x stays finite)
+        const bool large = __float_as_uint(c.a) > LARGE_BITS;
+        const float mul = large ? 448.f * 0x1p-20f : 448.f, div = large ? c.a * 0x1p-20f : c.a;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(v[i] * mul, div);
+    }
+    return make_uint2(pack_codes(q), pack_codes(q + 4));
+}
+
 // Their codes, into a row that starts at a multiple of 16 bytes and has room for K rounded up to 16.
-__device__ __forceinline__ void store8(unsigned char* row, int k, int K, const float (&v)[8], const Coding& c) {
-    if (k < K) *reinterpret_cast<uint2*>(row + k) = make_uint2(codes4(v, c), codes4(v + 4, c));
+template <typename T> __device__ __forceinline__ void store8(unsigned char* row, int k, int K, const Eight<T>& e, const Coding& c) {
+    if (k < K) *reinterpret_cast<uint2*>(row + k) = codes8<T>(e, c);
 }
 }  // namespace

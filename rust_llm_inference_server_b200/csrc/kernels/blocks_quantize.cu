@@ -3,80 +3,68 @@
 #include "blocks.cuh"
 
 namespace {
-// Sixteen lanes take a block of a row, eight values each; a group of lanes takes UNITS blocks, all of whose loads are asked for first.
-constexpr int ROWS_THREADS = 256, UNITS = 2;
+// Sixteen lanes take a block of a row, eight values each; a group of lanes takes UNITS blocks, all of whose loads are asked for first.  A block's row is its number
+// divided by the blocks of a row: umulhi with ceil(2^32 / blocks) is exact for as many blocks as a launch takes (a division in 64 bits took as many
+// instructions as everything else).
+constexpr int ROWS_THREADS = 256, UNITS = 4, ROWS_PER_CTA = ROWS_THREADS / 16 * UNITS;
+constexpr long long MOST_UNITS = 1 << 16;
 template <typename T, bool VEC>
 __global__ __launch_bounds__(ROWS_THREADS) void quantize_rows_kernel(const T* __restrict__ x, long long ldx, unsigned char* __restrict__ codes, long long ldc,
-                                                                     float* __restrict__ scales, int n_tokens, int K, int k_blocks) {
+                                                                     float* __restrict__ scales, int n_tokens, int rows_per, int K, int k_blocks, unsigned magic) {
     pdl_wait_and_trigger();
     const int group = threadIdx.x >> 4, lane = threadIdx.x & 15;
-    const long long total = (long long)n_tokens * k_blocks;
-    const long long first = (long long)blockIdx.x * (ROWS_THREADS / 16 * UNITS) + group;
-    float v[UNITS][8];
+    const int row0 = blockIdx.y * rows_per, total = min(rows_per, n_tokens - row0) * k_blocks;
+    Eight<T> v[UNITS];
     int row[UNITS], kb[UNITS];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-        const long long unit = first + u * (ROWS_THREADS / 16);
-        row[u] = unit < total ? (int)(unit / k_blocks) : -1;
-        kb[u] = unit < total ? (int)(unit - (long long)row[u] * k_blocks) : 0;
-        if (row[u] >= 0) {
-            load8<T, VEC>(x + row[u] * ldx, kb[u] * QB + lane * 8, K, v[u]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-        }
+        const int unit = blockIdx.x * ROWS_PER_CTA + u * (ROWS_THREADS / 16) + group;
+        const int r = magic != 0u ? (int)__umulhi((unsigned)unit, magic) : unit;
+        row[u] = unit < total ? row0 + r : -1;
+        kb[u] = unit - r * k_blocks;
+        v[u] = row[u] >= 0 ? load8<T, VEC>(x + row[u] * ldx, kb[u] * QB + lane * 8, K) : nothing8<T>();
     }
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-        unsigned amax = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) amax = max(amax, abs_bits(v[u][i]));
+        unsigned amax = amax_bits(v[u]);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));      // within the sixteen lanes
         if (row[u] < 0) continue;
         const Coding c = coding_of(amax);
-        store8(codes + row[u] * ldc, kb[u] * QB + lane * 8, K, v[u], c);
+        store8<T>(codes + row[u] * ldc, kb[u] * QB + lane * 8, K, v[u], c);
         if (lane == 0) scales[(long long)kb[u] * n_tokens + row[u]] = c.scale;
     }
 }
 
-// A CTA takes a block of 128 x 128: sixteen lanes a row, sixteen rows at a time.
-constexpr int MATRIX_THREADS = 256, MATRIX_ROWS = QB / (MATRIX_THREADS / 16);
+// A CTA takes a block of 128 x 128: sixteen lanes a row, 32 rows at a time.
+constexpr int MATRIX_THREADS = 512, MATRIX_ROWS = QB / (MATRIX_THREADS / 16);
 template <typename T, bool VEC>
-__global__ __launch_bounds__(MATRIX_THREADS) void quantize_matrix_kernel(const T* __restrict__ w, long long ldw, long long stack_w, unsigned char* __restrict__ codes,
-                                                                         long long ldc, float* __restrict__ scales, int N, int K) {
+__global__ __launch_bounds__(MATRIX_THREADS, sizeof(T) == 4 ? 2 : 3) void quantize_matrix_kernel(const T* __restrict__ w, long long ldw, long long stack_w, unsigned char* __restrict__ codes,
+                                                                            long long ldc, float* __restrict__ scales, int N, int K) {
     pdl_wait_and_trigger();
     __shared__ unsigned part[MATRIX_THREADS / 32];
     const int kb = blockIdx.x, nb = blockIdx.y, e = blockIdx.z;
     const int r0 = nb * QB + (threadIdx.x >> 4), k = kb * QB + (threadIdx.x & 15) * 8;
     w += e * stack_w;
     codes += (long long)e * N * ldc;
-    float v[MATRIX_ROWS][8];
-    unsigned amax = 0;
+    Eight<T> v[MATRIX_ROWS];
 #pragma unroll
     for (int i = 0; i < MATRIX_ROWS; ++i) {
         const int r = r0 + i * (MATRIX_THREADS / 16);
-        if (r < N) {
-            load8<T, VEC>(w + r * ldw, k, K, v[i]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-        }
+        v[i] = r < N ? load8<T, VEC>(w + r * ldw, k, K) : nothing8<T>();
     }
+    unsigned amax = 0;
 #pragma unroll
-    for (int i = 0; i < MATRIX_ROWS; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, abs_bits(v[i][j]));
+    for (int i = 0; i < MATRIX_ROWS; ++i) amax = max(amax, amax_bits(v[i]));
     amax = __reduce_max_sync(0xffffffffu, amax);
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < MATRIX_THREADS / 32; ++i) amax = max(amax, part[i]);
+    amax = __reduce_max_sync(0xffffffffu, part[threadIdx.x & (MATRIX_THREADS / 32 - 1)]);
     const Coding c = coding_of(amax);
 #pragma unroll
     for (int i = 0; i < MATRIX_ROWS; ++i) {
         const int r = r0 + i * (MATRIX_THREADS / 16);
-        if (r < N) store8(codes + r * ldc, k, K, v[i], c);
+        if (r < N) store8<T>(codes + r * ldc, k, K, v[i], c);
     }
     if (threadIdx.x == 0) scales[((long long)e * gridDim.y + nb) * gridDim.x + kb] = c.scale;
 }
@@ -88,16 +76,21 @@ bool in_vectors(const void* p, long long ld, int size) { return (reinterpret_cas
 extern "C" int rlis_quantize_rows(const void* x, long long ldx, void* codes, long long ldc, float* scales, int n_tokens, int K, int dtype, cudaStream_t stream) {
     if (n_tokens <= 0 || K <= 0) return 0;
     if ((dtype != RLIS_F32 && dtype != RLIS_BF16) || ldc < ((K + 15) & ~15) || ldc % 16 != 0 || (reinterpret_cast<uintptr_t>(codes) & 15) != 0) return RLIS_ERR_UNSUPPORTED;
-    const int k_blocks = (K + QB - 1) / QB, per = ROWS_THREADS / 16 * UNITS;
-    const long long ctas = ((long long)n_tokens * k_blocks + per - 1) / per;
-    if (ctas > 0x7fffffffLL) return RLIS_ERR_UNSUPPORTED;
+    const int k_blocks = (K + QB - 1) / QB;
+    // rows in bands whose blocks are few enough for the division by a product
+    const int most = MOST_UNITS / k_blocks > 0 ? (int)(MOST_UNITS / k_blocks) : 1, rows_per = n_tokens < most ? n_tokens : most;
+    const long long bands = (n_tokens + (long long)rows_per - 1) / rows_per;
+    if (k_blocks > MOST_UNITS || bands > 65535) return RLIS_ERR_UNSUPPORTED;
+    const unsigned magic = k_blocks > 1 ? (unsigned)(((1ull << 32) + k_blocks - 1) / k_blocks) : 0u;
     const bool vec = in_vectors(x, n_tokens > 1 ? ldx : 0, dtype == RLIS_F32 ? 4 : 2);
-    const dim3 grid((unsigned)ctas);
+    const dim3 grid((unsigned)((rows_per * k_blocks + ROWS_PER_CTA - 1) / ROWS_PER_CTA), (unsigned)bands);
     unsigned char* c = static_cast<unsigned char*>(codes);
     if (dtype == RLIS_F32)
-        rlis_launch(vec ? quantize_rows_kernel<float, true> : quantize_rows_kernel<float, false>, grid, ROWS_THREADS, 0, stream, (const float*)x, ldx, c, ldc, scales, n_tokens, K, k_blocks);
+        rlis_launch(vec ? quantize_rows_kernel<float, true> : quantize_rows_kernel<float, false>, grid, ROWS_THREADS, 0, stream, (const float*)x, ldx, c, ldc, scales, n_tokens,
+                    rows_per, K, k_blocks, magic);
     else
-        rlis_launch(vec ? quantize_rows_kernel<bf16, true> : quantize_rows_kernel<bf16, false>, grid, ROWS_THREADS, 0, stream, (const bf16*)x, ldx, c, ldc, scales, n_tokens, K, k_blocks);
+        rlis_launch(vec ? quantize_rows_kernel<bf16, true> : quantize_rows_kernel<bf16, false>, grid, ROWS_THREADS, 0, stream, (const bf16*)x, ldx, c, ldc, scales, n_tokens,
+                    rows_per, K, k_blocks, magic);
     return RLIS_LAUNCH_CHECK();
 }
 
