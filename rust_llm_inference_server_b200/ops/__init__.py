@@ -2388,4 +2388,4 @@ def nll_rows(logits: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
     return out
 
 
-from .blocks import BlockMatrix, BlockRows, linear_blocks, quantize_matrix, quantize_rows  # noqa: E402,F401  (at the end: it takes helpers of this file)
+from .blocks import MOE_LAYER_TOKENS, BlockMatrix, BlockRows, linear_blocks, moe_layer, quantize_matrix, quantize_rows  # noqa: E402,F401  (at the end: it takes helpers of this file)

@@ -6,6 +6,8 @@ taken as it is."""
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _code, _count, _stream
@@ -139,4 +141,108 @@ def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> 
         check(lib().rlis_blocks_gemm(x.values.data_ptr(), x.stride, x.scales.data_ptr(), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
                                      out_code, int(early), _stream()), "linear_blocks")
     _count("linear_blocks")
+    return out
+
+
+MOE_LAYER_TOKENS = 16           # tokens that `moe_layer` takes
+_SCORING = {"sigmoid": 0, "softmax_chosen": 1, "softmax": 2}
+
+
+class _LayerMatrix(ctypes.Structure):
+    _fields_ = [("w", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("row_bytes", ctypes.c_longlong), ("stack_bytes", ctypes.c_longlong)]
+
+
+class _MoeLayer(ctypes.Structure):
+    """A call of the layer (csrc/kernels/moe_layer.cu: RlisMoeLayer)."""
+    _fields_ = ([("x", ctypes.c_void_p), ("ldx", ctypes.c_longlong), ("router", ctypes.c_void_p), ("correction", ctypes.c_void_p), ("router_bias", ctypes.c_void_p)]
+                + [(n, _LayerMatrix) for n in ("up", "down", "shared_up", "shared_down")] + [("workspace", ctypes.c_void_p), ("out", ctypes.c_void_p)]
+                + [(n, ctypes.c_int) for n in ("n_tokens", "width", "inner", "inner_shared", "n_experts", "n_identity", "top", "scoring", "n_groups", "keep_groups",
+                                               "normalize", "shared_gate", "interleave", "interleave_shared")]
+                + [(n, ctypes.c_float) for n in ("route_scale", "slope", "limit", "shift")])
+
+
+def _layer_matrix(m, dims: int, rows, k, blocks: bool, device, name: str) -> _LayerMatrix:
+    """A matrix of the layer (or a stack of them) of `rows` x `k` (None: any), as the launcher takes it."""
+    if isinstance(m, BlockMatrix) != blocks:
+        raise KernelError(f"moe_layer: {name}: the layer's matrices are all in bfloat16 or all in blocks")
+    t = m.values if blocks else m
+    if not isinstance(t, torch.Tensor) or t.device != device or t.dim() != dims or (rows is not None and t.shape[-2] != rows) or (k is not None and t.shape[-1] != k):
+        raise KernelError(f"moe_layer: {name}: expected {'a stack of matrices' if dims == 3 else 'a matrix'} of {rows} x {k} on {device}, "
+                          f"got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
+    if blocks:
+        return _LayerMatrix(t.data_ptr(), m.scales.data_ptr(), m.stride, t.shape[-2] * m.stride)
+    if t.dtype != torch.bfloat16 or not t.is_contiguous():
+        raise KernelError(f"moe_layer: {name}: expected contiguous bfloat16 or a BlockMatrix, got {t.dtype} with strides {t.stride()}")
+    return _LayerMatrix(t.data_ptr(), None, 2 * t.shape[-1], 2 * t.shape[-2] * t.shape[-1])
+
+
+def _layer_vector(v, n: int, device, name: str):
+    if v is None:
+        return None
+    if v.dtype != torch.float32 or tuple(v.shape) != (n,) or not v.is_contiguous() or v.device != device:
+        raise KernelError(f"moe_layer: {name}: expected contiguous float32 [{n}] on {device}")
+    return v.data_ptr()
+
+
+def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: int, route_scale: float = 1.0, *, correction: torch.Tensor | None = None,
+              router_bias: torch.Tensor | None = None, scoring: str = "sigmoid", groups: tuple | None = None, normalize: bool = False, n_identity: int = 0,
+              shared: tuple | None = None, shared_gate: bool = False, slope: float = 1.0, limit: float | None = None, up_shift: float = 0.0, interleave: int = 0,
+              shared_interleave: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A whole mixture of experts for up to `MOE_LAYER_TOKENS` tokens in two launches: what `moe_route`, `moe_up`, `moe_down`, a shared expert and `moe_combine`
+    compute, every weight read once.  x [T, W] bfloat16 (rows of a wider tensor if need be); the result [T, W] bfloat16 (`out`, or a new tensor).
+
+    w_router float32 [experts + n_identity (+ 1), W] (with `shared_gate` its last row is the logit of the shared expert's gate), `correction`, `router_bias`,
+    `scoring` ("sigmoid", "softmax" or "softmax_chosen"), `groups`, `normalize` and `n_identity` as `moe_route` takes them; `top` up to 16.
+    w_gate_up [experts, 2 I, W] and w_down [experts, W, I], both contiguous bfloat16 or both stacks in blocks; `shared` = (gate|up [2 S, W], down [W, S]) of the
+    shared expert in the same form; `interleave` (`shared_interleave`) as `moe_up` takes it (in blocks 0, 4 or a multiple of 8); the gating of `glu_act` with
+    `slope`, `limit` and `up_shift`.  W, I and S are multiples of 8, in blocks of 16.
+
+    Scores, sums and the experts' gated results (as pairs of bfloat16, to 2^-17) are float32; a token's result is rounded once.  Codes are e4m3's finite
+    numbers here: a NaN code of a stored matrix counts as 480 (one that `quantize_matrix` wrote has a scale of NaN beside it)."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
+        raise KernelError("moe_layer: expected bfloat16 rows [T, W] with unit stride on the device; there is no CPU path")
+    dev = x.device
+    if x.get_device() != _device():
+        with torch.cuda.device(dev):
+            return moe_layer(x, w_router, w_gate_up, w_down, top, route_scale, correction=correction, router_bias=router_bias, scoring=scoring, groups=groups,
+                             normalize=normalize, n_identity=n_identity, shared=shared, shared_gate=shared_gate, slope=slope, limit=limit, up_shift=up_shift,
+                             interleave=interleave, shared_interleave=shared_interleave, out=out)
+    T, W = x.shape
+    if T > MOE_LAYER_TOKENS:
+        raise KernelError(f"moe_layer: takes up to {MOE_LAYER_TOKENS} tokens, got {T}; more go through moe_route, moe_up, moe_down and moe_combine")
+    if scoring not in _SCORING:
+        raise KernelError(f"moe_layer: unknown scoring {scoring!r}; known: {sorted(_SCORING)}")
+    blocks = isinstance(w_gate_up, BlockMatrix)
+    up = _layer_matrix(w_gate_up, 3, None, W, blocks, dev, "w_gate_up")
+    E, I2 = w_gate_up.shape[:2]
+    down = _layer_matrix(w_down, 3, W, I2 // 2, blocks, dev, "w_down")
+    if w_down.shape[0] != E or I2 % 2:
+        raise KernelError(f"moe_layer: {E} and {w_down.shape[0]} experts, {I2} rows of gate and linear branch")
+    S2, shared_up, shared_down = 0, _LayerMatrix(), _LayerMatrix()
+    if shared is not None:
+        shared_up = _layer_matrix(shared[0], 2, None, W, blocks, dev, "shared gate|up")
+        S2 = shared[0].shape[0]
+        shared_down = _layer_matrix(shared[1], 2, W, S2 // 2, blocks, dev, "shared down")
+        if S2 % 2 or S2 < 2:
+            raise KernelError(f"moe_layer: {S2} rows of the shared expert's gate and linear branch")
+    elif shared_gate:
+        raise KernelError("moe_layer: a gate on the shared expert, and no shared expert")
+    n_out = E + int(n_identity)
+    if w_router.dtype != torch.float32 or tuple(w_router.shape) != (n_out + (1 if shared_gate else 0), W) or not w_router.is_contiguous() or w_router.device != dev:
+        raise KernelError(f"moe_layer: expected a contiguous float32 router [{n_out + (1 if shared_gate else 0)}, {W}] on {dev}, got {w_router.dtype} {tuple(w_router.shape)}")
+    n_groups, keep = groups if groups is not None else (1, 1)
+    if out is None:
+        out = torch.empty((T, W), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, W) or not out.is_contiguous() or out.device != dev:
+        raise KernelError(f"moe_layer: out: expected contiguous bfloat16 {(T, W)} on {dev}")
+    if T == 0:
+        return out
+    work = torch.empty((lib().rlis_moe_layer_bytes(T, int(top), I2 // 2, S2 // 2),), dtype=torch.uint8, device=dev)
+    call = _MoeLayer(x.data_ptr(), x.stride(0) if T > 1 else W, w_router.data_ptr(), _layer_vector(correction, n_out, dev, "correction"),
+                     _layer_vector(router_bias, n_out, dev, "router_bias"), up, down, shared_up, shared_down, work.data_ptr(), out.data_ptr(), T, W, I2 // 2, S2 // 2, E,
+                     int(n_identity), int(top), _SCORING[scoring], int(n_groups), int(keep), 1 if normalize else 0, 1 if shared_gate else 0, int(interleave),
+                     int(shared_interleave), float(route_scale), float(slope), float("inf") if limit is None else float(limit), float(up_shift))
+    check(lib().rlis_moe_layer(ctypes.addressof(call), _stream()), "moe_layer")
+    _count("moe_layer.up" + (".blocks" if blocks else ""))
+    _count("moe_layer.down" + (".blocks" if blocks else ""))
     return out

@@ -115,6 +115,8 @@ SIGNATURES = {
     "rlis_stream_gemm_timeline": [I],
     "rlis_stream_gemm_timeline_read": [P, P],
     "rlis_attention_decode_last_variant": [],
+    "rlis_moe_layer_bytes": [I, I, I, I],
+    "rlis_moe_layer": [P, P],
     "rlis_quantize_rows": [P, LL, P, LL, P, I, I, I, P],
     "rlis_quantize_matrix": [P, LL, LL, P, LL, P, I, I, I, I, P],
     "rlis_blocks_gemm_rows": [P, LL, I, P, P, LL, P, P, I, I, I, I, P],
