@@ -9,11 +9,13 @@
 // shared memory between: a sum over k may take k in any order, so a thread's 16 bytes of a row, eight neighbouring k, serve as its k slots of two
 // instructions, and the tokens' rows, which stay in the first-level cache, are read in the same order.  A warp takes 128 k of 16 rows at a time (a chunk, a
 // block's edge; for weights in e4m3 blocks a chunk's sums are scaled before they join the others) and has the next chunks, of the next rows if need be, on
-// their way while it works on one: 128 KB an SM (96 KB of codes) are in flight.  The warps of a CTA take different k of the same rows and add their sums
-// in shared memory in the order of the warps, so results do not depend on timing.
+// their way while it works on one: 128 KB an SM (96 KB of codes) are in flight.  Four warps (up) or a CTA's sixteen (down) take different k of the same rows
+// and add their sums in shared memory in the order of the warps, so results do not depend on timing.
 //
 // Routing sits in the up kernel: the CTAs of a cluster share the router's rows, hand each other the logits (distributed shared memory), and each chooses
-// for all tokens itself: no launch of its own, no grid-wide barrier, no workspace but h and the plan, which the first CTA leaves for the down kernel.
+// for all tokens itself: no launch of its own, no grid-wide barrier, no workspace but h and the plan, which the first CTA leaves for the down kernel.  The
+// router's float32 rows go through the same instructions as three bfloat16 numbers each, whose sum they are to 2^-24 (a token's logits are sums of exact
+// products in float32, as a chain of FMAs would give them; as FMAs, 128 rows against 16 tokens took 20 us).
 //
 // The weights of the choice are multiplied into h in float32, and h is handed on as two bfloat16 numbers (their sum is h to 2^-17), so that nothing but the
 // result is rounded to the activations' type; the down product is then one long sum over the chosen experts' k, with the step's tokens as columns whoever
@@ -29,14 +31,20 @@ constexpr int L_CLUSTER = 8;            // CTAs that share the router's rows
 constexpr int L_MAX_OUT = 512;          // router outputs
 constexpr int L_MAX_PAIRS = 256;        // tokens * top
 constexpr int LK = 128;                 // k of a chunk
+constexpr int MOST_K = 16384;           // of a matrix of the layer (items' numbers stay within what a product divides)
 constexpr float E4M3_TO_BF16 = 0x1p120f;
 
-// What the up kernel leaves for the down kernel.
+// An expert that some token chose: the tokens as bits, as a list (four bits each), and which of a token's choices it is (four bits a token).
+struct ActiveExpert {
+    int expert;
+    unsigned tokens;
+    unsigned long long list, choice;
+};
+// What the up kernel leaves for the down kernel: the active experts, ascending.
 struct LayerPlan {
-    int n_active;
-    int expert[L_MAX_PAIRS];            // the experts that some token chose, ascending
-    short slot[L_MAX_PAIRS][LT];        // row of h of (such an expert, token), or -1
+    int n_active, unused;
     float identity[LT];                 // a token's weights of identity experts, summed
+    ActiveExpert of[L_MAX_PAIRS];
 };
 
 // One matrix of the layer (or a stack): `ld` elements (bfloat16) or bytes (codes) between rows; codes have scales [matrix][row / 128][k / 128].
@@ -60,8 +68,12 @@ struct LayerArgs {
     LayerPlan* plan;
     bf16 *h_hi, *h_lo;                  // [tokens * top + tokens, h_row]
     int h_row;
+    unsigned per_expert_magic, own_chunks_magic;        // see quotient()
     bf16* out;
 };
+
+// n / d with d's magic number ceil(2^32 / d) (0 for d 1), exact for n below 2^32 / d.
+__device__ __forceinline__ int quotient(int n, unsigned magic) { return magic != 0u ? (int)__umulhi((unsigned)n, magic) : n; }
 
 __device__ __forceinline__ uint4 stream16(const void* p) {
     uint4 v;
@@ -100,60 +112,53 @@ __device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& even, uint32_t
     odd = place(w);
 }
 
-// acc += chunk * the columns' rows: `rows[i]` is this lane's column's (lane / 4) row of bfloat16 from the chunk's first k on, or null (a column of zeros).
+// d += chunk * the sum of a column's rows: `rows` are this lane's column's (lane / 4) rows of bfloat16 from the chunk's first k on, or null (a column of zeros);
+// `left`: k from there on.  All of the rows are asked for before the first is used.
 template <bool CODES, int ROWS>
-__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const bf16* const (&rows)[ROWS], int k0, int K, int lane, float (*acc)[4], const int (&to)[ROWS], bool second) {
-    constexpr int PER = CODES ? 16 : 8;
-    float part[2][4] = {};
+__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const bf16* const (&rows)[ROWS], int left, int lane, float (&d)[4]) {
+    constexpr int PER = CODES ? 16 : 8, VECS = PER / 8, STEPS = Chunk<CODES>::STEPS;
+    uint4 b[STEPS][ROWS][VECS];
 #pragma unroll
-    for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
-        const int k = s * 4 * PER + (lane & 3) * PER;
-        const bool in = k0 + k < K;
-        uint32_t a[CODES ? 4 : 2][4];
+    for (int s = 0; s < STEPS; ++s)
+#pragma unroll
+        for (int i = 0; i < ROWS; ++i)
+#pragma unroll
+            for (int v = 0; v < VECS; ++v) {
+                const int k = (s * 4 + (lane & 3)) * PER + v * 8;
+                b[s][i][v] = rows[i] != nullptr && k < left ? *reinterpret_cast<const uint4*>(rows[i] + k) : make_uint4(0, 0, 0, 0);
+            }
+    float part[4] = {};
+    float(&sum)[4] = CODES ? part : d;
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
         const uint32_t r0[4] = {c.a[s][0].x, c.a[s][0].y, c.a[s][0].z, c.a[s][0].w}, r1[4] = {c.a[s][1].x, c.a[s][1].y, c.a[s][1].z, c.a[s][1].w};
         if constexpr (CODES) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                widen_codes(r0[j], a[j][0], a[j][2]);
-                widen_codes(r1[j], a[j][1], a[j][3]);
+                uint32_t a[4];
+                widen_codes(r0[j], a[0], a[2]);
+                widen_codes(r1[j], a[1], a[3]);
+#pragma unroll
+                for (int i = 0; i < ROWS; ++i) {
+                    const uint4 v = b[s][i][j / 2];
+                    const uint32_t x0 = j & 1 ? v.z : v.x, x1 = j & 1 ? v.w : v.y;
+                    mma_bf16_16816(sum, a, __byte_perm(x0, x1, 0x5410), __byte_perm(x0, x1, 0x7632));
+                }
             }
         } else {
+            const uint32_t a0[4] = {r0[0], r1[0], r0[1], r1[1]}, a1[4] = {r0[2], r1[2], r0[3], r1[3]};
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                a[j][0] = r0[2 * j];
-                a[j][1] = r1[2 * j];
-                a[j][2] = r0[2 * j + 1];
-                a[j][3] = r1[2 * j + 1];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            if (to[i] == 1 && !second) continue;
-            const bool have = in && rows[i] != nullptr;
-            float(&d)[4] = CODES ? part[to[i]] : acc[to[i]];
-            if constexpr (CODES) {
-                const uint4 lo = have ? *reinterpret_cast<const uint4*>(rows[i] + k) : make_uint4(0, 0, 0, 0);
-                const uint4 hi = have ? *reinterpret_cast<const uint4*>(rows[i] + k + 8) : make_uint4(0, 0, 0, 0);
-                mma_bf16_16816(d, a[0], __byte_perm(lo.x, lo.y, 0x5410), __byte_perm(lo.x, lo.y, 0x7632));
-                mma_bf16_16816(d, a[1], __byte_perm(lo.z, lo.w, 0x5410), __byte_perm(lo.z, lo.w, 0x7632));
-                mma_bf16_16816(d, a[2], __byte_perm(hi.x, hi.y, 0x5410), __byte_perm(hi.x, hi.y, 0x7632));
-                mma_bf16_16816(d, a[3], __byte_perm(hi.z, hi.w, 0x5410), __byte_perm(hi.z, hi.w, 0x7632));
-            } else {
-                const uint4 b = have ? *reinterpret_cast<const uint4*>(rows[i] + k) : make_uint4(0, 0, 0, 0);
-                mma_bf16_16816(d, a[0], b.x, b.y);
-                mma_bf16_16816(d, a[1], b.z, b.w);
+            for (int i = 0; i < ROWS; ++i) {
+                mma_bf16_16816(sum, a0, b[s][i][0].x, b[s][i][0].y);
+                mma_bf16_16816(sum, a1, b[s][i][0].z, b[s][i][0].w);
             }
         }
     }
     if constexpr (CODES) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            if (n == 1 && !second) break;
-            acc[n][0] = fmaf(part[n][0], c.scale[0], acc[n][0]);
-            acc[n][1] = fmaf(part[n][1], c.scale[0], acc[n][1]);
-            acc[n][2] = fmaf(part[n][2], c.scale[1], acc[n][2]);
-            acc[n][3] = fmaf(part[n][3], c.scale[1], acc[n][3]);
-        }
+        d[0] = fmaf(part[0], c.scale[0], d[0]);
+        d[1] = fmaf(part[1], c.scale[0], d[1]);
+        d[2] = fmaf(part[2], c.scale[1], d[2]);
+        d[3] = fmaf(part[3], c.scale[1], d[3]);
     }
 }
 
@@ -167,86 +172,107 @@ __device__ __forceinline__ unsigned order_of(float v) {
 }
 __device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
 
-// One warp chooses for one token: z [n_out] logits in, scores out; key [n_out] and rank [n_groups] are scratch.
-__device__ __forceinline__ void choose(const LayerArgs& p, float* z, unsigned* key, float* rank, int* idx, float* weight, int lane) {
+// One warp chooses for one token: z [n_out] logits in; the scores' bits stay in the lanes (output lane + 32 i in place i).  `scratch` [n_out + n_groups] for groups.
+// Lane k ends with choice k and its weight.
+template <int PLACES>
+__device__ __forceinline__ void choose(const LayerArgs& p, const float* z, unsigned* scratch, int lane, int& chosen, float& weight) {
     const int n = p.n_out;
+    float score[PLACES];
+    unsigned key[PLACES];
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+        const int e = lane + 32 * i;
+        score[i] = e < n ? z[e] + (p.router_bias != nullptr ? p.router_bias[e] : 0.f) : -INFINITY;
+    }
     if (p.scoring == 2) {
         float mx = -INFINITY, sum = 0.f;
-        for (int e = lane; e < n; e += 32) {
-            z[e] += p.router_bias != nullptr ? p.router_bias[e] : 0.f;
-            mx = fmaxf(mx, z[e]);
-        }
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i) mx = fmaxf(mx, score[i]);
         mx = warp_max(mx);
-        for (int e = lane; e < n; e += 32) sum += expf(z[e] - mx);
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i)
+            if (lane + 32 * i < n) sum += score[i] = expf(score[i] - mx);
         sum = warp_sum(sum);
-        for (int e = lane; e < n; e += 32) z[e] = expf(z[e] - mx) / sum;
-    } else {
-        for (int e = lane; e < n; e += 32) {
-            const float v = z[e] + (p.router_bias != nullptr ? p.router_bias[e] : 0.f);
-            z[e] = p.scoring == 0 ? logistic(v) : v;
-        }
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i) score[i] = score[i] / sum;
+    } else if (p.scoring == 0) {
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i) score[i] = logistic(score[i]);
     }
-    for (int e = lane; e < n; e += 32) key[e] = order_of(z[e] + (p.correction != nullptr ? p.correction[e] : 0.f));
-    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < PLACES; ++i) {
+        const int e = lane + 32 * i;
+        key[i] = e < n ? order_of(score[i] + (p.correction != nullptr ? p.correction[e] : 0.f)) : 0u;
+    }
     if (p.n_groups > 1) {
         // a group's rank is its best choice score; a group is kept when fewer than keep_groups rank before it (ties: the lower one first)
         const int per = n / p.n_groups;
-        unsigned* best = reinterpret_cast<unsigned*>(rank);
+        unsigned* best = scratch + n;
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i)
+            if (lane + 32 * i < n) scratch[lane + 32 * i] = key[i];
+        __syncwarp();
         for (int g = lane; g < p.n_groups; g += 32) {
             unsigned m = 0u;
-            for (int e = g * per; e < (g + 1) * per; ++e) m = max(m, key[e]);
+            for (int e = g * per; e < (g + 1) * per; ++e) m = max(m, scratch[e]);
             best[g] = m;
         }
         __syncwarp();
-        for (int g = lane; g < p.n_groups; g += 32) {
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i) {
+            const int e = lane + 32 * i;
+            if (e >= n) continue;
+            const int g = e / per;
             int before = 0;
             for (int o = 0; o < p.n_groups; ++o) before += best[o] > best[g] || (best[o] == best[g] && o < g);
-            if (before >= p.keep_groups)
-                for (int e = g * per; e < (g + 1) * per; ++e) key[e] = 0u;
+            if (before >= p.keep_groups) key[i] = 0u;
         }
-        __syncwarp();
     }
-    float total = 0.f, first = 0.f;
+    chosen = 0;
+    weight = 0.f;
+    unsigned taken = 0u;            // this lane's places that are chosen
     for (int k = 0; k < p.top; ++k) {
         unsigned best = 0u;
-        int at = 0x7fffffff;
-        for (int e = lane; e < n; e += 32)
-            if (key[e] > best) {
-                best = key[e];
-                at = e;
+        int at = 0;
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i)
+            if (key[i] > best) {
+                best = key[i];
+                at = i;
             }
         const unsigned m = __reduce_max_sync(0xffffffffu, best);
-        at = (int)__reduce_min_sync(0xffffffffu, (unsigned)(best == m && m != 0u ? at : 0x7fffffff));
-        if (at >= n) {
-            // nothing is left that compares: the first output not chosen yet
-            at = 0;
-            for (bool taken = true; taken && at < n;) {
-                taken = false;
-                for (int j = 0; j < k; ++j) taken = taken || idx[j] == at;
-                if (taken) ++at;
-            }
-        }
-        __syncwarp();
-        const float s = z[at];
-        if (lane == 0) {
-            idx[k] = at;
-            weight[k] = s;
-            key[at] = 0u;
-        }
-        if (k == 0) first = s;
-        total += s;
-        __syncwarp();
-    }
-    if (lane == 0) {
-        if (p.scoring == 1) {               // the softmax over the chosen logits, the largest of which comes first
-            float sum = 0.f;
-            for (int k = 0; k < p.top; ++k) sum += weight[k] = expf(weight[k] - first);
-            for (int k = 0; k < p.top; ++k) weight[k] = weight[k] / sum * p.route_scale;
+        unsigned e;
+        if (m != 0u) {
+            e = __reduce_min_sync(0xffffffffu, best == m ? (unsigned)(lane + 32 * at) : 0xffffffffu);
         } else {
-            for (int k = 0; k < p.top; ++k) weight[k] = p.normalize ? weight[k] / (total + 1e-20f) * p.route_scale : weight[k] * p.route_scale;
+            // nothing is left that compares: the first output that is not chosen yet
+            const int free = __ffs((int)~taken) - 1;
+            e = __reduce_min_sync(0xffffffffu, free < PLACES && lane + 32 * free < n ? (unsigned)(lane + 32 * free) : 0xffffffffu);
+        }
+        const int place = (int)(e >> 5);
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < PLACES; ++i)
+            if (i == place) {
+                s = score[i];
+                if (lane == (int)(e & 31u)) {
+                    key[i] = 0u;
+                    taken |= 1u << i;
+                }
+            }
+        s = __shfl_sync(0xffffffffu, s, (int)(e & 31u));
+        if (lane == k) {
+            chosen = (int)e;
+            weight = s;
         }
     }
-    __syncwarp();
+    const bool mine = lane < p.top;
+    if (p.scoring == 1) {               // the softmax over the chosen logits
+        const float mx = warp_max(mine ? weight : -INFINITY), v = mine ? expf(weight - mx) : 0.f;
+        weight = v / warp_sum(v) * p.route_scale;
+    } else {
+        weight = p.normalize ? weight / (warp_sum(mine ? weight : 0.f) + 1e-20f) * p.route_scale : weight * p.route_scale;
+    }
 }
 
 // A float into the shared memory of the cluster's CTA `rank` (at the offset of `local`); a cluster barrier orders it before the reads.
@@ -258,59 +284,97 @@ __device__ __forceinline__ void st_cluster_f32(float* local, float v, uint32_t r
 
 // ---- up --------------------------------------------------------------------------------------------------------------------------------
 
+constexpr int TEAM = 4, TEAMS = L_WARPS / TEAM;             // warps that share an item's k
+
 struct UpShared {
-    float reduce[2][L_WARPS][16][LT + 1];       // the warps' sums of 16 rows (two sets in turn); before that the router's partial sums
+    float reduce[2][L_WARPS][16][LT + 1];       // the warps' sums of 16 rows (two sets in turn); before that the router's
     LayerPlan plan;
-    int idx[LT][L_MAX_PAIRS / LT];              // chosen outputs and their weights
-    float weight[LT][L_MAX_PAIRS / LT];
     float gate[LT];
-    unsigned mask[L_MAX_OUT];                   // the tokens that chose an expert; then its number among the active ones
-    unsigned votes[L_MAX_OUT / 32];
-    unsigned char columns[L_MAX_PAIRS][LT], n_columns[L_MAX_PAIRS];         // the tokens of an active expert, in their order
+    unsigned long long choice[L_MAX_OUT];       // which of a token's choices an expert is, four bits a token
+    unsigned tokens[L_MAX_OUT];                 // the tokens that chose an expert
 };
 
-// This CTA's rows of the router against all tokens, into every CTA's z [LT][z_row].  The warps share k; within a warp lanes are TL tokens x 32 / TL parts of its k.
+// This CTA's rows of the router against all tokens, into every CTA's z [LT][z_row].  Sixteen rows at a time; the warps share k: a warp takes 128 k of the
+// sixteen rows as three bfloat16 each.
 __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared& sh, float* z, int z_row, int rank, int cluster) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int rows = p.n_out + p.shared_gate, per = (rows + cluster - 1) / cluster, first = rank * per, mine = max(0, min(per, rows - first));
-    int lanes = 1;
-    while (lanes < p.n_tokens) lanes *= 2;
-    const int t = lane & (lanes - 1), part = lane / lanes, parts = 32 / lanes;
-    const bf16* x = p.x + (long long)min(t, p.n_tokens - 1) * p.ldx;
-    float* sums = &sh.reduce[0][0][0][0];                       // [warp][4 rows][LT]
-    for (int r0 = 0; r0 < mine; r0 += 4) {
-        float dot[4] = {};
-        const float* w[4];
+    const int tiles = (per + 15) / 16, n_chunks = (p.width + LK - 1) / LK;
+    const bool second = p.n_tokens > 8;
+    bool met = false;
+    for (int tile = 0; tile < tiles; ++tile) {
+        float acc[2][4] = {};
+        const int r0 = tile * 16 + g, r1 = r0 + 8;
+        const float *w0 = p.router + (long long)(first + min(r0, mine - 1)) * p.width, *w1 = p.router + (long long)(first + min(r1, mine - 1)) * p.width;
+        for (int chunk = warp; chunk < n_chunks && tile * 16 < mine; chunk += L_WARPS) {
+            const int k0 = chunk * LK + (lane & 3) * 8;
+            float4 a[4][2][2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = p.router + (long long)(first + min(r0 + j, mine - 1)) * p.width;
-#pragma unroll 2
-        for (int k = (warp * parts + part) * 8; k < p.width; k += L_WARPS * parts * 8) {
-            const uint4 raw = *reinterpret_cast<const uint4*>(x + k);
-            const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+            for (int s = 0; s < 4; ++s)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float4 wa = *reinterpret_cast<const float4*>(w[j] + k), wb = *reinterpret_cast<const float4*>(w[j] + k + 4);
-                const float wv[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
+                for (int h = 0; h < 2; ++h) {
+                    const int k = k0 + s * 32;
+                    a[s][0][h] = k < p.width ? *reinterpret_cast<const float4*>(w0 + k + 4 * h) : make_float4(0, 0, 0, 0);
+                    a[s][1][h] = k < p.width ? *reinterpret_cast<const float4*>(w1 + k + 4 * h) : make_float4(0, 0, 0, 0);
+                }
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dot[j] = fmaf(wv[i], __uint_as_float((i & 1) ? words[i >> 1] & 0xffff0000u : words[i >> 1] << 16), dot[j]);
+            for (int s = 0; s < 4; ++s) {
+                uint4 x[2];
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int k = k0 + s * 32, t = n * 8 + g;
+                    x[n] = k < p.width && t < p.n_tokens ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
+                }
+                float v[2][8];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    v[r][0] = a[s][r][0].x, v[r][1] = a[s][r][0].y, v[r][2] = a[s][r][0].z, v[r][3] = a[s][r][0].w;
+                    v[r][4] = a[s][r][1].x, v[r][5] = a[s][r][1].y, v[r][6] = a[s][r][1].z, v[r][7] = a[s][r][1].w;
+                }
+#pragma unroll
+                for (int part = 0; part < 3; ++part) {
+                    uint32_t w[2][4];
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            w[r][i] = pack_bf16(v[r][2 * i], v[r][2 * i + 1]);
+                            v[r][2 * i] -= __uint_as_float(w[r][i] << 16);
+                            v[r][2 * i + 1] -= __uint_as_float(w[r][i] & 0xffff0000u);
+                        }
+                    const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
+#pragma unroll
+                    for (int n = 0; n < 2; ++n) {
+                        if (n == 1 && !second) break;
+                        mma_bf16_16816(acc[n], a0, x[n].x, x[n].y);
+                        mma_bf16_16816(acc[n], a1, x[n].z, x[n].w);
+                    }
+                }
             }
         }
+        float(*sums)[LT + 1] = sh.reduce[tile & 1][warp];
+        const int col = (lane & 3) * 2;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            for (int o = lanes; o < 32; o *= 2) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
-            if (part == 0) sums[(warp * 4 + j) * LT + t] = dot[j];
+        for (int n = 0; n < 2; ++n) {
+            sums[g][n * 8 + col] = acc[n][0];
+            sums[g][n * 8 + col + 1] = acc[n][1];
+            sums[g + 8][n * 8 + col] = acc[n][2];
+            sums[g + 8][n * 8 + col + 1] = acc[n][3];
         }
         __syncthreads();
-        if (threadIdx.x < 4 * LT) {
-            const int j = threadIdx.x / LT, tt = threadIdx.x % LT;
-            if (r0 + j < mine && tt < p.n_tokens) {
+        if (!met) {                     // every CTA of the cluster has begun before its shared memory is written from another
+            asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+            met = true;
+        }
+        if (threadIdx.x < 16 * LT) {
+            const int r = threadIdx.x / LT, t = threadIdx.x % LT;
+            if (tile * 16 + r < mine && t < p.n_tokens) {
                 float v = 0.f;
 #pragma unroll
-                for (int i = 0; i < L_WARPS; ++i) v += sums[(i * 4 + j) * LT + tt];
-                for (int c = 0; c < cluster; ++c) st_cluster_f32(z + tt * z_row + first + r0 + j, v, (uint32_t)c);
+                for (int i = 0; i < L_WARPS; ++i) v += sh.reduce[tile & 1][i][r][t];
+                for (int c = 0; c < cluster; ++c) st_cluster_f32(z + t * z_row + first + tile * 16 + r, v, (uint32_t)c);
             }
         }
-        __syncthreads();
     }
 }
 
@@ -318,76 +382,77 @@ template <bool CODES>
 __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerArgs p) {
     extern __shared__ __align__(16) unsigned char up_smem[];
     UpShared& sh = *reinterpret_cast<UpShared*>(up_smem);
-    float* z = reinterpret_cast<float*>(up_smem + sizeof(UpShared));                     // [LT][z_row]: logits; behind them keys and group ranks
+    float* z = reinterpret_cast<float*>(up_smem + sizeof(UpShared));                     // [LT][z_row]: logits, later the weights of what was chosen
     const int z_row = p.n_out + 1;
-    unsigned* keys = reinterpret_cast<unsigned*>(z + LT * z_row);                        // [L_WARPS][n_out + n_groups]
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cluster = L_CLUSTER;
+    unsigned* scratch = reinterpret_cast<unsigned*>(z + LT * z_row);                     // [L_WARPS][n_out + n_groups], with groups
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    for (int e = threadIdx.x; e < p.n_out; e += L_THREADS) {
+        sh.tokens[e] = 0u;
+        sh.choice[e] = 0ull;
+    }
     pdl_wait();
-    for (int e = threadIdx.x; e < p.n_out; e += L_THREADS) sh.mask[e] = 0u;
-    cluster_sync_all();             // (every CTA of the cluster has begun before its shared memory is written from another)
-    router_logits(p, sh, z, z_row, blockIdx.x % cluster, cluster);
+    router_logits(p, sh, z, z_row, blockIdx.x % L_CLUSTER, L_CLUSTER);
     cluster_sync_all();
 
     if (warp < p.n_tokens) {
-        unsigned* key = keys + warp * (p.n_out + p.n_groups);
-        choose(p, z + warp * z_row, key, reinterpret_cast<float*>(key + p.n_out), sh.idx[warp], sh.weight[warp], lane);
+        int e;
+        float w;
+        unsigned* mine = scratch + warp * (p.n_out + p.n_groups);
+        if (p.n_out <= 128) choose<4>(p, z + warp * z_row, mine, lane, e, w);
+        else choose<L_MAX_OUT / 32>(p, z + warp * z_row, mine, lane, e, w);
+        const bool have = lane < p.top, real = have && e < p.n_real;
+        const float identity = warp_sum(have && !real ? w : 0.f);
+        if (real) {
+            atomicOr(&sh.tokens[e], 1u << warp);
+            atomicOr(&sh.choice[e], (unsigned long long)lane << (4 * warp));
+        }
         if (lane == 0) {
             sh.gate[warp] = p.shared_gate ? logistic(z[warp * z_row + p.n_out]) : 1.f;
-            float w = 0.f;
-            for (int k = 0; k < p.top; ++k) {
-                const int e = sh.idx[warp][k];
-                if (e < p.n_real) atomicOr(&sh.mask[e], 1u << warp);
-                else w += sh.weight[warp][k];
-            }
-            sh.plan.identity[warp] = w;
+            sh.plan.identity[warp] = identity;
         }
+        __syncwarp();
+        if (real) z[warp * z_row + e] = w;
     }
     __syncthreads();
-    // the experts that some token chose, ascending: 32 a warp's vote, then their places
-    const int groups32 = (p.n_real + 31) / 32;
-    for (int c = warp; c < groups32; c += L_WARPS) {
-        const int e = c * 32 + lane;
-        const unsigned votes = __ballot_sync(0xffffffffu, e < p.n_real && sh.mask[e] != 0u);
-        if (lane == 0) sh.votes[c] = votes;
-    }
-    for (int i = threadIdx.x; i < L_MAX_PAIRS * LT; i += L_THREADS) sh.plan.slot[i / LT][i % LT] = -1;
-    __syncthreads();
+    // the experts that some token chose, ascending: every warp counts them all, 32 at a vote, and writes down its own
     int n_active = 0;
-    for (int c = 0; c < groups32; ++c) {
-        const unsigned votes = sh.votes[c];
-        if (warp == c % L_WARPS && (votes >> lane & 1u)) sh.plan.expert[n_active + __popc(votes & ((1u << lane) - 1u))] = c * 32 + lane;
+    for (int c = 0; c * 32 < p.n_real; ++c) {
+        const int e = c * 32 + lane;
+        const unsigned tokens = e < p.n_real ? sh.tokens[e] : 0u, votes = __ballot_sync(0xffffffffu, tokens != 0u);
+        if (warp == c % L_WARPS && tokens != 0u) {
+            ActiveExpert& a = sh.plan.of[n_active + __popc(votes & ((1u << lane) - 1u))];
+            unsigned long long list = 0ull;
+            int n = 0;
+            for (unsigned m = tokens; m != 0u; m &= m - 1u, ++n) list |= (unsigned long long)(__ffs((int)m) - 1) << (4 * n);
+            a.expert = e;
+            a.tokens = tokens;
+            a.list = list;
+            a.choice = sh.choice[e];
+        }
         n_active += __popc(votes);
     }
     if (threadIdx.x == 0) sh.plan.n_active = n_active;
     __syncthreads();
-    for (int a = threadIdx.x; a < n_active; a += L_THREADS) {
-        const int e = sh.plan.expert[a];
-        int n = 0;
-        for (unsigned m = sh.mask[e]; m != 0u; m &= m - 1u) sh.columns[a][n++] = (unsigned char)(__ffs((int)m) - 1);
-        sh.n_columns[a] = (unsigned char)n;
-        sh.mask[e] = (unsigned)a;
+    if (blockIdx.x == 0) {
+        const int words = (int)(offsetof(LayerPlan, of) + (size_t)n_active * sizeof(ActiveExpert)) / 8;
+        for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(p.plan)[i] = reinterpret_cast<const unsigned long long*>(&sh.plan)[i];
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < p.n_tokens * p.top; i += L_THREADS) {
-        const int t = i / p.top, e = sh.idx[t][i % p.top];
-        if (e < p.n_real) sh.plan.slot[sh.mask[e]][t] = (short)i;
-    }
-    __syncthreads();
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i < (int)(sizeof(LayerPlan) / 4); i += L_THREADS) reinterpret_cast<int*>(p.plan)[i] = reinterpret_cast<const int*>(&sh.plan)[i];
     pdl_trigger();
 
-    // items: eight features of the shared expert, then of every active one; a warp takes chunks warp, warp + L_WARPS, .. of their k, a round each
+    // items: eight features of the shared expert, then of every active one; a team's warp takes every TEAM-th chunk of their k, a round each
     const int shared_items = p.inner_shared / 8, per_expert = p.inner / 8, n_items = shared_items + n_active * per_expert;
-    const int n_chunks = (p.width + LK - 1) / LK, rounds = (n_chunks + L_WARPS - 1) / L_WARPS;
+    const int n_chunks = (p.width + LK - 1) / LK, rounds = (n_chunks + TEAM - 1) / TEAM;
+    const int team = warp / TEAM, member = warp % TEAM, stride = gridDim.x * TEAMS, first = team * gridDim.x + blockIdx.x;
+    auto active_of = [&](int item) { return quotient(item - shared_items, p.per_expert_magic); };
     auto load = [&](Chunk<CODES>& c, int item, int round) {
         if (item >= n_items) return;
         const bool own = item >= shared_items;
-        const int a = own ? (item - shared_items) / per_expert : 0, f = (own ? item - shared_items - a * per_expert : item) * 8 + g, e = own ? sh.plan.expert[a] : 0;
+        const int a = own ? active_of(item) : 0, f = (own ? item - shared_items - a * per_expert : item) * 8 + g, e = own ? sh.plan.of[a].expert : 0;
         const LayerMatrix& m = own ? p.up : p.shared_up;
-        const int il = own ? p.interleave : p.interleave_shared, chunk = warp + round * L_WARPS;
+        const int il = own ? p.interleave : p.interleave_shared, chunk = member + round * TEAM;
         // row g of the 16 is a gate row, row g + 8 the row of the linear branch of the same feature
-        const int r0 = il > 0 ? f / il * 2 * il + f % il : f, r1 = r0 + (il > 0 ? il : own ? p.inner : p.inner_shared);
+        const int r0 = il == 0 ? f : il == 4 ? 2 * f - (f & 3) : f / il * 2 * il + f % il, r1 = r0 + (il > 0 ? il : own ? p.inner : p.inner_shared);
         const unsigned char* base = m.w + e * m.stack_bytes;
         load_chunk<CODES>(c, base + r0 * m.row_bytes, base + r1 * m.row_bytes, chunk * LK, p.width, lane);
         if (CODES) {
@@ -398,76 +463,88 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
     };
     constexpr int AHEAD = Chunk<CODES>::AHEAD;
     Chunk<CODES> held[AHEAD];
-    int to_load = blockIdx.x, load_round = 0;
+    int to_load = first, load_round = 0;
     auto load_next = [&](Chunk<CODES>& c) {
         load(c, to_load, load_round);
         if (++load_round == rounds) {
             load_round = 0;
-            to_load += gridDim.x;
+            to_load += stride;
         }
     };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) load_next(held[i]);
     float acc[2][4];
-    const bf16* rows[2];
-    const int to[2] = {0, 1};
+    const bf16 *row0 = nullptr, *row1 = nullptr;
     int n_cols = 0, set = 0;
-    for (int item = blockIdx.x, round = 0; item < n_items;) {
+    for (int item = first, round = 0; item < n_items;) {
 #pragma unroll
         for (int i = 0; i < AHEAD; ++i) {
             if (item >= n_items) break;
             const bool own = item >= shared_items;
-            const int a = own ? (item - shared_items) / per_expert : 0;
+            const int a = own ? active_of(item) : 0;
             if (round == 0) {
                 // this lane's columns: the tokens that chose the expert, or all for the shared one
-                n_cols = own ? sh.n_columns[a] : p.n_tokens;
+                const unsigned long long list = own ? sh.plan.of[a].list : 0xfedcba9876543210ull;
+                n_cols = own ? __popc(sh.plan.of[a].tokens) : p.n_tokens;
+                row0 = g < n_cols ? p.x + (long long)((list >> (4 * g)) & 15) * p.ldx : nullptr;
+                row1 = 8 + g < n_cols ? p.x + (long long)((list >> (32 + 4 * g)) & 15) * p.ldx : nullptr;
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int c = n * 8 + g;
-                    rows[n] = c < n_cols ? p.x + (own ? sh.columns[a][c] : c) * p.ldx : nullptr;
+                for (int n = 0; n < 2; ++n)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
-                }
             }
-            const bool second = n_cols > 8;
-            const int chunk = warp + round * L_WARPS;
+            const int chunk = member + round * TEAM, k0 = chunk * LK;
             if (chunk < n_chunks) {
-                const bf16* at[2] = {rows[0] != nullptr ? rows[0] + chunk * LK : nullptr, rows[1] != nullptr ? rows[1] + chunk * LK : nullptr};
-                multiply<CODES, 2>(held[i], at, chunk * LK, p.width, lane, acc, to, second);
+                const bf16* at[1] = {row0 != nullptr ? row0 + k0 : nullptr};
+                multiply<CODES, 1>(held[i], at, p.width - k0, lane, acc[0]);
+                if (n_cols > 8) {
+                    const bf16* at1[1] = {row1 != nullptr ? row1 + k0 : nullptr};
+                    multiply<CODES, 1>(held[i], at1, p.width - k0, lane, acc[1]);
+                }
             }
             load_next(held[i]);
             if (++round < rounds) continue;
             const int f0 = (own ? item - shared_items - a * per_expert : item) * 8;
             round = 0;
-            item += gridDim.x;
+            item += stride;
             float(*mine)[LT + 1] = sh.reduce[set][warp];
             const int col = (lane & 3) * 2;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                if (n == 1 && !second) break;
+                if (n == 1 && n_cols <= 8) break;
                 mine[g][n * 8 + col] = acc[n][0];
                 mine[g][n * 8 + col + 1] = acc[n][1];
                 mine[g + 8][n * 8 + col] = acc[n][2];
                 mine[g + 8][n * 8 + col + 1] = acc[n][3];
             }
-            __syncthreads();            // (two sets in turn: nobody writes this one again before all have come to the next item's barrier)
-            const int f = threadIdx.x & 7, c = threadIdx.x >> 3;
+            // (two sets in turn: nobody writes this one again before the team has come to the next item's barrier)
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TEAM) : "memory");
+            const int f = lane & 7, c = member * 4 + (lane >> 3);
             if (c < n_cols) {
                 float gate = 0.f, lin = 0.f;
 #pragma unroll
-                for (int w = 0; w < L_WARPS; ++w) {
-                    gate += sh.reduce[set][w][f][c];
-                    lin += sh.reduce[set][w][f + 8][c];
+                for (int w = 0; w < TEAM; ++w) {
+                    gate += sh.reduce[set][team * TEAM + w][f][c];
+                    lin += sh.reduce[set][team * TEAM + w][f + 8][c];
                 }
                 if (p.limit != INFINITY) {          // (a NaN stays one)
                     gate = gate > p.limit ? p.limit : gate;
                     lin = lin > p.limit ? p.limit : lin < -p.limit ? -p.limit : lin;
                 }
-                const int t = own ? sh.columns[a][c] : c, pair = own ? (int)sh.plan.slot[a][t] : p.n_tokens * p.top + t;
-                const float w = own ? sh.weight[t][pair - t * p.top] : sh.gate[t];
+                int row, t = c;
+                float w;
+                if (own) {
+                    const ActiveExpert& ex = sh.plan.of[a];
+                    t = (int)(ex.list >> (4 * c)) & 15;
+                    row = t * p.top + ((int)(ex.choice >> (4 * t)) & 15);
+                    w = z[t * z_row + ex.expert];
+                } else {
+                    row = p.n_tokens * p.top + t;
+                    w = sh.gate[t];
+                }
                 const float v = glu_gate(gate, p.slope) * (lin + p.shift) * w;
                 const bf16 hi = __float2bfloat16_rn(v);
-                const long long at = (long long)pair * p.h_row + f0 + f;
+                const long long at = (long long)row * p.h_row + f0 + f;
                 p.h_hi[at] = hi;
                 p.h_lo[at] = __float2bfloat16_rn(v - __bfloat162float(hi));
             }
@@ -492,17 +569,19 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int rank = blockIdx.x % parts, clusters = gridDim.x / parts, n_groups = (p.width + 15) / 16;
     pdl_wait();
-    for (int i = threadIdx.x; i < (int)(sizeof(LayerPlan) / 4); i += L_THREADS) reinterpret_cast<int*>(&sh.plan)[i] = reinterpret_cast<const int*>(p.plan)[i];
+    // (as much of the plan as the step can have: its length comes with it)
+    const int words = (int)(offsetof(LayerPlan, of) + (size_t)min(p.n_tokens * p.top, p.n_real) * sizeof(ActiveExpert)) / 8;
+    for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(&sh.plan)[i] = reinterpret_cast<const unsigned long long*>(p.plan)[i];
     __syncthreads();
     pdl_trigger();
     const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK, n_chunks = shared_chunks + sh.plan.n_active * own_chunks;
+    auto active_of = [&](int chunk) { return quotient(chunk - shared_chunks, p.own_chunks_magic); };
     const int step = parts * L_WARPS, first = rank * L_WARPS + warp;
-    const bool second = p.n_tokens > 8;
     auto load = [&](Chunk<CODES>& c, int group, int chunk) {
         const bool own = chunk >= shared_chunks;
-        const int a = own ? (chunk - shared_chunks) / own_chunks : 0, kb = own ? (chunk - shared_chunks) - a * own_chunks : chunk;
+        const int a = own ? active_of(chunk) : 0, kb = own ? (chunk - shared_chunks) - a * own_chunks : chunk;
         const bool some = chunk < n_chunks;
-        const int e = own && some ? sh.plan.expert[a] : 0;
+        const int e = own && some ? sh.plan.of[a].expert : 0;
         const LayerMatrix& m = own ? p.down : p.shared_down;
         const int r0 = min(group * 16 + g, p.width - 1), r1 = min(group * 16 + g + 8, p.width - 1);
         const unsigned char* base = m.w + e * m.stack_bytes;
@@ -517,16 +596,18 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     auto work = [&](const Chunk<CODES>& c, int chunk) {
         if (chunk >= n_chunks) return;
         const bool own = chunk >= shared_chunks;
-        const int a = own ? (chunk - shared_chunks) / own_chunks : 0, kb = own ? (chunk - shared_chunks) - a * own_chunks : chunk;
-        const bf16* rows[4];
-        const int to[4] = {0, 0, 1, 1};
+        const int a = own ? active_of(chunk) : 0, kb = own ? (chunk - shared_chunks) - a * own_chunks : chunk;
+        const unsigned tokens = own ? sh.plan.of[a].tokens : (1u << p.n_tokens) - 1u;
+        const unsigned long long choice = own ? sh.plan.of[a].choice : 0ull;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const int t = n * 8 + g, slot = t < p.n_tokens ? own ? (int)sh.plan.slot[a][t] : p.n_tokens * p.top + t : -1;
-            rows[2 * n] = slot >= 0 ? p.h_hi + (long long)slot * p.h_row + kb * LK : nullptr;
-            rows[2 * n + 1] = slot >= 0 ? p.h_lo + (long long)slot * p.h_row + kb * LK : nullptr;
+            if ((tokens >> (8 * n) & 0xffu) == 0u) continue;                // (none of these eight columns)
+            const int t = n * 8 + g, row = own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+            const long long at = (long long)row * p.h_row + kb * LK;
+            const bool have = tokens >> t & 1u;
+            const bf16* rows[2] = {have ? p.h_hi + at : nullptr, have ? p.h_lo + at : nullptr};
+            multiply<CODES, 2>(c, rows, (own ? p.inner : p.inner_shared) - kb * LK, lane, acc[n]);
         }
-        multiply<CODES, 4>(c, rows, kb * LK, own ? p.inner : p.inner_shared, lane, acc, to, second);
     };
     constexpr int AHEAD = Chunk<CODES>::AHEAD;
     const int rounds = max(1, (n_chunks + step - 1) / step), turns = (rounds + AHEAD - 1) / AHEAD * AHEAD;       // (empty chunks fill the last turn)
@@ -579,7 +660,9 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     }
 }
 
-size_t up_smem_bytes(const LayerArgs& p) { return sizeof(UpShared) + (size_t)LT * (p.n_out + 1) * 4 + (size_t)L_WARPS * (p.n_out + p.n_groups) * 4; }
+size_t up_smem_bytes(const LayerArgs& p) {
+    return sizeof(UpShared) + (size_t)LT * (p.n_out + 1) * 4 + (p.n_groups > 1 ? (size_t)L_WARPS * (p.n_out + p.n_groups) * 4 : 0);
+}
 
 // Clusters of the up kernel that the device holds at once (asked for once a device): a grid that needs a second round would route twice.
 template <bool CODES> int up_clusters(size_t smem) {
@@ -652,7 +735,7 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
         a->scoring > 2 || a->n_groups < 1 || n_out % a->n_groups != 0 || a->keep_groups < 1 || a->keep_groups > a->n_groups ||
         a->top > a->keep_groups * (n_out / a->n_groups) || a->width <= 0 || a->width % unit != 0 || a->inner <= 0 || a->inner % unit != 0 || a->inner_shared % unit != 0 ||
         a->inner_shared < 0 || (a->shared_gate && !shared) || a->interleave < 0 || (a->interleave > 0 && a->inner % a->interleave != 0) || a->interleave_shared < 0 ||
-        (a->interleave_shared > 0 && a->inner_shared % a->interleave_shared != 0) || a->width > (1 << 24) || a->inner > (1 << 24) || a->inner_shared > (1 << 24))
+        (a->interleave_shared > 0 && a->inner_shared % a->interleave_shared != 0) || a->width > MOST_K || a->inner > MOST_K || a->inner_shared > MOST_K)
         return RLIS_ERR_UNSUPPORTED;
     // codes: the eight rows that a load instruction takes lie in one block of rows
     if (codes && ((a->interleave > 0 && a->interleave != 4 && a->interleave % 8 != 0) || (a->interleave_shared > 0 && a->interleave_shared != 4 && a->interleave_shared % 8 != 0)))
@@ -699,6 +782,9 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     p.h_hi = reinterpret_cast<bf16*>(static_cast<unsigned char*>(a->workspace) + (sizeof(LayerPlan) + 15) / 16 * 16);
     p.h_lo = p.h_hi + (long long)(a->n_tokens * a->top + a->n_tokens) * p.h_row;
     p.out = static_cast<bf16*>(a->out);
+    auto magic = [](int d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; };
+    p.per_expert_magic = magic(a->inner / 8);
+    p.own_chunks_magic = magic((a->inner + LK - 1) / LK);
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (up_smem_bytes(p) > 200 * 1024) return RLIS_ERR_UNSUPPORTED;
