@@ -7,10 +7,11 @@
 // With so few tokens the layer is a stream of the chosen experts' weights from memory (8 tokens, 4 of 32 experts of 2,048 x 1,024 and a shared one: 278 MB, 42 us
 // at the rate of a copy).  So every weight is read once, by 16-byte loads of 16 rows side by side straight into the registers of mma.sync m16n8k16, no
 // shared memory between: a sum over k may take k in any order, so a thread's 16 bytes of a row, eight neighbouring k, serve as its k slots of two
-// instructions, and the tokens' rows, which stay in the first-level cache, are read in the same order.  A warp takes 128 k of 16 rows at a time (a chunk, a
-// block's edge; for weights in e4m3 blocks a chunk's sums are scaled before they join the others) and has the next chunks, of the next rows if need be, on
-// their way while it works on one: 128 KB an SM (96 KB of codes) are in flight.  Four warps (up) or a CTA's sixteen (down) take different k of the same rows
-// and add their sums in shared memory in the order of the warps, so results do not depend on timing.
+// instructions, and the tokens' rows, which stay in the caches, are read in the same order.  A warp takes 128 k of 16 rows at a time (a chunk, a block's edge; for
+// weights in e4m3 blocks a chunk's sums are scaled before they join the others) and has the next chunks, of the next rows if need be, on their way while it
+// works on one.  Four warps (up) or a CTA's sixteen (down) take different k of the same rows and add their sums in shared memory in the order of the
+// warps, so results do not depend on timing.  (Chunks by asynchronous copies through 180 KB of shared memory: 65 -> 99 us for the layer above; the first-level
+// cache that is left holds no tokens' rows.)
 //
 // Routing sits in the up kernel: the CTAs of a cluster share the router's rows, hand each other the logits (distributed shared memory), and each chooses
 // for all tokens itself: no launch of its own, no grid-wide barrier, no workspace but h and the plan, which the first CTA leaves for the down kernel.  The
@@ -84,82 +85,77 @@ __device__ __forceinline__ uint4 stream16(const void* p) {
 // 128 k of rows g and g + 8 of a warp's 16 (g = lane / 4): lane % 4 holds every fourth 16 bytes.
 template <bool CODES> struct Chunk {
     static constexpr int STEPS = CODES ? 2 : 4;
-    static constexpr int AHEAD = CODES ? 3 : 2;         // chunks that a warp holds or waits for
     uint4 a[STEPS][2];
     float scale[2];             // codes: of row g, of row g + 8
 };
+// `row0`, `row1`: this lane's rows from the chunk's first k on, of which `left` are there.
 template <bool CODES>
-__device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char* row0, const unsigned char* row1, int k0, int K, int lane) {
-    constexpr int PER = CODES ? 16 : 8;             // k in 16 bytes
+__device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char* row0, const unsigned char* row1, int left, int lane) {
 #pragma unroll
     for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
-        const int k = k0 + s * 4 * PER + (lane & 3) * PER;
-        const bool in = k < K;
-        c.a[s][0] = in ? stream16(row0 + (long long)k * (CODES ? 1 : 2)) : make_uint4(0, 0, 0, 0);
-        c.a[s][1] = in ? stream16(row1 + (long long)k * (CODES ? 1 : 2)) : make_uint4(0, 0, 0, 0);
+        const int at = (s * 4 + (lane & 3)) * 16;
+        const bool in = (CODES ? at : at / 2) < left;
+        c.a[s][0] = in ? stream16(row0 + at) : make_uint4(0, 0, 0, 0);
+        c.a[s][1] = in ? stream16(row1 + at) : make_uint4(0, 0, 0, 0);
     }
 }
 
-// Four codes as bfloat16: the even ones and the odd ones.  An e4m3's bits moved to a bfloat16's places are its value times 2^-120, subnormal ones included.
-__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& even, uint32_t& odd) {
+// Four codes as bfloat16, in their order.  An e4m3's bits moved to a bfloat16's places are its value times 2^-120, subnormal ones included.
+__device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& first, uint32_t& last) {
     const __nv_bfloat162 up = __float2bfloat162_rn(E4M3_TO_BF16);
     auto place = [&](uint32_t v) {
         const uint32_t bits = ((v >> 4) & 0x07f007f0u) | (v & 0x80008000u);
         const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), up);
         return *reinterpret_cast<const uint32_t*>(&r);
     };
-    even = place(w << 8);
-    odd = place(w);
+    first = place(__byte_perm(w, 0u, 0x1404));          // bytes 0 and 1 into the high bytes of the halves
+    last = place(__byte_perm(w, 0u, 0x3424));
 }
 
-// d += chunk * the sum of a column's rows: `rows` are this lane's column's (lane / 4) rows of bfloat16 from the chunk's first k on, or null (a column of zeros);
-// `left`: k from there on.  All of the rows are asked for before the first is used.
-template <bool CODES, int ROWS>
-__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const bf16* const (&rows)[ROWS], int left, int lane, float (&d)[4]) {
-    constexpr int PER = CODES ? 16 : 8, VECS = PER / 8, STEPS = Chunk<CODES>::STEPS;
-    uint4 b[STEPS][ROWS][VECS];
+// This lane's part of a column's row over a chunk: the vectors of bfloat16 that its A vectors meet.
+template <bool CODES> struct Column {
+    static constexpr int VECS = CODES ? 2 : 1;
+    uint4 b[Chunk<CODES>::STEPS][VECS];
+};
+// `row`: the column's row from this lane's first k of the chunk on, of which `left` are there; not `have`: a column of zeros.
+template <bool CODES> __device__ __forceinline__ void load_column(Column<CODES>& c, const bf16* row, int left, bool have) {
+    constexpr int PER = CODES ? 16 : 8;
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s)
+    for (int s = 0; s < Chunk<CODES>::STEPS; ++s)
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i)
+        for (int v = 0; v < Column<CODES>::VECS; ++v) {
+            const int k = s * 4 * PER + v * 8;
+            c.b[s][v] = have && k < left ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
+        }
+}
+// acc += chunk * the sum of the columns (COLS of each of eight tokens).  Neighbouring instructions add to different sums: one waits some 35 cycles for the one before
+// it on the same.
+template <bool CODES, int COLS>
+__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<CODES> (&cols)[COLS], float (&acc)[4]) {
+    float part[2][4] = {};
 #pragma unroll
-            for (int v = 0; v < VECS; ++v) {
-                const int k = (s * 4 + (lane & 3)) * PER + v * 8;
-                b[s][i][v] = rows[i] != nullptr && k < left ? *reinterpret_cast<const uint4*>(rows[i] + k) : make_uint4(0, 0, 0, 0);
-            }
-    float part[4] = {};
-    float(&sum)[4] = CODES ? part : d;
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
+    for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
         const uint32_t r0[4] = {c.a[s][0].x, c.a[s][0].y, c.a[s][0].z, c.a[s][0].w}, r1[4] = {c.a[s][1].x, c.a[s][1].y, c.a[s][1].z, c.a[s][1].w};
-        if constexpr (CODES) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t a[4];
+        for (int j = 0; j < (CODES ? 4 : 2); ++j) {
+            uint32_t a[4];
+            if constexpr (CODES) {
                 widen_codes(r0[j], a[0], a[2]);
                 widen_codes(r1[j], a[1], a[3]);
-#pragma unroll
-                for (int i = 0; i < ROWS; ++i) {
-                    const uint4 v = b[s][i][j / 2];
-                    const uint32_t x0 = j & 1 ? v.z : v.x, x1 = j & 1 ? v.w : v.y;
-                    mma_bf16_16816(sum, a, __byte_perm(x0, x1, 0x5410), __byte_perm(x0, x1, 0x7632));
-                }
+            } else {
+                a[0] = r0[2 * j], a[1] = r1[2 * j], a[2] = r0[2 * j + 1], a[3] = r1[2 * j + 1];
             }
-        } else {
-            const uint32_t a0[4] = {r0[0], r1[0], r0[1], r1[1]}, a1[4] = {r0[2], r1[2], r0[3], r1[3]};
 #pragma unroll
-            for (int i = 0; i < ROWS; ++i) {
-                mma_bf16_16816(sum, a0, b[s][i][0].x, b[s][i][0].y);
-                mma_bf16_16816(sum, a1, b[s][i][0].z, b[s][i][0].w);
+            for (int i = 0; i < COLS; ++i) {
+                const uint4 b = cols[i].b[s][CODES ? j / 2 : 0];
+                mma_bf16_16816(part[(j + i) & 1], a, j & 1 ? b.z : b.x, j & 1 ? b.w : b.y);
             }
         }
     }
-    if constexpr (CODES) {
-        d[0] = fmaf(part[0], c.scale[0], d[0]);
-        d[1] = fmaf(part[1], c.scale[0], d[1]);
-        d[2] = fmaf(part[2], c.scale[1], d[2]);
-        d[3] = fmaf(part[3], c.scale[1], d[3]);
-    }
+    acc[0] = fmaf(part[0][0] + part[1][0], CODES ? c.scale[0] : 1.f, acc[0]);
+    acc[1] = fmaf(part[0][1] + part[1][1], CODES ? c.scale[0] : 1.f, acc[1]);
+    acc[2] = fmaf(part[0][2] + part[1][2], CODES ? c.scale[1] : 1.f, acc[2]);
+    acc[3] = fmaf(part[0][3] + part[1][3], CODES ? c.scale[1] : 1.f, acc[3]);
 }
 
 // ---- the choice ------------------------------------------------------------------------------------------------------------------------
@@ -172,103 +168,82 @@ __device__ __forceinline__ unsigned order_of(float v) {
 }
 __device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
 
-// One warp chooses for one token: z [n_out] logits in; the scores' bits stay in the lanes (output lane + 32 i in place i).  `scratch` [n_out + n_groups] for groups.
-// Lane k ends with choice k and its weight.
-template <int PLACES>
-__device__ __forceinline__ void choose(const LayerArgs& p, const float* z, unsigned* scratch, int lane, int& chosen, float& weight) {
+// One warp chooses for one token: z [n_out] logits in, scores out; `key` [n_out + n_groups] is scratch.  Lane k ends with choice k and its weight.
+__device__ __forceinline__ void choose(const LayerArgs& p, float* z, unsigned* key, int lane, int& chosen, float& weight) {
     const int n = p.n_out;
-    float score[PLACES];
-    unsigned key[PLACES];
-#pragma unroll
-    for (int i = 0; i < PLACES; ++i) {
-        const int e = lane + 32 * i;
-        score[i] = e < n ? z[e] + (p.router_bias != nullptr ? p.router_bias[e] : 0.f) : -INFINITY;
-    }
+    float mx = -INFINITY;
     if (p.scoring == 2) {
-        float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < PLACES; ++i) mx = fmaxf(mx, score[i]);
+#pragma unroll 1
+        for (int e = lane; e < n; e += 32) mx = fmaxf(mx, z[e] + (p.router_bias != nullptr ? p.router_bias[e] : 0.f));
         mx = warp_max(mx);
-#pragma unroll
-        for (int i = 0; i < PLACES; ++i)
-            if (lane + 32 * i < n) sum += score[i] = expf(score[i] - mx);
-        sum = warp_sum(sum);
-#pragma unroll
-        for (int i = 0; i < PLACES; ++i) score[i] = score[i] / sum;
-    } else if (p.scoring == 0) {
-#pragma unroll
-        for (int i = 0; i < PLACES; ++i) score[i] = logistic(score[i]);
     }
-#pragma unroll
-    for (int i = 0; i < PLACES; ++i) {
-        const int e = lane + 32 * i;
-        key[i] = e < n ? order_of(score[i] + (p.correction != nullptr ? p.correction[e] : 0.f)) : 0u;
+    float sum = 0.f;
+#pragma unroll 1
+    for (int e = lane; e < n; e += 32) {
+        float v = z[e] + (p.router_bias != nullptr ? p.router_bias[e] : 0.f);
+        if (p.scoring != 1) v = expf(p.scoring == 2 ? v - mx : -v);
+        if (p.scoring == 0) v = 1.0f / (1.0f + v);
+        sum += v;
+        z[e] = v;
     }
+    if (p.scoring == 2) sum = warp_sum(sum);
+#pragma unroll 1
+    for (int e = lane; e < n; e += 32) {
+        const float v = p.scoring == 2 ? z[e] / sum : z[e];
+        z[e] = v;
+        key[e] = order_of(v + (p.correction != nullptr ? p.correction[e] : 0.f));
+    }
+    __syncwarp();
     if (p.n_groups > 1) {
         // a group's rank is its best choice score; a group is kept when fewer than keep_groups rank before it (ties: the lower one first)
         const int per = n / p.n_groups;
-        unsigned* best = scratch + n;
-#pragma unroll
-        for (int i = 0; i < PLACES; ++i)
-            if (lane + 32 * i < n) scratch[lane + 32 * i] = key[i];
-        __syncwarp();
+        unsigned* best = key + n;
         for (int g = lane; g < p.n_groups; g += 32) {
             unsigned m = 0u;
-            for (int e = g * per; e < (g + 1) * per; ++e) m = max(m, scratch[e]);
+            for (int e = g * per; e < (g + 1) * per; ++e) m = max(m, key[e]);
             best[g] = m;
         }
         __syncwarp();
-#pragma unroll
-        for (int i = 0; i < PLACES; ++i) {
-            const int e = lane + 32 * i;
-            if (e >= n) continue;
-            const int g = e / per;
+        for (int g = lane; g < p.n_groups; g += 32) {
             int before = 0;
             for (int o = 0; o < p.n_groups; ++o) before += best[o] > best[g] || (best[o] == best[g] && o < g);
-            if (before >= p.keep_groups) key[i] = 0u;
+            if (before >= p.keep_groups)
+                for (int e = g * per; e < (g + 1) * per; ++e) key[e] = 0u;
         }
+        __syncwarp();
     }
     chosen = 0;
     weight = 0.f;
-    unsigned taken = 0u;            // this lane's places that are chosen
+    unsigned taken = 0u;            // this lane's outputs (lane + 32 i: bit i) that are chosen
+#pragma unroll 1
     for (int k = 0; k < p.top; ++k) {
         unsigned best = 0u;
         int at = 0;
-#pragma unroll
-        for (int i = 0; i < PLACES; ++i)
-            if (key[i] > best) {
-                best = key[i];
-                at = i;
+#pragma unroll 4
+        for (int i = 0; i * 32 < n; ++i) {
+            const int e = lane + 32 * i;
+            const unsigned v = e < n ? key[e] : 0u;
+            if (v > best) {
+                best = v;
+                at = e;
             }
-        const unsigned m = __reduce_max_sync(0xffffffffu, best);
-        unsigned e;
-        if (m != 0u) {
-            e = __reduce_min_sync(0xffffffffu, best == m ? (unsigned)(lane + 32 * at) : 0xffffffffu);
-        } else {
-            // nothing is left that compares: the first output that is not chosen yet
-            const int free = __ffs((int)~taken) - 1;
-            e = __reduce_min_sync(0xffffffffu, free < PLACES && lane + 32 * free < n ? (unsigned)(lane + 32 * free) : 0xffffffffu);
         }
-        const int place = (int)(e >> 5);
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < PLACES; ++i)
-            if (i == place) {
-                s = score[i];
-                if (lane == (int)(e & 31u)) {
-                    key[i] = 0u;
-                    taken |= 1u << i;
-                }
-            }
-        s = __shfl_sync(0xffffffffu, s, (int)(e & 31u));
+        const unsigned m = __reduce_max_sync(0xffffffffu, best);
+        // (where nothing is left that compares, the first output that is not chosen yet)
+        const int open = 32 * (__ffs((int)~taken) - 1) + lane;
+        const unsigned e = __reduce_min_sync(0xffffffffu, m != 0u ? best == m ? (unsigned)at : 0xffffffffu : open < n ? (unsigned)open : 0xffffffffu);
+        if (lane == (int)(e & 31u)) {
+            taken |= 1u << (e >> 5);
+            key[e] = 0u;
+        }
         if (lane == k) {
             chosen = (int)e;
-            weight = s;
+            weight = z[e];
         }
     }
     const bool mine = lane < p.top;
     if (p.scoring == 1) {               // the softmax over the chosen logits
-        const float mx = warp_max(mine ? weight : -INFINITY), v = mine ? expf(weight - mx) : 0.f;
+        const float most = warp_max(mine ? weight : -INFINITY), v = mine ? expf(weight - most) : 0.f;
         weight = v / warp_sum(v) * p.route_scale;
     } else {
         weight = p.normalize ? weight / (warp_sum(mine ? weight : 0.f) + 1e-20f) * p.route_scale : weight * p.route_scale;
@@ -378,13 +353,13 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared& sh, 
     }
 }
 
-template <bool CODES>
+template <bool CODES, int GROUPS /* of eight tokens */>
 __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerArgs p) {
     extern __shared__ __align__(16) unsigned char up_smem[];
     UpShared& sh = *reinterpret_cast<UpShared*>(up_smem);
     float* z = reinterpret_cast<float*>(up_smem + sizeof(UpShared));                     // [LT][z_row]: logits, later the weights of what was chosen
     const int z_row = p.n_out + 1;
-    unsigned* scratch = reinterpret_cast<unsigned*>(z + LT * z_row);                     // [L_WARPS][n_out + n_groups], with groups
+    unsigned* keys = reinterpret_cast<unsigned*>(z + LT * z_row);                        // [LT][n_out + n_groups]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     for (int e = threadIdx.x; e < p.n_out; e += L_THREADS) {
@@ -398,9 +373,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
     if (warp < p.n_tokens) {
         int e;
         float w;
-        unsigned* mine = scratch + warp * (p.n_out + p.n_groups);
-        if (p.n_out <= 128) choose<4>(p, z + warp * z_row, mine, lane, e, w);
-        else choose<L_MAX_OUT / 32>(p, z + warp * z_row, mine, lane, e, w);
+        choose(p, z + warp * z_row, keys + warp * (p.n_out + p.n_groups), lane, e, w);
         const bool have = lane < p.top, real = have && e < p.n_real;
         const float identity = warp_sum(have && !real ? w : 0.f);
         if (real) {
@@ -445,68 +418,71 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
     const int n_chunks = (p.width + LK - 1) / LK, rounds = (n_chunks + TEAM - 1) / TEAM;
     const int team = warp / TEAM, member = warp % TEAM, stride = gridDim.x * TEAMS, first = team * gridDim.x + blockIdx.x;
     auto active_of = [&](int item) { return quotient(item - shared_items, p.per_expert_magic); };
-    auto load = [&](Chunk<CODES>& c, int item, int round) {
-        if (item >= n_items) return;
+    constexpr int AHEAD = CODES ? 4 : 2, K_BYTES = LK * (CODES ? 1 : 2);              // 64 registers of chunks that are held or on their way
+    const int turns = (rounds + AHEAD - 1) / AHEAD * AHEAD;                            // (empty chunks fill an item's last turn)
+    // an item's rows from this warp's first chunk on, and their scales: row g of the 16 is a gate row, row g + 8 the row of the linear branch of the same feature
+    const unsigned char *row0 = nullptr, *row1 = nullptr;
+    const float *scale0 = nullptr, *scale1 = nullptr;
+    auto rows_of = [&](int item) {
         const bool own = item >= shared_items;
         const int a = own ? active_of(item) : 0, f = (own ? item - shared_items - a * per_expert : item) * 8 + g, e = own ? sh.plan.of[a].expert : 0;
         const LayerMatrix& m = own ? p.up : p.shared_up;
-        const int il = own ? p.interleave : p.interleave_shared, chunk = member + round * TEAM;
-        // row g of the 16 is a gate row, row g + 8 the row of the linear branch of the same feature
+        const int il = own ? p.interleave : p.interleave_shared;
         const int r0 = il == 0 ? f : il == 4 ? 2 * f - (f & 3) : f / il * 2 * il + f % il, r1 = r0 + (il > 0 ? il : own ? p.inner : p.inner_shared);
-        const unsigned char* base = m.w + e * m.stack_bytes;
-        load_chunk<CODES>(c, base + r0 * m.row_bytes, base + r1 * m.row_bytes, chunk * LK, p.width, lane);
+        const unsigned char* base = m.w + e * m.stack_bytes + (long long)member * K_BYTES;
+        row0 = base + r0 * m.row_bytes;
+        row1 = base + r1 * m.row_bytes;
         if (CODES) {
-            const float* scales = m.scales + (long long)e * m.row_blocks * m.k_blocks + min(chunk, n_chunks - 1);
-            c.scale[0] = scales[(long long)(r0 / LK) * m.k_blocks];
-            c.scale[1] = scales[(long long)(r1 / LK) * m.k_blocks];
+            const float* scales = m.scales + (long long)e * m.row_blocks * m.k_blocks + member;
+            scale0 = scales + (long long)(r0 / LK) * m.k_blocks;
+            scale1 = scales + (long long)(r1 / LK) * m.k_blocks;
         }
     };
-    constexpr int AHEAD = Chunk<CODES>::AHEAD;
+    auto load = [&](Chunk<CODES>& c, int round) {
+        const int chunk = member + round * TEAM;
+        if (chunk >= n_chunks) return;
+        load_chunk<CODES>(c, row0 + round * (TEAM * K_BYTES), row1 + round * (TEAM * K_BYTES), p.width - chunk * LK, lane);
+        if (CODES) c.scale[0] = scale0[round * TEAM], c.scale[1] = scale1[round * TEAM];
+    };
     Chunk<CODES> held[AHEAD];
-    int to_load = first, load_round = 0;
-    auto load_next = [&](Chunk<CODES>& c) {
-        load(c, to_load, load_round);
-        if (++load_round == rounds) {
-            load_round = 0;
-            to_load += stride;
-        }
-    };
+    if (first < n_items) {
+        rows_of(first);
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) load_next(held[i]);
-    float acc[2][4];
-    const bf16 *row0 = nullptr, *row1 = nullptr;
-    int n_cols = 0, set = 0;
-    for (int item = first, round = 0; item < n_items;) {
-#pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-            if (item >= n_items) break;
+        for (int i = 0; i < AHEAD; ++i) load(held[i], i);
+    }
+    int set = 0;
+#pragma unroll 1
+    for (int item = first; item < n_items; item += stride) {
+        {
             const bool own = item >= shared_items;
             const int a = own ? active_of(item) : 0;
-            if (round == 0) {
-                // this lane's columns: the tokens that chose the expert, or all for the shared one
-                const unsigned long long list = own ? sh.plan.of[a].list : 0xfedcba9876543210ull;
-                n_cols = own ? __popc(sh.plan.of[a].tokens) : p.n_tokens;
-                row0 = g < n_cols ? p.x + (long long)((list >> (4 * g)) & 15) * p.ldx : nullptr;
-                row1 = 8 + g < n_cols ? p.x + (long long)((list >> (32 + 4 * g)) & 15) * p.ldx : nullptr;
+            // this lane's columns: the tokens that chose the expert, or all for the shared one
+            const unsigned long long list = own ? sh.plan.of[a].list : 0xfedcba9876543210ull;
+            const int n_cols = own ? __popc(sh.plan.of[a].tokens) : p.n_tokens;
+            const int at = (lane & 3) * (CODES ? 16 : 8) + member * LK;
+            const bf16 *x0 = p.x + (long long)((list >> (4 * g)) & 15) * p.ldx + at, *x1 = p.x + (long long)((list >> (32 + 4 * g)) & 15) * p.ldx + at;
+            float acc[2][4] = {};
+#pragma unroll 1
+            for (int round = 0; round < turns; round += AHEAD) {
+                const bool last = round + AHEAD >= turns, more = !last || item + stride < n_items;
+                if (last && more) rows_of(item + stride);
 #pragma unroll
-                for (int n = 0; n < 2; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
-            }
-            const int chunk = member + round * TEAM, k0 = chunk * LK;
-            if (chunk < n_chunks) {
-                const bf16* at[1] = {row0 != nullptr ? row0 + k0 : nullptr};
-                multiply<CODES, 1>(held[i], at, p.width - k0, lane, acc[0]);
-                if (n_cols > 8) {
-                    const bf16* at1[1] = {row1 != nullptr ? row1 + k0 : nullptr};
-                    multiply<CODES, 1>(held[i], at1, p.width - k0, lane, acc[1]);
+                for (int i = 0; i < AHEAD; ++i) {
+                    const int chunk = member + (round + i) * TEAM;
+                    if (chunk < n_chunks) {
+                        const int k = (round + i) * TEAM * LK, left = p.width - at - k;
+                        Column<CODES> x[1];
+                        load_column<CODES>(x[0], x0 + k, left, g < n_cols);
+                        multiply<CODES, 1>(held[i], x, acc[0]);
+                        if (GROUPS > 1 && n_cols > 8) {
+                            load_column<CODES>(x[0], x1 + k, left, 8 + g < n_cols);
+                            multiply<CODES, 1>(held[i], x, acc[1]);
+                        }
+                    }
+                    if (more) load(held[i], last ? i : round + AHEAD + i);
                 }
             }
-            load_next(held[i]);
-            if (++round < rounds) continue;
             const int f0 = (own ? item - shared_items - a * per_expert : item) * 8;
-            round = 0;
-            item += stride;
             float(*mine)[LT + 1] = sh.reduce[set][warp];
             const int col = (lane & 3) * 2;
 #pragma unroll
@@ -562,7 +538,7 @@ struct DownShared {
 };
 
 // CTA r of a cluster of `parts` takes its share of the chunks of 16 output features; a cluster takes features 16 (blockIdx / parts), ...
-template <bool CODES>
+template <bool CODES, int GROUPS>
 __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const LayerArgs p, int parts) {
     extern __shared__ __align__(16) unsigned char down_smem[];
     DownShared& sh = *reinterpret_cast<DownShared*>(down_smem);
@@ -577,54 +553,64 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK, n_chunks = shared_chunks + sh.plan.n_active * own_chunks;
     auto active_of = [&](int chunk) { return quotient(chunk - shared_chunks, p.own_chunks_magic); };
     const int step = parts * L_WARPS, first = rank * L_WARPS + warp;
-    auto load = [&](Chunk<CODES>& c, int group, int chunk) {
-        const bool own = chunk >= shared_chunks;
-        const int a = own ? active_of(chunk) : 0, kb = own ? (chunk - shared_chunks) - a * own_chunks : chunk;
-        const bool some = chunk < n_chunks;
-        const int e = own && some ? sh.plan.of[a].expert : 0;
-        const LayerMatrix& m = own ? p.down : p.shared_down;
-        const int r0 = min(group * 16 + g, p.width - 1), r1 = min(group * 16 + g + 8, p.width - 1);
-        const unsigned char* base = m.w + e * m.stack_bytes;
-        load_chunk<CODES>(c, base + r0 * m.row_bytes, base + r1 * m.row_bytes, kb * LK, some ? own ? p.inner : p.inner_shared : 0, lane);
-        if (CODES && some) {
-            const float* s = m.scales + (long long)e * m.row_blocks * m.k_blocks;
-            c.scale[0] = s[(long long)(r0 / LK) * m.k_blocks + kb];
-            c.scale[1] = s[(long long)(r1 / LK) * m.k_blocks + kb];
-        }
-    };
-    float acc[2][4];
-    auto work = [&](const Chunk<CODES>& c, int chunk) {
-        if (chunk >= n_chunks) return;
-        const bool own = chunk >= shared_chunks;
-        const int a = own ? active_of(chunk) : 0, kb = own ? (chunk - shared_chunks) - a * own_chunks : chunk;
-        const unsigned tokens = own ? sh.plan.of[a].tokens : (1u << p.n_tokens) - 1u;
-        const unsigned long long choice = own ? sh.plan.of[a].choice : 0ull;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            if ((tokens >> (8 * n) & 0xffu) == 0u) continue;                // (none of these eight columns)
-            const int t = n * 8 + g, row = own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
-            const long long at = (long long)row * p.h_row + kb * LK;
-            const bool have = tokens >> t & 1u;
-            const bf16* rows[2] = {have ? p.h_hi + at : nullptr, have ? p.h_lo + at : nullptr};
-            multiply<CODES, 2>(c, rows, (own ? p.inner : p.inner_shared) - kb * LK, lane, acc[n]);
-        }
-    };
-    constexpr int AHEAD = Chunk<CODES>::AHEAD;
+    constexpr int AHEAD = CODES ? 4 : 2, PER = CODES ? 16 : 8;              // 64 registers of chunks that are held or on their way
     const int rounds = max(1, (n_chunks + step - 1) / step), turns = (rounds + AHEAD - 1) / AHEAD * AHEAD;       // (empty chunks fill the last turn)
+    struct Place {              // a chunk: which active expert's (or the shared one's), and where in its k
+        bool own;
+        int a, kb;
+    };
+    auto place_of = [&](int chunk) {
+        Place at;
+        at.own = chunk >= shared_chunks;
+        at.a = at.own ? quotient(chunk - shared_chunks, p.own_chunks_magic) : 0;
+        at.kb = at.own ? (chunk - shared_chunks) - at.a * own_chunks : chunk;
+        return at;
+    };
+    auto load = [&](Chunk<CODES>& c, int group, int chunk) {
+        if (chunk >= n_chunks) return;
+        const Place at = place_of(chunk);
+        const LayerMatrix& m = at.own ? p.down : p.shared_down;
+        const int e = at.own ? sh.plan.of[at.a].expert : 0, r0 = min(group * 16 + g, p.width - 1), r1 = min(group * 16 + g + 8, p.width - 1);
+        const unsigned char* base = m.w + e * m.stack_bytes + (long long)at.kb * LK * (CODES ? 1 : 2);
+        load_chunk<CODES>(c, base + r0 * m.row_bytes, base + r1 * m.row_bytes, (at.own ? p.inner : p.inner_shared) - at.kb * LK, lane);
+        if (CODES) {
+            const float* s = m.scales + (long long)e * m.row_blocks * m.k_blocks + at.kb;
+            c.scale[0] = s[(long long)(r0 / LK) * m.k_blocks];
+            c.scale[1] = s[(long long)(r1 / LK) * m.k_blocks];
+        }
+    };
     Chunk<CODES> held[AHEAD];
 #pragma unroll
-    for (int i = 0; i < AHEAD; ++i) load(held[i], blockIdx.x / parts, first + i * step);
+    for (int i = 0; i < AHEAD; ++i)
+        if (blockIdx.x / parts < n_groups) load(held[i], blockIdx.x / parts, first + i * step);
+#pragma unroll 1
     for (int group = blockIdx.x / parts; group < n_groups; group += clusters) {
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
+        float acc[2][4] = {};
+#pragma unroll 1
         for (int round = 0; round < turns; round += AHEAD) {
+            const bool last = round + AHEAD >= turns, more = !last || group + clusters < n_groups;
+            const int next_group = last ? group + clusters : group, next_round = last ? 0 : round + AHEAD;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
-                work(held[i], first + (round + i) * step);
-                if (round + AHEAD < turns) load(held[i], group, first + (round + i + AHEAD) * step);
-                else if (group + clusters < n_groups) load(held[i], group + clusters, first + i * step);
+                const int chunk = first + (round + i) * step;
+                if (chunk < n_chunks) {
+                    // the columns: h's rows (both halves) of the tokens that chose the chunk's expert, from the second-level cache
+                    const Place at = place_of(chunk);
+                    const int left = (at.own ? p.inner : p.inner_shared) - at.kb * LK - (lane & 3) * PER;
+                    const unsigned seen = at.own ? sh.plan.of[at.a].tokens : (1u << p.n_tokens) - 1u;
+                    const unsigned long long choice = at.own ? sh.plan.of[at.a].choice : 0ull;
+#pragma unroll
+                    for (int n = 0; n < GROUPS; ++n) {
+                        if ((seen >> (8 * n) & 0xffu) == 0u) continue;
+                        const int t = n * 8 + g, row = at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+                        const long long from = (long long)row * p.h_row + at.kb * LK + (lane & 3) * PER;
+                        Column<CODES> b[2];
+                        load_column<CODES>(b[0], p.h_hi + from, left, seen >> t & 1u);
+                        load_column<CODES>(b[1], p.h_lo + from, left, seen >> t & 1u);
+                        multiply<CODES, 2>(held[i], b, acc[n]);
+                    }
+                }
+                if (more) load(held[i], next_group, first + (next_round + i) * step);
             }
         }
         const int col = (lane & 3) * 2;
@@ -660,12 +646,10 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     }
 }
 
-size_t up_smem_bytes(const LayerArgs& p) {
-    return sizeof(UpShared) + (size_t)LT * (p.n_out + 1) * 4 + (p.n_groups > 1 ? (size_t)L_WARPS * (p.n_out + p.n_groups) * 4 : 0);
-}
+size_t up_smem_bytes(const LayerArgs& p) { return sizeof(UpShared) + (size_t)LT * (p.n_out + 1) * 4 + (size_t)LT * (p.n_out + p.n_groups) * 4; }
 
 // Clusters of the up kernel that the device holds at once (asked for once a device): a grid that needs a second round would route twice.
-template <bool CODES> int up_clusters(size_t smem) {
+template <bool CODES, int GROUPS> int up_clusters(size_t smem) {
     static std::atomic<int> known[64];
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 1;
@@ -681,25 +665,25 @@ template <bool CODES> int up_clusters(size_t smem) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, moe_layer_up_kernel<CODES>, &cfg) != cudaSuccess || n < 1) n = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, moe_layer_up_kernel<CODES, GROUPS>, &cfg) != cudaSuccess || n < 1) n = 1;
     if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
-template <bool CODES> int launch_layer(const LayerArgs& p, int sms, cudaStream_t stream) {
+template <bool CODES, int GROUPS> int launch_layer(const LayerArgs& p, int sms, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed_up{0}, allowed_down{0};
-    cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES>, 200 * 1024, allowed_up);
-    if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES>, (int)sizeof(DownShared), allowed_down);
+    cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES, GROUPS>, 200 * 1024, allowed_up);
+    if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES, GROUPS>, (int)sizeof(DownShared), allowed_down);
     if (e != cudaSuccess) return (int)e;
-    const int clusters = up_clusters<CODES>(up_smem_bytes(p));
-    rlis_launch_cluster(moe_layer_up_kernel<CODES>, dim3((unsigned)(clusters * L_CLUSTER)), dim3(L_THREADS), up_smem_bytes(p), stream, dim3(L_CLUSTER, 1, 1), p);
+    const int clusters = up_clusters<CODES, GROUPS>(up_smem_bytes(p));
+    rlis_launch_cluster(moe_layer_up_kernel<CODES, GROUPS>, dim3((unsigned)(clusters * L_CLUSTER)), dim3(L_THREADS), up_smem_bytes(p), stream, dim3(L_CLUSTER, 1, 1), p);
     const int rc = RLIS_LAUNCH_CHECK();
     if (rc != 0) return rc;
     const int groups = (p.width + 15) / 16;
     int parts = 1;
     while (parts < 4 && groups * parts * 4 < 3 * sms) parts *= 2;
     const int at_once = sms / parts < groups ? sms / parts : groups;
-    rlis_launch_cluster(moe_layer_down_kernel<CODES>, dim3((unsigned)(at_once * parts)), dim3(L_THREADS), sizeof(DownShared), stream, dim3((unsigned)parts, 1, 1), p, parts);
+    rlis_launch_cluster(moe_layer_down_kernel<CODES, GROUPS>, dim3((unsigned)(at_once * parts)), dim3(L_THREADS), sizeof(DownShared), stream, dim3((unsigned)parts, 1, 1), p, parts);
     return RLIS_LAUNCH_CHECK();
 }
 }  // namespace
@@ -788,5 +772,6 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (up_smem_bytes(p) > 200 * 1024) return RLIS_ERR_UNSUPPORTED;
-    return codes ? launch_layer<true>(p, sms, stream) : launch_layer<false>(p, sms, stream);
+    if (p.n_tokens <= 8) return codes ? launch_layer<true, 1>(p, sms, stream) : launch_layer<false, 1>(p, sms, stream);
+    return codes ? launch_layer<true, 2>(p, sms, stream) : launch_layer<false, 2>(p, sms, stream);
 }
