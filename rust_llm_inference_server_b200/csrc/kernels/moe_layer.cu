@@ -67,7 +67,7 @@ struct LayerArgs {
     LayerMatrix up, down, shared_up, shared_down;
     float slope, limit, shift;
     LayerPlan* plan;
-    bf16 *h_hi, *h_lo;                  // [tokens * top + tokens, h_row]
+    bf16 *h_hi, *h_lo;                  // [tokens * top + tokens + 1, h_row]: the pairs', the shared expert's, a row of zeros
     int h_row;
     unsigned per_expert_magic, own_chunks_magic;        // see quotient()
     bf16* out;
@@ -88,28 +88,42 @@ template <bool CODES> struct Chunk {
     uint4 a[STEPS][2];
     float scale[2];             // codes: of row g, of row g + 8
 };
-// `row0`, `row1`: this lane's rows from the chunk's first k on, of which `left` are there.
+// `row0`, `row1`: this lane's rows from the chunk's first k on, of which `left` are there.  (A whole chunk without a test for each load: zeros that may be wanted are
+// instructions, too.)
 template <bool CODES>
 __device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char* row0, const unsigned char* row1, int left, int lane) {
+    row0 += (lane & 3) * 16;
+    row1 += (lane & 3) * 16;
+    if (left >= LK) {
 #pragma unroll
-    for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
-        const int at = (s * 4 + (lane & 3)) * 16;
-        const bool in = (CODES ? at : at / 2) < left;
-        c.a[s][0] = in ? stream16(row0 + at) : make_uint4(0, 0, 0, 0);
-        c.a[s][1] = in ? stream16(row1 + at) : make_uint4(0, 0, 0, 0);
+        for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
+            c.a[s][0] = stream16(row0 + s * 64);
+            c.a[s][1] = stream16(row1 + s * 64);
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
+            const bool in = (s * 4 + (lane & 3)) * (CODES ? 16 : 8) < left;
+            c.a[s][0] = in ? stream16(row0 + s * 64) : make_uint4(0, 0, 0, 0);
+            c.a[s][1] = in ? stream16(row1 + s * 64) : make_uint4(0, 0, 0, 0);
+        }
     }
 }
 
-// Four codes as bfloat16, in their order.  An e4m3's bits moved to a bfloat16's places are its value times 2^-120, subnormal ones included.
+// Four codes as bfloat16, in their order.  An e4m3's bits moved to a bfloat16's places are its value times 2^-120, subnormal ones included: a byte with its sign spread
+// over the byte above it, four places up, has the sign on top and the other seven bits where they belong.
 __device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& first, uint32_t& last) {
     const __nv_bfloat162 up = __float2bfloat162_rn(E4M3_TO_BF16);
     auto place = [&](uint32_t v) {
-        const uint32_t bits = ((v >> 4) & 0x07f007f0u) | (v & 0x80008000u);
+        const uint32_t bits = (v << 4) & 0x87f087f0u;
         const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), up);
         return *reinterpret_cast<const uint32_t*>(&r);
     };
-    first = place(__byte_perm(w, 0u, 0x1404));          // bytes 0 and 1 into the high bytes of the halves
-    last = place(__byte_perm(w, 0u, 0x3424));
+    uint32_t a, b;
+    asm("prmt.b32 %0, %1, 0, 0x9180;" : "=r"(a) : "r"(w));
+    asm("prmt.b32 %0, %1, 0, 0xb3a2;" : "=r"(b) : "r"(w));
+    first = place(a);
+    last = place(b);
 }
 
 // This lane's part of a column's row over a chunk: the vectors of bfloat16 that its A vectors meet.
@@ -117,16 +131,23 @@ template <bool CODES> struct Column {
     static constexpr int VECS = CODES ? 2 : 1;
     uint4 b[Chunk<CODES>::STEPS][VECS];
 };
-// `row`: the column's row from this lane's first k of the chunk on, of which `left` are there; not `have`: a column of zeros.
-template <bool CODES> __device__ __forceinline__ void load_column(Column<CODES>& c, const bf16* row, int left, bool have) {
+// `row`: the column's row from this lane's first k of the chunk on, of which `left` are there (what lies behind them meets zeros of A and is not read).
+template <bool CODES> __device__ __forceinline__ void load_column(Column<CODES>& c, const bf16* row, int left) {
     constexpr int PER = CODES ? 16 : 8;
+    if (left >= LK) {
 #pragma unroll
-    for (int s = 0; s < Chunk<CODES>::STEPS; ++s)
+        for (int s = 0; s < Chunk<CODES>::STEPS; ++s)
 #pragma unroll
-        for (int v = 0; v < Column<CODES>::VECS; ++v) {
-            const int k = s * 4 * PER + v * 8;
-            c.b[s][v] = have && k < left ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
-        }
+            for (int v = 0; v < Column<CODES>::VECS; ++v) c.b[s][v] = *reinterpret_cast<const uint4*>(row + s * 4 * PER + v * 8);
+    } else {
+#pragma unroll
+        for (int s = 0; s < Chunk<CODES>::STEPS; ++s)
+#pragma unroll
+            for (int v = 0; v < Column<CODES>::VECS; ++v) {
+                const int k = s * 4 * PER + v * 8;
+                c.b[s][v] = k < left ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
+            }
+    }
 }
 // acc += chunk * the sum of the columns (COLS of each of eight tokens).  Neighbouring instructions add to different sums: one waits some 35 cycles for the one before
 // it on the same.
@@ -411,6 +432,10 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
         const int words = (int)(offsetof(LayerPlan, of) + (size_t)n_active * sizeof(ActiveExpert)) / 8;
         for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(p.plan)[i] = reinterpret_cast<const unsigned long long*>(&sh.plan)[i];
     }
+    if (blockIdx.x == 1) {              // (a cluster has more than one)
+        const long long at = (long long)p.n_tokens * (p.top + 1) * p.h_row;
+        for (int i = threadIdx.x; i < p.h_row; i += L_THREADS) p.h_hi[at + i] = p.h_lo[at + i] = __float2bfloat16_rn(0.f);
+    }
     pdl_trigger();
 
     // items: eight features of the shared expert, then of every active one; a team's warp takes every TEAM-th chunk of their k, a round each
@@ -456,7 +481,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
         {
             const bool own = item >= shared_items;
             const int a = own ? active_of(item) : 0;
-            // this lane's columns: the tokens that chose the expert, or all for the shared one
+            // this lane's columns: the tokens that chose the expert, or all for the shared one (behind them the first token again, whose sums nobody reads)
             const unsigned long long list = own ? sh.plan.of[a].list : 0xfedcba9876543210ull;
             const int n_cols = own ? __popc(sh.plan.of[a].tokens) : p.n_tokens;
             const int at = (lane & 3) * (CODES ? 16 : 8) + member * LK;
@@ -470,12 +495,12 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                 for (int i = 0; i < AHEAD; ++i) {
                     const int chunk = member + (round + i) * TEAM;
                     if (chunk < n_chunks) {
-                        const int k = (round + i) * TEAM * LK, left = p.width - at - k;
+                        const int k = (round + i) * TEAM * LK, left = p.width - chunk * LK >= LK ? LK : p.width - at - k;
                         Column<CODES> x[1];
-                        load_column<CODES>(x[0], x0 + k, left, g < n_cols);
+                        load_column<CODES>(x[0], x0 + k, left);
                         multiply<CODES, 1>(held[i], x, acc[0]);
                         if (GROUPS > 1 && n_cols > 8) {
-                            load_column<CODES>(x[0], x1 + k, left, 8 + g < n_cols);
+                            load_column<CODES>(x[0], x1 + k, left);
                             multiply<CODES, 1>(held[i], x, acc[1]);
                         }
                     }
@@ -596,17 +621,18 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
                 if (chunk < n_chunks) {
                     // the columns: h's rows (both halves) of the tokens that chose the chunk's expert, from the second-level cache
                     const Place at = place_of(chunk);
-                    const int left = (at.own ? p.inner : p.inner_shared) - at.kb * LK - (lane & 3) * PER;
+                    const int whole = (at.own ? p.inner : p.inner_shared) - at.kb * LK, left = whole >= LK ? LK : whole - (lane & 3) * PER;
                     const unsigned seen = at.own ? sh.plan.of[at.a].tokens : (1u << p.n_tokens) - 1u;
                     const unsigned long long choice = at.own ? sh.plan.of[at.a].choice : 0ull;
 #pragma unroll
                     for (int n = 0; n < GROUPS; ++n) {
                         if ((seen >> (8 * n) & 0xffu) == 0u) continue;
-                        const int t = n * 8 + g, row = at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+                        // (the others' columns: the row of zeros behind h's)
+                        const int t = n * 8 + g, row = !(seen >> t & 1u) ? p.n_tokens * (p.top + 1) : at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
                         const long long from = (long long)row * p.h_row + at.kb * LK + (lane & 3) * PER;
                         Column<CODES> b[2];
-                        load_column<CODES>(b[0], p.h_hi + from, left, seen >> t & 1u);
-                        load_column<CODES>(b[1], p.h_lo + from, left, seen >> t & 1u);
+                        load_column<CODES>(b[0], p.h_hi + from, left);
+                        load_column<CODES>(b[1], p.h_lo + from, left);
                         multiply<CODES, 2>(held[i], b, acc[n]);
                     }
                 }
@@ -707,7 +733,7 @@ struct RlisMoeLayer {
 // Bytes of workspace of a call.
 extern "C" int rlis_moe_layer_bytes(int n_tokens, int top, int inner, int inner_shared) {
     const long long row = ((inner > inner_shared ? inner : inner_shared) + 7) / 8 * 8;
-    return (int)((sizeof(LayerPlan) + 15) / 16 * 16 + 4 * (long long)(n_tokens * top + n_tokens) * row);
+    return (int)((sizeof(LayerPlan) + 15) / 16 * 16 + 4 * (long long)(n_tokens * top + n_tokens + 1) * row);
 }
 
 extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
@@ -764,7 +790,7 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     p.plan = static_cast<LayerPlan*>(a->workspace);
     p.h_row = ((a->inner > a->inner_shared ? a->inner : a->inner_shared) + 7) / 8 * 8;
     p.h_hi = reinterpret_cast<bf16*>(static_cast<unsigned char*>(a->workspace) + (sizeof(LayerPlan) + 15) / 16 * 16);
-    p.h_lo = p.h_hi + (long long)(a->n_tokens * a->top + a->n_tokens) * p.h_row;
+    p.h_lo = p.h_hi + (long long)(a->n_tokens * a->top + a->n_tokens + 1) * p.h_row;
     p.out = static_cast<bf16*>(a->out);
     auto magic = [](int d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; };
     p.per_expert_magic = magic(a->inner / 8);
