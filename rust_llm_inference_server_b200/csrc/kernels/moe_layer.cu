@@ -281,9 +281,10 @@ __device__ __forceinline__ void st_cluster_f32(float* local, float v, uint32_t r
 // ---- up --------------------------------------------------------------------------------------------------------------------------------
 
 constexpr int TEAM = 4, TEAMS = L_WARPS / TEAM;             // warps that share an item's k
+static_assert(TEAM * TEAMS <= 16, "a barrier for each team and set");
 
-struct UpShared {
-    float reduce[2][L_WARPS][16][LT + 1];       // the warps' sums of 16 rows (two sets in turn); before that the router's
+template <int GROUPS> struct UpShared {
+    float reduce[TEAM][L_WARPS][16][8 * GROUPS + 1];        // the warps' sums of 16 rows (sets in turn); before that the router's
     LayerPlan plan;
     float gate[LT];
     unsigned long long choice[L_MAX_OUT];       // which of a token's choices an expert is, four bits a token
@@ -292,35 +293,34 @@ struct UpShared {
 
 // This CTA's rows of the router against all tokens, into every CTA's z [LT][z_row].  Sixteen rows at a time; the warps share k: a warp takes 128 k of the
 // sixteen rows as three bfloat16 each.
-__device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared& sh, float* z, int z_row, int rank, int cluster) {
+template <int GROUPS>
+__device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUPS>& sh, float* z, int z_row, int rank, int cluster) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int rows = p.n_out + p.shared_gate, per = (rows + cluster - 1) / cluster, first = rank * per, mine = max(0, min(per, rows - first));
     const int tiles = (per + 15) / 16, n_chunks = (p.width + LK - 1) / LK;
-    const bool second = p.n_tokens > 8;
     bool met = false;
     for (int tile = 0; tile < tiles; ++tile) {
-        float acc[2][4] = {};
+        float acc[GROUPS][4] = {};
         const int r0 = tile * 16 + g, r1 = r0 + 8;
         const float *w0 = p.router + (long long)(first + min(r0, mine - 1)) * p.width, *w1 = p.router + (long long)(first + min(r1, mine - 1)) * p.width;
         for (int chunk = warp; chunk < n_chunks && tile * 16 < mine; chunk += L_WARPS) {
             const int k0 = chunk * LK + (lane & 3) * 8;
             float4 a[4][2][2];
+            uint4 x[4][GROUPS];
 #pragma unroll
-            for (int s = 0; s < 4; ++s)
+            for (int s = 0; s < 4; ++s) {
+                const int k = k0 + s * 32;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int k = k0 + s * 32;
                     a[s][0][h] = k < p.width ? *reinterpret_cast<const float4*>(w0 + k + 4 * h) : make_float4(0, 0, 0, 0);
                     a[s][1][h] = k < p.width ? *reinterpret_cast<const float4*>(w1 + k + 4 * h) : make_float4(0, 0, 0, 0);
                 }
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                uint4 x[2];
+                for (int n = 0; n < GROUPS; ++n)
+                    x[s][n] = k < p.width && n * 8 + g < p.n_tokens ? *reinterpret_cast<const uint4*>(p.x + (n * 8 + g) * p.ldx + k) : make_uint4(0, 0, 0, 0);
+            }
 #pragma unroll
-                for (int n = 0; n < 2; ++n) {
-                    const int k = k0 + s * 32, t = n * 8 + g;
-                    x[n] = k < p.width && t < p.n_tokens ? *reinterpret_cast<const uint4*>(p.x + t * p.ldx + k) : make_uint4(0, 0, 0, 0);
-                }
+            for (int s = 0; s < 4; ++s) {
                 float v[2][8];
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
@@ -340,18 +340,17 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared& sh, 
                         }
                     const uint32_t a0[4] = {w[0][0], w[1][0], w[0][1], w[1][1]}, a1[4] = {w[0][2], w[1][2], w[0][3], w[1][3]};
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        if (n == 1 && !second) break;
-                        mma_bf16_16816(acc[n], a0, x[n].x, x[n].y);
-                        mma_bf16_16816(acc[n], a1, x[n].z, x[n].w);
+                    for (int n = 0; n < GROUPS; ++n) {
+                        mma_bf16_16816(acc[n], a0, x[s][n].x, x[s][n].y);
+                        mma_bf16_16816(acc[n], a1, x[s][n].z, x[s][n].w);
                     }
                 }
             }
         }
-        float(*sums)[LT + 1] = sh.reduce[tile & 1][warp];
+        auto& sums = sh.reduce[tile & 1][warp];
         const int col = (lane & 3) * 2;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < GROUPS; ++n) {
             sums[g][n * 8 + col] = acc[n][0];
             sums[g][n * 8 + col + 1] = acc[n][1];
             sums[g + 8][n * 8 + col] = acc[n][2];
@@ -377,8 +376,8 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared& sh, 
 template <bool CODES, int GROUPS /* of eight tokens */>
 __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerArgs p) {
     extern __shared__ __align__(16) unsigned char up_smem[];
-    UpShared& sh = *reinterpret_cast<UpShared*>(up_smem);
-    float* z = reinterpret_cast<float*>(up_smem + sizeof(UpShared));                     // [LT][z_row]: logits, later the weights of what was chosen
+    UpShared<GROUPS>& sh = *reinterpret_cast<UpShared<GROUPS>*>(up_smem);
+    float* z = reinterpret_cast<float*>(up_smem + sizeof(UpShared<GROUPS>));                     // [LT][z_row]: logits, later the weights of what was chosen
     const int z_row = p.n_out + 1;
     unsigned* keys = reinterpret_cast<unsigned*>(z + LT * z_row);                        // [LT][n_out + n_groups]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
@@ -388,7 +387,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
         sh.choice[e] = 0ull;
     }
     pdl_wait();
-    router_logits(p, sh, z, z_row, blockIdx.x % L_CLUSTER, L_CLUSTER);
+    router_logits<GROUPS>(p, sh, z, z_row, blockIdx.x % L_CLUSTER, L_CLUSTER);
     cluster_sync_all();
 
     if (warp < p.n_tokens) {
@@ -486,47 +485,74 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
             const int n_cols = own ? __popc(sh.plan.of[a].tokens) : p.n_tokens;
             const int at = (lane & 3) * (CODES ? 16 : 8) + member * LK;
             const bf16 *x0 = p.x + (long long)((list >> (4 * g)) & 15) * p.ldx + at, *x1 = p.x + (long long)((list >> (32 + 4 * g)) & 15) * p.ldx + at;
-            float acc[2][4] = {};
+            float acc[GROUPS][4] = {};
 #pragma unroll 1
             for (int round = 0; round < turns; round += AHEAD) {
                 const bool last = round + AHEAD >= turns, more = !last || item + stride < n_items;
                 if (last && more) rows_of(item + stride);
 #pragma unroll
-                for (int i = 0; i < AHEAD; ++i) {
-                    const int chunk = member + (round + i) * TEAM;
-                    if (chunk < n_chunks) {
-                        const int k = (round + i) * TEAM * LK, left = p.width - chunk * LK >= LK ? LK : p.width - at - k;
-                        Column<CODES> x[1];
-                        load_column<CODES>(x[0], x0 + k, left);
-                        multiply<CODES, 1>(held[i], x, acc[0]);
+                for (int i = 0; i < AHEAD; i += 2) {
+                    // two chunks at a time, whose loads and sums do not wait for each other
+                    const int chunk = member + (round + i) * TEAM, k = (round + i) * TEAM * LK;
+                    Column<CODES> x[2][1];
+                    if ((chunk + TEAM + 1) * LK <= p.width) {
+                        load_column<CODES>(x[0][0], x0 + k, LK);
+                        load_column<CODES>(x[1][0], x0 + k + TEAM * LK, LK);
+                        multiply<CODES, 1>(held[i], x[0], acc[0]);
+                        multiply<CODES, 1>(held[i + 1], x[1], acc[0]);
                         if (GROUPS > 1 && n_cols > 8) {
-                            load_column<CODES>(x[0], x1 + k, left);
-                            multiply<CODES, 1>(held[i], x, acc[1]);
+                            load_column<CODES>(x[0][0], x1 + k, LK);
+                            load_column<CODES>(x[1][0], x1 + k + TEAM * LK, LK);
+                            multiply<CODES, 1>(held[i], x[0], acc[GROUPS - 1]);
+                            multiply<CODES, 1>(held[i + 1], x[1], acc[GROUPS - 1]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            if (chunk + j * TEAM >= n_chunks) continue;
+                            const int kj = k + j * TEAM * LK, left = p.width - (chunk + j * TEAM) * LK >= LK ? LK : p.width - at - kj;
+                            load_column<CODES>(x[j][0], x0 + kj, left);
+                            multiply<CODES, 1>(held[i + j], x[j], acc[0]);
+                            if (GROUPS > 1 && n_cols > 8) {
+                                load_column<CODES>(x[j][0], x1 + kj, left);
+                                multiply<CODES, 1>(held[i + j], x[j], acc[GROUPS - 1]);
+                            }
                         }
                     }
-                    if (more) load(held[i], last ? i : round + AHEAD + i);
+                    if (more) {
+                        load(held[i], last ? i : round + AHEAD + i);
+                        load(held[i + 1], last ? i + 1 : round + AHEAD + i + 1);
+                    }
                 }
             }
             const int f0 = (own ? item - shared_items - a * per_expert : item) * 8;
-            float(*mine)[LT + 1] = sh.reduce[set][warp];
+            auto& mine = sh.reduce[set][warp];
             const int col = (lane & 3) * 2;
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
+            for (int n = 0; n < GROUPS; ++n) {
                 if (n == 1 && n_cols <= 8) break;
                 mine[g][n * 8 + col] = acc[n][0];
                 mine[g][n * 8 + col + 1] = acc[n][1];
                 mine[g + 8][n * 8 + col] = acc[n][2];
                 mine[g + 8][n * 8 + col + 1] = acc[n][3];
             }
-            // (two sets in turn: nobody writes this one again before the team has come to the next item's barrier)
-            asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * TEAM) : "memory");
-            const int f = lane & 7, c = member * 4 + (lane >> 3);
-            if (c < n_cols) {
+            // The team's warps take the ends of items in turn, and the others go on.  (As many sets as warps: before a warp writes a set again it has ended an item
+            // itself since, for which it waited for all; the warp that read the set had done so by then.)  Barriers 0 .. 15: nothing else uses one from here on.
+            const int barrier = team * TEAM + set, mine_to_end = set == member;
+            set = set + 1 == TEAM ? 0 : set + 1;
+            if (!mine_to_end) {
+                asm volatile("bar.arrive %0, %1;" ::"r"(barrier), "n"(32 * TEAM) : "memory");
+                continue;
+            }
+            asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(32 * TEAM) : "memory");
+            const int f = lane & 7;
+#pragma unroll 1
+            for (int c = lane >> 3; c < n_cols; c += 4) {
                 float gate = 0.f, lin = 0.f;
 #pragma unroll
                 for (int w = 0; w < TEAM; ++w) {
-                    gate += sh.reduce[set][team * TEAM + w][f][c];
-                    lin += sh.reduce[set][team * TEAM + w][f + 8][c];
+                    gate += sh.reduce[member][team * TEAM + w][f][c];
+                    lin += sh.reduce[member][team * TEAM + w][f + 8][c];
                 }
                 if (p.limit != INFINITY) {          // (a NaN stays one)
                     gate = gate > p.limit ? p.limit : gate;
@@ -549,7 +575,6 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                 p.h_hi[at] = hi;
                 p.h_lo[at] = __float2bfloat16_rn(v - __bfloat162float(hi));
             }
-            set ^= 1;
         }
     }
 }
@@ -672,7 +697,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     }
 }
 
-size_t up_smem_bytes(const LayerArgs& p) { return sizeof(UpShared) + (size_t)LT * (p.n_out + 1) * 4 + (size_t)LT * (p.n_out + p.n_groups) * 4; }
+template <int GROUPS> size_t up_smem_bytes(const LayerArgs& p) { return sizeof(UpShared<GROUPS>) + (size_t)LT * (p.n_out + 1) * 4 + (size_t)LT * (p.n_out + p.n_groups) * 4; }
 
 // Clusters of the up kernel that the device holds at once (asked for once a device): a grid that needs a second round would route twice.
 template <bool CODES, int GROUPS> int up_clusters(size_t smem) {
@@ -698,11 +723,12 @@ template <bool CODES, int GROUPS> int up_clusters(size_t smem) {
 
 template <bool CODES, int GROUPS> int launch_layer(const LayerArgs& p, int sms, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed_up{0}, allowed_down{0};
-    cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES, GROUPS>, 200 * 1024, allowed_up);
+    static_assert(sizeof(UpShared<2>) + (size_t)LT * (L_MAX_OUT + 1) * 4 + (size_t)LT * 2 * L_MAX_OUT * 4 <= 227 * 1024, "the most router outputs and groups");
+    cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES, GROUPS>, 227 * 1024, allowed_up);
     if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES, GROUPS>, (int)sizeof(DownShared), allowed_down);
     if (e != cudaSuccess) return (int)e;
-    const int clusters = up_clusters<CODES, GROUPS>(up_smem_bytes(p));
-    rlis_launch_cluster(moe_layer_up_kernel<CODES, GROUPS>, dim3((unsigned)(clusters * L_CLUSTER)), dim3(L_THREADS), up_smem_bytes(p), stream, dim3(L_CLUSTER, 1, 1), p);
+    const int clusters = up_clusters<CODES, GROUPS>(up_smem_bytes<GROUPS>(p));
+    rlis_launch_cluster(moe_layer_up_kernel<CODES, GROUPS>, dim3((unsigned)(clusters * L_CLUSTER)), dim3(L_THREADS), up_smem_bytes<GROUPS>(p), stream, dim3(L_CLUSTER, 1, 1), p);
     const int rc = RLIS_LAUNCH_CHECK();
     if (rc != 0) return rc;
     const int groups = (p.width + 15) / 16;
@@ -797,7 +823,6 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     p.own_chunks_magic = magic((a->inner + LK - 1) / LK);
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    if (up_smem_bytes(p) > 200 * 1024) return RLIS_ERR_UNSUPPORTED;
     if (p.n_tokens <= 8) return codes ? launch_layer<true, 1>(p, sms, stream) : launch_layer<false, 1>(p, sms, stream);
     return codes ? launch_layer<true, 2>(p, sms, stream) : launch_layer<false, 2>(p, sms, stream);
 }
