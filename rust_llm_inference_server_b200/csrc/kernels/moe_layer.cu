@@ -18,11 +18,14 @@
 // router's float32 rows go through the same instructions as three bfloat16 numbers each, whose sum they are to 2^-24 (a token's logits are sums of exact
 // products in float32, as a chain of FMAs would give them; as FMAs, 128 rows against 16 tokens took 20 us).
 //
-// The weights of the choice are multiplied into h in float32, and h is handed on as two bfloat16 numbers (their sum is h to 2^-17), so that nothing but the
-// result is rounded to the activations' type; the down product is then one long sum over the chosen experts' k, with the step's tokens as columns whoever
-// chose them.
+// The weights of the choice are multiplied into h in float32; the down product is then one long sum over the chosen experts' k, with the step's tokens as columns
+// whoever chose them.  Nothing but the result is rounded to the activations' type: beside bfloat16 weights h is two bfloat16 numbers (their sum is h to 2^-17).
+// Codes become float16 by one instruction a pair (as bfloat16, which has none, a word of four took 10 cycles of a scheduler instead of 5, and the products waited
+// for it), so the tokens' rows and h's meet them as float16 of eleven bits, each row times the power of two that brings its largest value to 2^14 .. 2^15: x is
+// that exactly down to 2^-31 of the largest, h to 2^-11 of every value, an eighth of what the result is rounded by.
 #include "common.cuh"
 #include "mma_utils.cuh"
+#include <cuda_fp16.h>
 #include <math.h>
 
 namespace {
@@ -33,7 +36,6 @@ constexpr int L_MAX_OUT = 512;          // router outputs
 constexpr int L_MAX_PAIRS = 256;        // tokens * top
 constexpr int LK = 128;                 // k of a chunk
 constexpr int MOST_K = 16384;           // of a matrix of the layer (items' numbers stay within what a product divides)
-constexpr float E4M3_TO_BF16 = 0x1p120f;
 
 // An expert that some token chose: the tokens as bits, as a list (four bits each), and which of a token's choices it is (four bits a token).
 struct ActiveExpert {
@@ -67,7 +69,11 @@ struct LayerArgs {
     LayerMatrix up, down, shared_up, shared_down;
     float slope, limit, shift;
     LayerPlan* plan;
-    bf16 *h_hi, *h_lo;                  // [tokens * top + tokens + 1, h_row]: the pairs', the shared expert's, a row of zeros
+    bf16 *h_hi, *h_lo;                  // [tokens * top + tokens + 1, h_row]: the pairs', the shared expert's, a row of zeros; or, beside codes, float32:
+    float* h;
+    unsigned char* h_top;               // the largest exponent of every eight of a row, rows top_row apart
+    __half* x_scaled;                   // [cluster of the up kernel][tokens][width]
+    int top_row;
     int h_row;
     unsigned per_expert_magic, own_chunks_magic;        // see quotient()
     bf16* out;
@@ -110,20 +116,29 @@ __device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char*
     }
 }
 
-// Four codes as bfloat16, in their order.  An e4m3's bits moved to a bfloat16's places are its value times 2^-120, subnormal ones included: a byte with its sign spread
-// over the byte above it, four places up, has the sign on top and the other seven bits where they belong.
+// Four codes as float16, in their order.
 __device__ __forceinline__ void widen_codes(uint32_t w, uint32_t& first, uint32_t& last) {
-    const __nv_bfloat162 up = __float2bfloat162_rn(E4M3_TO_BF16);
-    auto place = [&](uint32_t v) {
-        const uint32_t bits = (v << 4) & 0x87f087f0u;
-        const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), up);
-        return *reinterpret_cast<const uint32_t*>(&r);
-    };
-    uint32_t a, b;
-    asm("prmt.b32 %0, %1, 0, 0x9180;" : "=r"(a) : "r"(w));
-    asm("prmt.b32 %0, %1, 0, 0xb3a2;" : "=r"(b) : "r"(w));
-    first = place(a);
-    last = place(b);
+    asm("{\n"
+        ".reg .b16 lo, hi;\n"
+        "mov.b32 {lo, hi}, %2;\n"
+        "cvt.rn.f16x2.e4m3x2 %0, lo;\n"
+        "cvt.rn.f16x2.e4m3x2 %1, hi;\n"
+        "}\n"
+        : "=r"(first), "=r"(last) : "r"(w));
+}
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The powers of two that bring a row whose largest float32 exponent is e (biased) to 2^14 .. 2^15 and back; rows below 2^-112 stay below that.
+constexpr int LEAST_EXPONENT = 15;
+__device__ __forceinline__ float scaling_of(int e) { return __uint_as_float((unsigned)(268 - e) << 23); }
+__device__ __forceinline__ float unscaling_of(int e) { return __uint_as_float((unsigned)(e - 14) << 23); }
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // This lane's part of a column's row over a chunk: the vectors of bfloat16 that its A vectors meet.
@@ -149,10 +164,23 @@ template <bool CODES> __device__ __forceinline__ void load_column(Column<CODES>&
             }
     }
 }
-// acc += chunk * the sum of the columns (COLS of each of eight tokens).  Neighbouring instructions add to different sums: one waits some 35 cycles for the one before
+// The same of a row of float32, scaled.
+__device__ __forceinline__ void load_column(Column<true>& c, const float* row, int left, float scaling) {
+#pragma unroll
+    for (int s = 0; s < Chunk<true>::STEPS; ++s) {
+        float4 f[4];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) f[v] = s * 64 + v * 4 < left ? *reinterpret_cast<const float4*>(row + s * 64 + v * 4) : make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+            c.b[s][v] = make_uint4(pack_half(f[2 * v].x * scaling, f[2 * v].y * scaling), pack_half(f[2 * v].z * scaling, f[2 * v].w * scaling),
+                                   pack_half(f[2 * v + 1].x * scaling, f[2 * v + 1].y * scaling), pack_half(f[2 * v + 1].z * scaling, f[2 * v + 1].w * scaling));
+    }
+}
+// acc += chunk * the sum of the columns (COLS of each of eight tokens), times `back0` and `back1` in the lane's two columns.  Neighbouring instructions add to different sums: one waits some 35 cycles for the one before
 // it on the same.
 template <bool CODES, int COLS>
-__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<CODES> (&cols)[COLS], float (&acc)[4]) {
+__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<CODES> (&cols)[COLS], float (&acc)[4], float back0 = 1.f, float back1 = 1.f) {
     float part[2][4] = {};
 #pragma unroll
     for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
@@ -169,14 +197,16 @@ __device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<COD
 #pragma unroll
             for (int i = 0; i < COLS; ++i) {
                 const uint4 b = cols[i].b[s][CODES ? j / 2 : 0];
-                mma_bf16_16816(part[(j + i) & 1], a, j & 1 ? b.z : b.x, j & 1 ? b.w : b.y);
+                if constexpr (CODES) mma_f16_16816(part[(j + i) & 1], a, j & 1 ? b.z : b.x, j & 1 ? b.w : b.y);
+                else mma_bf16_16816(part[(j + i) & 1], a, j & 1 ? b.z : b.x, j & 1 ? b.w : b.y);
             }
         }
     }
-    acc[0] = fmaf(part[0][0] + part[1][0], CODES ? c.scale[0] : 1.f, acc[0]);
-    acc[1] = fmaf(part[0][1] + part[1][1], CODES ? c.scale[0] : 1.f, acc[1]);
-    acc[2] = fmaf(part[0][2] + part[1][2], CODES ? c.scale[1] : 1.f, acc[2]);
-    acc[3] = fmaf(part[0][3] + part[1][3], CODES ? c.scale[1] : 1.f, acc[3]);
+    const float s0 = CODES ? c.scale[0] : 1.f, s1 = CODES ? c.scale[1] : 1.f;
+    acc[0] = fmaf((part[0][0] + part[1][0]) * back0, s0, acc[0]);
+    acc[1] = fmaf((part[0][1] + part[1][1]) * back1, s0, acc[1]);
+    acc[2] = fmaf((part[0][2] + part[1][2]) * back0, s1, acc[2]);
+    acc[3] = fmaf((part[0][3] + part[1][3]) * back1, s1, acc[3]);
 }
 
 // ---- the choice ------------------------------------------------------------------------------------------------------------------------
@@ -287,6 +317,8 @@ template <int GROUPS> struct UpShared {
     float reduce[TEAM][L_WARPS][16][8 * GROUPS + 1];        // the warps' sums of 16 rows (sets in turn); before that the router's
     LayerPlan plan;
     float gate[LT];
+    int exponent[LT];                           // beside codes: the largest exponent of a token's row
+    unsigned top[L_WARPS];
     unsigned long long choice[L_MAX_OUT];       // which of a token's choices an expert is, four bits a token
     unsigned tokens[L_MAX_OUT];                 // the tokens that chose an expert
 };
@@ -373,6 +405,32 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUP
     }
 }
 
+// The cluster's copy of the tokens' rows as scaled float16 (8 KB of a token's row a CTA, two tokens at the most), and their exponents in every CTA.
+template <int GROUPS>
+__device__ __forceinline__ void scale_rows(const LayerArgs& p, UpShared<GROUPS>& sh, __half* to, int rank, int cluster) {
+    static_assert(L_CLUSTER * 2 >= LT && L_WARPS == 16, "eight warps a token");
+    const int warp = threadIdx.x >> 5, t = rank + cluster * (warp >> 3), i0 = threadIdx.x & 255;
+    const bf16* x = p.x + (long long)min(t, p.n_tokens - 1) * p.ldx;
+    unsigned m = 0u;
+    for (int k = i0 * 8; k < p.width; k += 2048) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + k);
+        m = __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    }
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+    if ((threadIdx.x & 31) == 0) sh.top[warp] = m;
+    __syncthreads();
+    for (int w = 0; w < 8; ++w) m = max(m, sh.top[(warp & 8) + w]);
+    if (t >= p.n_tokens) return;
+    const int e = max((int)(m >> 7), LEAST_EXPONENT);
+    const float scaling = scaling_of(e);
+    for (int k = i0 * 8; k < p.width; k += 2048) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + k);
+        auto two = [&](uint32_t w) { return pack_half(__uint_as_float(w << 16) * scaling, __uint_as_float(w & 0xffff0000u) * scaling); };
+        *reinterpret_cast<uint4*>(to + (long long)t * p.width + k) = make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+    }
+    if (i0 < cluster) st_cluster_f32(reinterpret_cast<float*>(&sh.exponent[t]), __int_as_float(e), (uint32_t)i0);
+}
+
 template <bool CODES, int GROUPS /* of eight tokens */>
 __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerArgs p) {
     extern __shared__ __align__(16) unsigned char up_smem[];
@@ -388,6 +446,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
     }
     pdl_wait();
     router_logits<GROUPS>(p, sh, z, z_row, blockIdx.x % L_CLUSTER, L_CLUSTER);
+    __half* x_scaled = p.x_scaled + (long long)(blockIdx.x / L_CLUSTER) * p.n_tokens * p.width;
+    if (CODES) scale_rows<GROUPS>(p, sh, x_scaled, blockIdx.x % L_CLUSTER, L_CLUSTER);
     cluster_sync_all();
 
     if (warp < p.n_tokens) {
@@ -433,7 +493,10 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
     }
     if (blockIdx.x == 1) {              // (a cluster has more than one)
         const long long at = (long long)p.n_tokens * (p.top + 1) * p.h_row;
-        for (int i = threadIdx.x; i < p.h_row; i += L_THREADS) p.h_hi[at + i] = p.h_lo[at + i] = __float2bfloat16_rn(0.f);
+        for (int i = threadIdx.x; i < p.h_row; i += L_THREADS) {
+            if (CODES) p.h[at + i] = 0.f;
+            else p.h_hi[at + i] = p.h_lo[at + i] = __float2bfloat16_rn(0.f);
+        }
     }
     pdl_trigger();
 
@@ -442,7 +505,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
     const int n_chunks = (p.width + LK - 1) / LK, rounds = (n_chunks + TEAM - 1) / TEAM;
     const int team = warp / TEAM, member = warp % TEAM, stride = gridDim.x * TEAMS, first = team * gridDim.x + blockIdx.x;
     auto active_of = [&](int item) { return quotient(item - shared_items, p.per_expert_magic); };
-    constexpr int AHEAD = CODES ? 4 : 2, K_BYTES = LK * (CODES ? 1 : 2);              // 64 registers of chunks that are held or on their way
+    constexpr int AHEAD = CODES && GROUPS == 1 ? 4 : 2, K_BYTES = LK * (CODES ? 1 : 2);           // chunks that are held or on their way, as registers last
     const int turns = (rounds + AHEAD - 1) / AHEAD * AHEAD;                            // (empty chunks fill an item's last turn)
     // an item's rows from this warp's first chunk on, and their scales: row g of the 16 is a gate row, row g + 8 the row of the linear branch of the same feature
     const unsigned char *row0 = nullptr, *row1 = nullptr;
@@ -484,7 +547,9 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
             const unsigned long long list = own ? sh.plan.of[a].list : 0xfedcba9876543210ull;
             const int n_cols = own ? __popc(sh.plan.of[a].tokens) : p.n_tokens;
             const int at = (lane & 3) * (CODES ? 16 : 8) + member * LK;
-            const bf16 *x0 = p.x + (long long)((list >> (4 * g)) & 15) * p.ldx + at, *x1 = p.x + (long long)((list >> (32 + 4 * g)) & 15) * p.ldx + at;
+            const bf16* x = CODES ? reinterpret_cast<const bf16*>(x_scaled) : p.x;
+            const long long ldx = CODES ? p.width : p.ldx;
+            const bf16 *x0 = x + (long long)((list >> (4 * g)) & 15) * ldx + at, *x1 = x + (long long)((list >> (32 + 4 * g)) & 15) * ldx + at;
             float acc[GROUPS][4] = {};
 #pragma unroll 1
             for (int round = 0; round < turns; round += AHEAD) {
@@ -494,28 +559,28 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                 for (int i = 0; i < AHEAD; i += 2) {
                     // two chunks at a time, whose loads and sums do not wait for each other
                     const int chunk = member + (round + i) * TEAM, k = (round + i) * TEAM * LK;
-                    Column<CODES> x[2][1];
+                    Column<CODES> col_x[2][1];
                     if ((chunk + TEAM + 1) * LK <= p.width) {
-                        load_column<CODES>(x[0][0], x0 + k, LK);
-                        load_column<CODES>(x[1][0], x0 + k + TEAM * LK, LK);
-                        multiply<CODES, 1>(held[i], x[0], acc[0]);
-                        multiply<CODES, 1>(held[i + 1], x[1], acc[0]);
+                        load_column<CODES>(col_x[0][0], x0 + k, LK);
+                        load_column<CODES>(col_x[1][0], x0 + k + TEAM * LK, LK);
+                        multiply<CODES, 1>(held[i], col_x[0], acc[0]);
+                        multiply<CODES, 1>(held[i + 1], col_x[1], acc[0]);
                         if (GROUPS > 1 && n_cols > 8) {
-                            load_column<CODES>(x[0][0], x1 + k, LK);
-                            load_column<CODES>(x[1][0], x1 + k + TEAM * LK, LK);
-                            multiply<CODES, 1>(held[i], x[0], acc[GROUPS - 1]);
-                            multiply<CODES, 1>(held[i + 1], x[1], acc[GROUPS - 1]);
+                            load_column<CODES>(col_x[0][0], x1 + k, LK);
+                            load_column<CODES>(col_x[1][0], x1 + k + TEAM * LK, LK);
+                            multiply<CODES, 1>(held[i], col_x[0], acc[GROUPS - 1]);
+                            multiply<CODES, 1>(held[i + 1], col_x[1], acc[GROUPS - 1]);
                         }
                     } else {
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             if (chunk + j * TEAM >= n_chunks) continue;
                             const int kj = k + j * TEAM * LK, left = p.width - (chunk + j * TEAM) * LK >= LK ? LK : p.width - at - kj;
-                            load_column<CODES>(x[j][0], x0 + kj, left);
-                            multiply<CODES, 1>(held[i + j], x[j], acc[0]);
+                            load_column<CODES>(col_x[j][0], x0 + kj, left);
+                            multiply<CODES, 1>(held[i + j], col_x[j], acc[0]);
                             if (GROUPS > 1 && n_cols > 8) {
-                                load_column<CODES>(x[j][0], x1 + kj, left);
-                                multiply<CODES, 1>(held[i + j], x[j], acc[GROUPS - 1]);
+                                load_column<CODES>(col_x[j][0], x1 + kj, left);
+                                multiply<CODES, 1>(held[i + j], col_x[j], acc[GROUPS - 1]);
                             }
                         }
                     }
@@ -554,10 +619,6 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                     gate += sh.reduce[member][team * TEAM + w][f][c];
                     lin += sh.reduce[member][team * TEAM + w][f + 8][c];
                 }
-                if (p.limit != INFINITY) {          // (a NaN stays one)
-                    gate = gate > p.limit ? p.limit : gate;
-                    lin = lin > p.limit ? p.limit : lin < -p.limit ? -p.limit : lin;
-                }
                 int row, t = c;
                 float w;
                 if (own) {
@@ -569,11 +630,28 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                     row = p.n_tokens * p.top + t;
                     w = sh.gate[t];
                 }
+                if (CODES) {
+                    const float back = unscaling_of(sh.exponent[t]);
+                    gate *= back;
+                    lin *= back;
+                }
+                if (p.limit != INFINITY) {          // (a NaN stays one)
+                    gate = gate > p.limit ? p.limit : gate;
+                    lin = lin > p.limit ? p.limit : lin < -p.limit ? -p.limit : lin;
+                }
                 const float v = glu_gate(gate, p.slope) * (lin + p.shift) * w;
-                const bf16 hi = __float2bfloat16_rn(v);
                 const long long at = (long long)row * p.h_row + f0 + f;
-                p.h_hi[at] = hi;
-                p.h_lo[at] = __float2bfloat16_rn(v - __bfloat162float(hi));
+                if (CODES) {
+                    p.h[at] = v;
+                    unsigned e = __float_as_uint(v) >> 23 & 255u;           // of the eight lanes
+#pragma unroll
+                    for (int o = 4; o > 0; o >>= 1) e = max(e, __shfl_xor_sync(0xffu << (lane & 24), e, o));
+                    if (f == 0) p.h_top[row * p.top_row + f0 / 8] = (unsigned char)e;
+                } else {
+                    const bf16 hi = __float2bfloat16_rn(v);
+                    p.h_hi[at] = hi;
+                    p.h_lo[at] = __float2bfloat16_rn(v - __bfloat162float(hi));
+                }
             }
         }
     }
@@ -584,6 +662,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
 struct DownShared {
     float reduce[L_WARPS][16][LT + 1];
     float cluster[16][LT];
+    int exponent[L_MAX_PAIRS + LT + 1];         // beside codes: of h's rows
     LayerPlan plan;
 };
 
@@ -600,6 +679,24 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(&sh.plan)[i] = reinterpret_cast<const unsigned long long*>(p.plan)[i];
     __syncthreads();
     pdl_trigger();
+    if (CODES) {
+        // eight lanes a row
+        const int n_rows = p.n_tokens * (p.top + 1);
+#pragma unroll 1
+        for (int row = threadIdx.x >> 3; row < (n_rows + 3) / 4 * 4; row += L_THREADS / 8) {
+            const int n = (row < p.n_tokens * p.top ? p.inner : p.inner_shared) / 16;
+            const unsigned short* tops = reinterpret_cast<const unsigned short*>(p.h_top + min(row, n_rows - 1) * p.top_row);
+            unsigned e = 0u;
+#pragma unroll 8
+            for (int i = lane & 7; i < n; i += 8) e = __vmaxu4(e, tops[i]);
+            e = max(e & 255u, e >> 8);
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
+            if ((lane & 7) == 0 && row < n_rows) sh.exponent[row] = max((int)e, LEAST_EXPONENT);
+        }
+        if (threadIdx.x == 0) sh.exponent[n_rows] = LEAST_EXPONENT;
+        __syncthreads();
+    }
     const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK, n_chunks = shared_chunks + sh.plan.n_active * own_chunks;
     auto active_of = [&](int chunk) { return quotient(chunk - shared_chunks, p.own_chunks_magic); };
     const int step = parts * L_WARPS, first = rank * L_WARPS + warp;
@@ -653,12 +750,22 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
                     for (int n = 0; n < GROUPS; ++n) {
                         if ((seen >> (8 * n) & 0xffu) == 0u) continue;
                         // (the others' columns: the row of zeros behind h's)
-                        const int t = n * 8 + g, row = !(seen >> t & 1u) ? p.n_tokens * (p.top + 1) : at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+                        auto row_of = [&](int t) {
+                            return !(seen >> t & 1u) ? p.n_tokens * (p.top + 1) : at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+                        };
+                        const int row = row_of(n * 8 + g);
                         const long long from = (long long)row * p.h_row + at.kb * LK + (lane & 3) * PER;
-                        Column<CODES> b[2];
-                        load_column<CODES>(b[0], p.h_hi + from, left);
-                        load_column<CODES>(b[1], p.h_lo + from, left);
-                        multiply<CODES, 2>(held[i], b, acc[n]);
+                        if constexpr (CODES) {
+                            Column<CODES> b[1];
+                            load_column(b[0], p.h + from, left, scaling_of(sh.exponent[row]));
+                            multiply<CODES, 1>(held[i], b, acc[n], unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2)]),
+                                               unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2 + 1)]));
+                        } else {
+                            Column<CODES> b[2];
+                            load_column<CODES>(b[0], p.h_hi + from, left);
+                            load_column<CODES>(b[1], p.h_lo + from, left);
+                            multiply<CODES, 2>(held[i], b, acc[n]);
+                        }
                     }
                 }
                 if (more) load(held[i], next_group, first + (next_round + i) * step);
@@ -700,7 +807,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
 template <int GROUPS> size_t up_smem_bytes(const LayerArgs& p) { return sizeof(UpShared<GROUPS>) + (size_t)LT * (p.n_out + 1) * 4 + (size_t)LT * (p.n_out + p.n_groups) * 4; }
 
 // Clusters of the up kernel that the device holds at once (asked for once a device): a grid that needs a second round would route twice.
-template <bool CODES, int GROUPS> int up_clusters(size_t smem) {
+template <bool CODES, int GROUPS> int up_clusters(size_t smem, int sms) {
     static std::atomic<int> known[64];
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 1;
@@ -717,6 +824,7 @@ template <bool CODES, int GROUPS> int up_clusters(size_t smem) {
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     if (cudaOccupancyMaxActiveClusters(&n, moe_layer_up_kernel<CODES, GROUPS>, &cfg) != cudaSuccess || n < 1) n = 1;
+    if (n > sms / L_CLUSTER) n = sms / L_CLUSTER > 0 ? sms / L_CLUSTER : 1;           // (what the workspace has room for)
     if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
@@ -727,7 +835,7 @@ template <bool CODES, int GROUPS> int launch_layer(const LayerArgs& p, int sms, 
     cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES, GROUPS>, 227 * 1024, allowed_up);
     if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES, GROUPS>, (int)sizeof(DownShared), allowed_down);
     if (e != cudaSuccess) return (int)e;
-    const int clusters = up_clusters<CODES, GROUPS>(up_smem_bytes<GROUPS>(p));
+    const int clusters = up_clusters<CODES, GROUPS>(up_smem_bytes<GROUPS>(p), sms);
     rlis_launch_cluster(moe_layer_up_kernel<CODES, GROUPS>, dim3((unsigned)(clusters * L_CLUSTER)), dim3(L_THREADS), up_smem_bytes<GROUPS>(p), stream, dim3(L_CLUSTER, 1, 1), p);
     const int rc = RLIS_LAUNCH_CHECK();
     if (rc != 0) return rc;
@@ -756,10 +864,35 @@ struct RlisMoeLayer {
     float route_scale, slope, limit, shift;
 };
 
-// Bytes of workspace of a call.
-extern "C" int rlis_moe_layer_bytes(int n_tokens, int top, int inner, int inner_shared) {
-    const long long row = ((inner > inner_shared ? inner : inner_shared) + 7) / 8 * 8;
-    return (int)((sizeof(LayerPlan) + 15) / 16 * 16 + 4 * (long long)(n_tokens * top + n_tokens + 1) * row);
+namespace {
+// Where a call's parts of the workspace lie; `bytes` of it in all.
+struct LayerSpace {
+    long long h, top, x, bytes;
+    int h_row, top_row;
+};
+LayerSpace space_of(int n_tokens, int top, int width, int inner, int inner_shared, bool codes, int sms) {
+    LayerSpace s;
+    const int most = inner > inner_shared ? inner : inner_shared;
+    const long long rows = (long long)n_tokens * (top + 1) + 1;
+    s.h_row = (most + 7) / 8 * 8;
+    s.top_row = (s.h_row / 8 + 15) / 16 * 16;
+    s.h = (sizeof(LayerPlan) + 15) / 16 * 16;
+    s.top = s.h + 4 * rows * s.h_row;
+    s.x = s.top + (codes ? rows * s.top_row : 0);
+    s.bytes = s.x + (codes ? (long long)(sms / L_CLUSTER + 1) * n_tokens * width * 2 : 0);
+    return s;
+}
+int layer_sms() {
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+}  // namespace
+
+// Bytes of workspace of a call on the current device (0: a size that is not taken).
+extern "C" long long rlis_moe_layer_bytes(int n_tokens, int top, int width, int inner, int inner_shared, int codes) {
+    if (n_tokens < 0 || n_tokens > LT || top < 0 || top > L_MAX_PAIRS / LT || width < 0 || inner < 0 || inner_shared < 0) return 0;
+    return space_of(n_tokens, top, width, inner, inner_shared, codes != 0, layer_sms()).bytes;
 }
 
 extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
@@ -814,15 +947,20 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     p.limit = a->limit;
     p.shift = a->shift;
     p.plan = static_cast<LayerPlan*>(a->workspace);
-    p.h_row = ((a->inner > a->inner_shared ? a->inner : a->inner_shared) + 7) / 8 * 8;
-    p.h_hi = reinterpret_cast<bf16*>(static_cast<unsigned char*>(a->workspace) + (sizeof(LayerPlan) + 15) / 16 * 16);
-    p.h_lo = p.h_hi + (long long)(a->n_tokens * a->top + a->n_tokens + 1) * p.h_row;
+    const int sms = layer_sms();
+    const LayerSpace space = space_of(a->n_tokens, a->top, a->width, a->inner, a->inner_shared, codes, sms);
+    unsigned char* work = static_cast<unsigned char*>(a->workspace);
+    p.h_row = space.h_row;
+    p.top_row = space.top_row;
+    p.h_hi = reinterpret_cast<bf16*>(work + space.h);
+    p.h_lo = p.h_hi + ((long long)a->n_tokens * (a->top + 1) + 1) * p.h_row;
+    p.h = reinterpret_cast<float*>(work + space.h);
+    p.h_top = work + space.top;
+    p.x_scaled = reinterpret_cast<__half*>(work + space.x);
     p.out = static_cast<bf16*>(a->out);
     auto magic = [](int d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; };
     p.per_expert_magic = magic(a->inner / 8);
     p.own_chunks_magic = magic((a->inner + LK - 1) / LK);
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (p.n_tokens <= 8) return codes ? launch_layer<true, 1>(p, sms, stream) : launch_layer<false, 1>(p, sms, stream);
     return codes ? launch_layer<true, 2>(p, sms, stream) : launch_layer<false, 2>(p, sms, stream);
 }

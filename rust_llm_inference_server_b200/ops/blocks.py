@@ -197,8 +197,8 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
     shared expert in the same form; `interleave` (`shared_interleave`) as `moe_up` takes it (in blocks 0, 4 or a multiple of 8); the gating of `glu_act` with
     `slope`, `limit` and `up_shift`.  W, I and S are multiples of 8, in blocks of 16.
 
-    Scores, sums and the experts' gated results (as pairs of bfloat16, to 2^-17) are float32; a token's result is rounded once.  Codes are e4m3's finite
-    numbers here: a NaN code of a stored matrix counts as 480 (one that `quantize_matrix` wrote has a scale of NaN beside it)."""
+    Scores and sums are float32; the experts' gated results go into the second product to 2^-17 of each (beside codes to 2^-11); a token's result is rounded
+    once."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
         raise KernelError("moe_layer: expected bfloat16 rows [T, W] with unit stride on the device; there is no CPU path")
     dev = x.device
@@ -237,7 +237,7 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
         raise KernelError(f"moe_layer: out: expected contiguous bfloat16 {(T, W)} on {dev}")
     if T == 0:
         return out
-    work = torch.empty((lib().rlis_moe_layer_bytes(T, int(top), I2 // 2, S2 // 2),), dtype=torch.uint8, device=dev)
+    work = torch.empty((lib().rlis_moe_layer_bytes(T, int(top), W, I2 // 2, S2 // 2, 1 if blocks else 0),), dtype=torch.uint8, device=dev)
     call = _MoeLayer(x.data_ptr(), x.stride(0) if T > 1 else W, w_router.data_ptr(), _layer_vector(correction, n_out, dev, "correction"),
                      _layer_vector(router_bias, n_out, dev, "router_bias"), up, down, shared_up, shared_down, work.data_ptr(), out.data_ptr(), T, W, I2 // 2, S2 // 2, E,
                      int(n_identity), int(top), _SCORING[scoring], int(n_groups), int(keep), 1 if normalize else 0, 1 if shared_gate else 0, int(interleave),

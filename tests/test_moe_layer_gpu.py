@@ -81,11 +81,12 @@ def plain(m, top, scale=1.0, correction=None, router_bias=None, scoring="sigmoid
 
 def close(y, m, want, size, top):
     """Where the sums of a unit's first product are off by r of themselves, its gated result is off by about 3 r of its size at this data's sums (silu and the
-    product), and pairs of bfloat16 by 2^-17; the second sum by its own roundings.  Sums of K terms in float32, in the order of tensor-core steps: half a unit
+    product), and pairs of bfloat16 by 2^-17; the second sum by its own roundings.  Beside codes h is float16: every value is off by up to 2^-11 of it, their sum with
+    the second matrix by 2^-11 of the sum of sizes.  Sums of K terms in float32, in the order of tensor-core steps: half a unit
     for each of K / 16 + 16 additions, of the sum of sizes, which is up to about sqrt(K) of the sum."""
     K = max(m["x"].shape[1], 256)
     r = (K / 16 + 24) * 2.0 ** -23
-    bound = (3 * r * math.sqrt(K) / 4 + 2.0 ** -16 + r) * size
+    bound = (3 * r * math.sqrt(K) / 4 + (2.0 ** -16 if isinstance(m["up"], torch.Tensor) else 2.0 ** -11) + r) * size
     bound = bound + 2.0 ** -8 * (want.abs() + bound) + 1e-30
     y = y.double().cpu()
     assert bool(((y - want).abs() <= bound).all()), float(((y - want).abs() / bound).max())
@@ -140,8 +141,9 @@ def test_ties_go_to_the_lower_index_and_nan_is_not_chosen():
     close(call(m, 6, correction=torch.full((6,), float("-inf"), device="cuda")), m, want, size, 6)
 
 
-def test_a_token_that_is_no_number_leaves_the_others():
-    m = make(9, 128, 64, 8, 32)
+@pytest.mark.parametrize("blocks", [False, True])
+def test_a_token_that_is_no_number_leaves_the_others(blocks):
+    m = make(9, 128, 64, 8, 32, blocks=blocks)
     clean = call(m, 2)
     m["x"][4, 17] = float("nan")
     y = call(m, 2)
@@ -150,8 +152,20 @@ def test_a_token_that_is_no_number_leaves_the_others():
     assert torch.equal(call(m, 2)[[0, 8]], clean[[0, 8]])
 
 
-def test_all_tokens_at_one_expert_and_rows_inside_wider_ones():
-    m = make(16, 256, 64, 8, 0)
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 1e4, 1e12])
+@pytest.mark.parametrize("blocks", [False, True])
+def test_activations_of_any_size(blocks, size):
+    """Rows far from one, each of its own size, and values far below a row's largest."""
+    m = make(6, 256, 64, 8, 32, blocks=blocks)
+    m["router"] *= 0.0              # (so that their size decides nothing about the choice)
+    m["x"] = (m["x"].float() * size * 10.0 ** torch.arange(-2, 4, device="cuda")[:, None] * (4.0 ** -torch.arange(256, device="cuda").remainder(12))).bfloat16()
+    want, size_of, _ = plain(m, 3)
+    close(call(m, 3), m, want, size_of, 3)
+
+
+@pytest.mark.parametrize("blocks", [False, True])
+def test_all_tokens_at_one_expert_and_rows_inside_wider_ones(blocks):
+    m = make(16, 256, 64, 8, 0, blocks=blocks)
     correction = torch.zeros(8, device="cuda")
     correction[5] = 10.0
     want, size, chosen = plain(m, 1, correction=correction)
@@ -183,9 +197,31 @@ def test_the_layer_is_what_its_parts_are():
     assert bool(((call(m, 4, 2.5).double().cpu() - parts.double().cpu()).abs() <= 2.0 ** -7 * want.abs() + 2.0 ** -7 * size).all())
 
 
-def test_calls_at_once_and_from_a_graph():
+def test_codes_and_scales_from_a_checkpoint():
+    """Every e4m3 there is, NaN left to its own row, and scales of either sign."""
+    from rust_llm_inference_server_b200 import ops
+    m = make(3, 256, 32, 4, blocks=True)
+    every = torch.arange(256, device="cuda").to(torch.uint8)
+    every[127], every[255] = 0, 0
+    up = m["up"].values.clone().view(torch.uint8)
+    up[:, 5, :] = every
+    up[:, 37, :] = every.flip(0)
+    m["up"] = ops.BlockMatrix(up.view(torch.float8_e4m3fn), m["up"].scales * torch.tensor([[1.0, -0.5]], device="cuda"))
+    want, size, _ = plain(m, 4)
+    y = call(m, 4)
+    close(y, m, want, size, 4)
+    down = m["down"].values.clone().view(torch.uint8)
+    down[2, 9, 17] = 127                            # NaN: its feature, for every token that chose the expert (all)
+    m["down"] = ops.BlockMatrix(down.view(torch.float8_e4m3fn), m["down"].scales)
+    z = call(m, 4)
+    rest = torch.arange(256, device="cuda") != 9
+    assert bool(z[:, 9].isnan().all()) and torch.equal(z[:, rest], y[:, rest])
+
+
+@pytest.mark.parametrize("blocks", [False, True])
+def test_calls_at_once_and_from_a_graph(blocks):
     """Two streams, and two graphs whose replays lie side by side: every call has a workspace of its own."""
-    ms = [make(4, 256, 64, 16, 64, True, seed=s) for s in (1, 2)]
+    ms = [make(4, 256, 64, 16, 64, True, blocks=blocks, seed=s) for s in (1, 2)]
     want = [call(m, 4, shared_gate=True) for m in ms]
     streams = [torch.cuda.Stream() for _ in ms]
     torch.cuda.synchronize()
