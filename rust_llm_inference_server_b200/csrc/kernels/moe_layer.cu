@@ -38,6 +38,7 @@ constexpr int LK = 128;                 // k of a chunk
 constexpr int MOST_K = 16384;           // of a matrix of the layer (items' numbers stay within what a product divides)
 
 // An expert that some token chose: the tokens as bits, as a list (four bits each), and which of a token's choices it is (four bits a token).
+constexpr unsigned SECOND = 0x8000u;
 struct ActiveExpert {
     int expert;
     unsigned tokens;
@@ -72,8 +73,8 @@ struct LayerArgs {
     bf16 *h_hi, *h_lo;                  // [tokens * top + tokens + 1, h_row]: the pairs', the shared expert's, a row of zeros; or, beside codes, float32:
     float* h;
     unsigned char* h_top;               // the largest exponent of every eight of a row, rows top_row apart
-    __half* x_scaled;                   // [cluster of the up kernel][tokens][width]
-    int top_row;
+    bf16* x_copy;                       // [cluster of the up kernel][tokens][x_row] (float16 beside codes)
+    int top_row, x_row;
     int h_row;
     unsigned per_expert_magic, own_chunks_magic;        // see quotient()
     bf16* out;
@@ -94,25 +95,16 @@ template <bool CODES> struct Chunk {
     uint4 a[STEPS][2];
     float scale[2];             // codes: of row g, of row g + 8
 };
-// `row0`, `row1`: this lane's rows from the chunk's first k on, of which `left` are there.  (A whole chunk without a test for each load: zeros that may be wanted are
-// instructions, too.)
+// `row0`, `row1`: this lane's rows of K; the chunk is k0 .. k0 + 127.  What lies past the row's end is its last 16 bytes again, which meet zeros: the columns' rows
+// are padded with them, so that no chunk needs code of its own.
 template <bool CODES>
-__device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char* row0, const unsigned char* row1, int left, int lane) {
-    row0 += (lane & 3) * 16;
-    row1 += (lane & 3) * 16;
-    if (left >= LK) {
+__device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char* row0, const unsigned char* row1, int k0, int K, int lane) {
+    constexpr int PER = CODES ? 16 : 8;
 #pragma unroll
-        for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
-            c.a[s][0] = stream16(row0 + s * 64);
-            c.a[s][1] = stream16(row1 + s * 64);
-        }
-    } else {
-#pragma unroll
-        for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
-            const bool in = (s * 4 + (lane & 3)) * (CODES ? 16 : 8) < left;
-            c.a[s][0] = in ? stream16(row0 + s * 64) : make_uint4(0, 0, 0, 0);
-            c.a[s][1] = in ? stream16(row1 + s * 64) : make_uint4(0, 0, 0, 0);
-        }
+    for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
+        const int at = min(k0 + (s * 4 + (lane & 3)) * PER, K - PER) * (16 / PER);
+        c.a[s][0] = stream16(row0 + at);
+        c.a[s][1] = stream16(row1 + at);
     }
 }
 
@@ -146,31 +138,20 @@ template <bool CODES> struct Column {
     static constexpr int VECS = CODES ? 2 : 1;
     uint4 b[Chunk<CODES>::STEPS][VECS];
 };
-// `row`: the column's row from this lane's first k of the chunk on, of which `left` are there (what lies behind them meets zeros of A and is not read).
-template <bool CODES> __device__ __forceinline__ void load_column(Column<CODES>& c, const bf16* row, int left) {
-    constexpr int PER = CODES ? 16 : 8;
-    if (left >= LK) {
+// `row`: the column's row from this lane's first k of the chunk on.
+template <bool CODES> __device__ __forceinline__ void load_column(Column<CODES>& c, const bf16* row) {
 #pragma unroll
-        for (int s = 0; s < Chunk<CODES>::STEPS; ++s)
+    for (int s = 0; s < Chunk<CODES>::STEPS; ++s)
 #pragma unroll
-            for (int v = 0; v < Column<CODES>::VECS; ++v) c.b[s][v] = *reinterpret_cast<const uint4*>(row + s * 4 * PER + v * 8);
-    } else {
-#pragma unroll
-        for (int s = 0; s < Chunk<CODES>::STEPS; ++s)
-#pragma unroll
-            for (int v = 0; v < Column<CODES>::VECS; ++v) {
-                const int k = s * 4 * PER + v * 8;
-                c.b[s][v] = k < left ? *reinterpret_cast<const uint4*>(row + k) : make_uint4(0, 0, 0, 0);
-            }
-    }
+        for (int v = 0; v < Column<CODES>::VECS; ++v) c.b[s][v] = *reinterpret_cast<const uint4*>(row + s * (CODES ? 64 : 32) + v * 8);
 }
 // The same of a row of float32, scaled.
-__device__ __forceinline__ void load_column(Column<true>& c, const float* row, int left, float scaling) {
+__device__ __forceinline__ void load_column(Column<true>& c, const float* row, float scaling) {
 #pragma unroll
     for (int s = 0; s < Chunk<true>::STEPS; ++s) {
         float4 f[4];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) f[v] = s * 64 + v * 4 < left ? *reinterpret_cast<const float4*>(row + s * 64 + v * 4) : make_float4(0, 0, 0, 0);
+        for (int v = 0; v < 4; ++v) f[v] = *reinterpret_cast<const float4*>(row + s * 64 + v * 4);
 #pragma unroll
         for (int v = 0; v < 2; ++v)
             c.b[s][v] = make_uint4(pack_half(f[2 * v].x * scaling, f[2 * v].y * scaling), pack_half(f[2 * v].z * scaling, f[2 * v].w * scaling),
@@ -207,6 +188,16 @@ __device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<COD
     acc[1] = fmaf((part[0][1] + part[1][1]) * back1, s0, acc[1]);
     acc[2] = fmaf((part[0][2] + part[1][2]) * back0, s1, acc[2]);
     acc[3] = fmaf((part[0][3] + part[1][3]) * back1, s1, acc[3]);
+}
+
+// A loop over eights of tokens works on the first sums and puts them behind the others.
+__device__ __forceinline__ void swap_sums(float (&a)[4], float (&b)[4]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float t = a[i];
+        a[i] = b[i];
+        b[i] = t;
+    }
 }
 
 // ---- the choice ------------------------------------------------------------------------------------------------------------------------
@@ -321,6 +312,7 @@ template <int GROUPS> struct UpShared {
     unsigned top[L_WARPS];
     unsigned long long choice[L_MAX_OUT];       // which of a token's choices an expert is, four bits a token
     unsigned tokens[L_MAX_OUT];                 // the tokens that chose an expert
+    unsigned short work[2 * L_MAX_PAIRS];       // active experts, with SECOND set for those after the first eight of an expert's tokens
 };
 
 // This CTA's rows of the router against all tokens, into every CTA's z [LT][z_row].  Sixteen rows at a time; the warps share k: a warp takes 128 k of the
@@ -359,7 +351,7 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUP
                     v[r][0] = a[s][r][0].x, v[r][1] = a[s][r][0].y, v[r][2] = a[s][r][0].z, v[r][3] = a[s][r][0].w;
                     v[r][4] = a[s][r][1].x, v[r][5] = a[s][r][1].y, v[r][6] = a[s][r][1].z, v[r][7] = a[s][r][1].w;
                 }
-#pragma unroll
+#pragma unroll 1
                 for (int part = 0; part < 3; ++part) {
                     uint32_t w[2][4];
 #pragma unroll
@@ -405,30 +397,37 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUP
     }
 }
 
-// The cluster's copy of the tokens' rows as scaled float16 (8 KB of a token's row a CTA, two tokens at the most), and their exponents in every CTA.
-template <int GROUPS>
-__device__ __forceinline__ void scale_rows(const LayerArgs& p, UpShared<GROUPS>& sh, __half* to, int rank, int cluster) {
-    static_assert(L_CLUSTER * 2 >= LT && L_WARPS == 16, "eight warps a token");
-    const int warp = threadIdx.x >> 5, t = rank + cluster * (warp >> 3), i0 = threadIdx.x & 255;
+// The cluster's copy of the tokens' rows, padded with zeros to x_row; beside codes as scaled float16, and their exponents in every CTA.  Eight warps a token.
+template <bool CODES, int GROUPS>
+__device__ __forceinline__ void copy_rows(const LayerArgs& p, UpShared<GROUPS>& sh, bf16* to, int rank) {
+    static_assert(L_CLUSTER * 2 >= LT && L_WARPS == 16, "two tokens a CTA at the most");
+    const int warp = threadIdx.x >> 5, t = rank + L_CLUSTER * (warp >> 3), i0 = threadIdx.x & 255;
     const bf16* x = p.x + (long long)min(t, p.n_tokens - 1) * p.ldx;
-    unsigned m = 0u;
-    for (int k = i0 * 8; k < p.width; k += 2048) {
-        const uint4 v = *reinterpret_cast<const uint4*>(x + k);
-        m = __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    int e = 0;
+    if (CODES) {
+        unsigned m = 0u;
+        for (int k = i0 * 8; k < p.width; k += 2048) {
+            const uint4 v = *reinterpret_cast<const uint4*>(x + k);
+            m = __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+        }
+        m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+        if ((threadIdx.x & 31) == 0) sh.top[warp] = m;
+        __syncthreads();
+        for (int w = 0; w < 8; ++w) m = max(m, sh.top[(warp & 8) + w]);
+        e = max((int)(m >> 7), LEAST_EXPONENT);
     }
-    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
-    if ((threadIdx.x & 31) == 0) sh.top[warp] = m;
-    __syncthreads();
-    for (int w = 0; w < 8; ++w) m = max(m, sh.top[(warp & 8) + w]);
     if (t >= p.n_tokens) return;
-    const int e = max((int)(m >> 7), LEAST_EXPONENT);
     const float scaling = scaling_of(e);
-    for (int k = i0 * 8; k < p.width; k += 2048) {
-        const uint4 v = *reinterpret_cast<const uint4*>(x + k);
-        auto two = [&](uint32_t w) { return pack_half(__uint_as_float(w << 16) * scaling, __uint_as_float(w & 0xffff0000u) * scaling); };
-        *reinterpret_cast<uint4*>(to + (long long)t * p.width + k) = make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+#pragma unroll 1
+    for (int k = i0 * 8; k < p.x_row; k += 2048) {
+        uint4 v = k < p.width ? *reinterpret_cast<const uint4*>(x + k) : make_uint4(0, 0, 0, 0);
+        if (CODES) {
+            auto two = [&](uint32_t w) { return pack_half(__uint_as_float(w << 16) * scaling, __uint_as_float(w & 0xffff0000u) * scaling); };
+            v = make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
+        }
+        *reinterpret_cast<uint4*>(to + (long long)t * p.x_row + k) = v;
     }
-    if (i0 < cluster) st_cluster_f32(reinterpret_cast<float*>(&sh.exponent[t]), __int_as_float(e), (uint32_t)i0);
+    if (CODES && i0 < L_CLUSTER) st_cluster_f32(reinterpret_cast<float*>(&sh.exponent[t]), __int_as_float(e), (uint32_t)i0);
 }
 
 template <bool CODES, int GROUPS /* of eight tokens */>
@@ -446,8 +445,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
     }
     pdl_wait();
     router_logits<GROUPS>(p, sh, z, z_row, blockIdx.x % L_CLUSTER, L_CLUSTER);
-    __half* x_scaled = p.x_scaled + (long long)(blockIdx.x / L_CLUSTER) * p.n_tokens * p.width;
-    if (CODES) scale_rows<GROUPS>(p, sh, x_scaled, blockIdx.x % L_CLUSTER, L_CLUSTER);
+    bf16* x_copy = p.x_copy + (long long)(blockIdx.x / L_CLUSTER) * p.n_tokens * p.x_row;
+    copy_rows<CODES, GROUPS>(p, sh, x_copy, blockIdx.x % L_CLUSTER);
     cluster_sync_all();
 
     if (warp < p.n_tokens) {
@@ -469,12 +468,14 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
     }
     __syncthreads();
     // the experts that some token chose, ascending: every warp counts them all, 32 at a vote, and writes down its own
-    int n_active = 0;
+    int n_active = 0, n_work = 0;
     for (int c = 0; c * 32 < p.n_real; ++c) {
         const int e = c * 32 + lane;
-        const unsigned tokens = e < p.n_real ? sh.tokens[e] : 0u, votes = __ballot_sync(0xffffffffu, tokens != 0u);
+        const unsigned tokens = e < p.n_real ? sh.tokens[e] : 0u, votes = __ballot_sync(0xffffffffu, tokens != 0u), below = (1u << lane) - 1u;
+        const unsigned many = __ballot_sync(0xffffffffu, __popc(tokens) > 8);
         if (warp == c % L_WARPS && tokens != 0u) {
-            ActiveExpert& a = sh.plan.of[n_active + __popc(votes & ((1u << lane) - 1u))];
+            const int at = n_active + __popc(votes & below), w = n_work + __popc(votes & below) + __popc(many & below);
+            ActiveExpert& a = sh.plan.of[at];
             unsigned long long list = 0ull;
             int n = 0;
             for (unsigned m = tokens; m != 0u; m &= m - 1u, ++n) list |= (unsigned long long)(__ffs((int)m) - 1) << (4 * n);
@@ -482,8 +483,11 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
             a.tokens = tokens;
             a.list = list;
             a.choice = sh.choice[e];
+            sh.work[w] = (unsigned short)at;
+            if (n > 8) sh.work[w + 1] = (unsigned short)((unsigned)at | SECOND);
         }
         n_active += __popc(votes);
+        n_work += __popc(votes) + __popc(many);
     }
     if (threadIdx.x == 0) sh.plan.n_active = n_active;
     __syncthreads();
@@ -491,116 +495,104 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
         const int words = (int)(offsetof(LayerPlan, of) + (size_t)n_active * sizeof(ActiveExpert)) / 8;
         for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(p.plan)[i] = reinterpret_cast<const unsigned long long*>(&sh.plan)[i];
     }
-    if (blockIdx.x == 1) {              // (a cluster has more than one)
-        const long long at = (long long)p.n_tokens * (p.top + 1) * p.h_row;
-        for (int i = threadIdx.x; i < p.h_row; i += L_THREADS) {
-            if (CODES) p.h[at + i] = 0.f;
-            else p.h_hi[at + i] = p.h_lo[at + i] = __float2bfloat16_rn(0.f);
-        }
+    if (blockIdx.x == 1) {              // (a cluster has more than one)  What no item writes of h: the row of zeros, and the rows' ends
+        const int pairs = p.n_tokens * p.top, rows = pairs + p.n_tokens;
+        for (int row = warp; row <= rows; row += L_WARPS)
+            for (int i = (row == rows ? 0 : row < pairs ? p.inner : p.inner_shared) + lane; i < p.h_row; i += 32) {
+                const long long at = (long long)row * p.h_row + i;
+                if (CODES) p.h[at] = 0.f;
+                else p.h_hi[at] = p.h_lo[at] = __float2bfloat16_rn(0.f);
+            }
     }
     pdl_trigger();
 
-    // items: eight features of the shared expert, then of every active one; a team's warp takes every TEAM-th chunk of their k, a round each
-    const int shared_items = p.inner_shared / 8, per_expert = p.inner / 8, n_items = shared_items + n_active * per_expert;
+    // items: eight features for up to eight tokens, of the shared expert, then of the active ones; a team's warp takes every TEAM-th chunk of their k, a round each
+    const int per_shared = p.inner_shared / 8, shared_items = per_shared * ((p.n_tokens + 7) / 8), per_expert = p.inner / 8, n_items = shared_items + n_work * per_expert;
     const int n_chunks = (p.width + LK - 1) / LK, rounds = (n_chunks + TEAM - 1) / TEAM;
     const int team = warp / TEAM, member = warp % TEAM, stride = gridDim.x * TEAMS, first = team * gridDim.x + blockIdx.x;
-    auto active_of = [&](int item) { return quotient(item - shared_items, p.per_expert_magic); };
-    constexpr int AHEAD = CODES && GROUPS == 1 ? 4 : 2, K_BYTES = LK * (CODES ? 1 : 2);           // chunks that are held or on their way, as registers last
-    const int turns = (rounds + AHEAD - 1) / AHEAD * AHEAD;                            // (empty chunks fill an item's last turn)
-    // an item's rows from this warp's first chunk on, and their scales: row g of the 16 is a gate row, row g + 8 the row of the linear branch of the same feature
+    struct Item {
+        bool own, second;           // not the shared expert's; after the first eight tokens
+        int a, f0;                  // which active expert's, from which feature on
+    };
+    auto item_of = [&](int item) {
+        Item it;
+        it.own = item >= shared_items;
+        const int w = it.own ? quotient(item - shared_items, p.per_expert_magic) : 0, entry = it.own ? sh.work[w] : 0;
+        it.second = it.own ? (entry & SECOND) != 0u : item >= per_shared;
+        it.a = entry & (SECOND - 1u);
+        it.f0 = (it.own ? item - shared_items - w * per_expert : it.second ? item - per_shared : item) * 8;
+        return it;
+    };
+    // an item's rows and their scales: row g of the 16 is a gate row, row g + 8 the row of the linear branch of the same feature
     const unsigned char *row0 = nullptr, *row1 = nullptr;
     const float *scale0 = nullptr, *scale1 = nullptr;
     auto rows_of = [&](int item) {
-        const bool own = item >= shared_items;
-        const int a = own ? active_of(item) : 0, f = (own ? item - shared_items - a * per_expert : item) * 8 + g, e = own ? sh.plan.of[a].expert : 0;
-        const LayerMatrix& m = own ? p.up : p.shared_up;
-        const int il = own ? p.interleave : p.interleave_shared;
-        const int r0 = il == 0 ? f : il == 4 ? 2 * f - (f & 3) : f / il * 2 * il + f % il, r1 = r0 + (il > 0 ? il : own ? p.inner : p.inner_shared);
-        const unsigned char* base = m.w + e * m.stack_bytes + (long long)member * K_BYTES;
+        const Item it = item_of(item);
+        const int f = it.f0 + g, e = it.own ? sh.plan.of[it.a].expert : 0;
+        const LayerMatrix& m = it.own ? p.up : p.shared_up;
+        const int il = it.own ? p.interleave : p.interleave_shared;
+        const int r0 = il == 0 ? f : il == 4 ? 2 * f - (f & 3) : f / il * 2 * il + f % il, r1 = r0 + (il > 0 ? il : it.own ? p.inner : p.inner_shared);
+        const unsigned char* base = m.w + e * m.stack_bytes;
         row0 = base + r0 * m.row_bytes;
         row1 = base + r1 * m.row_bytes;
         if (CODES) {
-            const float* scales = m.scales + (long long)e * m.row_blocks * m.k_blocks + member;
+            const float* scales = m.scales + (long long)e * m.row_blocks * m.k_blocks;
             scale0 = scales + (long long)(r0 / LK) * m.k_blocks;
             scale1 = scales + (long long)(r1 / LK) * m.k_blocks;
         }
     };
-    auto load = [&](Chunk<CODES>& c, int round) {
-        const int chunk = member + round * TEAM;
-        if (chunk >= n_chunks) return;
-        load_chunk<CODES>(c, row0 + round * (TEAM * K_BYTES), row1 + round * (TEAM * K_BYTES), p.width - chunk * LK, lane);
-        if (CODES) c.scale[0] = scale0[round * TEAM], c.scale[1] = scale1[round * TEAM];
+    // A chunk of bfloat16 and the next one in turn, one on its way while the other is worked on; or two chunks of codes at once.  (Two pairs of codes, or three or four
+    // chunks in turn: 50.9, 57.1 and 53.6 us instead of 48.3 for 8 tokens and 20 experts of 1,024: more code to fetch.)
+    constexpr int UNIT = CODES ? 2 : 1, UNITS = CODES ? 1 : 2, TURN = UNITS * UNIT;
+    const int turns = (rounds + TURN - 1) / TURN * TURN;
+    Chunk<CODES> held[UNITS][UNIT];
+    auto load = [&](Chunk<CODES> (&unit)[UNIT], int round) {
+#pragma unroll
+        for (int i = 0; i < UNIT; ++i) {
+            const int chunk = min(member + (round + i) * TEAM, n_chunks - 1);
+            load_chunk<CODES>(unit[i], row0, row1, chunk * LK, p.width, lane);
+            if (CODES) unit[i].scale[0] = scale0[chunk], unit[i].scale[1] = scale1[chunk];
+        }
     };
-    Chunk<CODES> held[AHEAD];
     if (first < n_items) {
         rows_of(first);
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) load(held[i], i);
+        for (int u = 0; u < UNITS; ++u) load(held[u], u * UNIT);
     }
     int set = 0;
 #pragma unroll 1
     for (int item = first; item < n_items; item += stride) {
         {
-            const bool own = item >= shared_items;
-            const int a = own ? active_of(item) : 0;
-            // this lane's columns: the tokens that chose the expert, or all for the shared one (behind them the first token again, whose sums nobody reads)
-            const unsigned long long list = own ? sh.plan.of[a].list : 0xfedcba9876543210ull;
-            const int n_cols = own ? __popc(sh.plan.of[a].tokens) : p.n_tokens;
-            const int at = (lane & 3) * (CODES ? 16 : 8) + member * LK;
-            const bf16* x = CODES ? reinterpret_cast<const bf16*>(x_scaled) : p.x;
-            const long long ldx = CODES ? p.width : p.ldx;
-            const bf16 *x0 = x + (long long)((list >> (4 * g)) & 15) * ldx + at, *x1 = x + (long long)((list >> (32 + 4 * g)) & 15) * ldx + at;
-            float acc[GROUPS][4] = {};
+            // this lane's column: a token that chose the expert, or any for the shared one (behind them token 0, whose sums nobody reads)
+            const Item it = item_of(item);
+            const unsigned long long every = it.own ? sh.plan.of[it.a].list : 0xfedcba9876543210ull;
+            const unsigned list = (unsigned)(it.second ? every >> 32 : every);
+            const int n_cols = min(8, (it.own ? __popc(sh.plan.of[it.a].tokens) : p.n_tokens) - (it.second ? 8 : 0)), token = (int)(list >> (4 * g)) & 15;
+            const bf16* x = x_copy + (long long)(g < n_cols ? token : 0) * p.x_row + (lane & 3) * (CODES ? 16 : 8) + member * LK;
+            float acc[4] = {};
 #pragma unroll 1
-            for (int round = 0; round < turns; round += AHEAD) {
-                const bool last = round + AHEAD >= turns, more = !last || item + stride < n_items;
+            for (int round = 0; round < turns; round += TURN) {
+                const bool last = round + TURN >= turns, more = !last || item + stride < n_items;
                 if (last && more) rows_of(item + stride);
 #pragma unroll
-                for (int i = 0; i < AHEAD; i += 2) {
-                    // two chunks at a time, whose loads and sums do not wait for each other
-                    const int chunk = member + (round + i) * TEAM, k = (round + i) * TEAM * LK;
-                    Column<CODES> col_x[2][1];
-                    if ((chunk + TEAM + 1) * LK <= p.width) {
-                        load_column<CODES>(col_x[0][0], x0 + k, LK);
-                        load_column<CODES>(col_x[1][0], x0 + k + TEAM * LK, LK);
-                        multiply<CODES, 1>(held[i], col_x[0], acc[0]);
-                        multiply<CODES, 1>(held[i + 1], col_x[1], acc[0]);
-                        if (GROUPS > 1 && n_cols > 8) {
-                            load_column<CODES>(col_x[0][0], x1 + k, LK);
-                            load_column<CODES>(col_x[1][0], x1 + k + TEAM * LK, LK);
-                            multiply<CODES, 1>(held[i], col_x[0], acc[GROUPS - 1]);
-                            multiply<CODES, 1>(held[i + 1], col_x[1], acc[GROUPS - 1]);
-                        }
-                    } else {
+                for (int u = 0; u < UNITS; ++u, x += UNIT * TEAM * LK) {
+                    if (member + (round + u * UNIT) * TEAM < n_chunks) {
+                        // (a unit's second chunk that is not there is the last one again and meets zeros)
+                        Column<CODES> columns[UNIT][1];
 #pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            if (chunk + j * TEAM >= n_chunks) continue;
-                            const int kj = k + j * TEAM * LK, left = p.width - (chunk + j * TEAM) * LK >= LK ? LK : p.width - at - kj;
-                            load_column<CODES>(col_x[j][0], x0 + kj, left);
-                            multiply<CODES, 1>(held[i + j], col_x[j], acc[0]);
-                            if (GROUPS > 1 && n_cols > 8) {
-                                load_column<CODES>(col_x[j][0], x1 + kj, left);
-                                multiply<CODES, 1>(held[i + j], col_x[j], acc[GROUPS - 1]);
-                            }
-                        }
+                        for (int i = 0; i < UNIT; ++i) load_column<CODES>(columns[i][0], x + i * TEAM * LK);
+#pragma unroll
+                        for (int i = 0; i < UNIT; ++i) multiply<CODES, 1>(held[u][i], columns[i], acc);
                     }
-                    if (more) {
-                        load(held[i], last ? i : round + AHEAD + i);
-                        load(held[i + 1], last ? i + 1 : round + AHEAD + i + 1);
-                    }
+                    if (more) load(held[u], last ? u * UNIT : round + TURN + u * UNIT);
                 }
             }
-            const int f0 = (own ? item - shared_items - a * per_expert : item) * 8;
             auto& mine = sh.reduce[set][warp];
             const int col = (lane & 3) * 2;
-#pragma unroll
-            for (int n = 0; n < GROUPS; ++n) {
-                if (n == 1 && n_cols <= 8) break;
-                mine[g][n * 8 + col] = acc[n][0];
-                mine[g][n * 8 + col + 1] = acc[n][1];
-                mine[g + 8][n * 8 + col] = acc[n][2];
-                mine[g + 8][n * 8 + col + 1] = acc[n][3];
-            }
+            mine[g][col] = acc[0];
+            mine[g][col + 1] = acc[1];
+            mine[g + 8][col] = acc[2];
+            mine[g + 8][col + 1] = acc[3];
             // The team's warps take the ends of items in turn, and the others go on.  (As many sets as warps: before a warp writes a set again it has ended an item
             // itself since, for which it waited for all; the warp that read the set had done so by then.)  Barriers 0 .. 15: nothing else uses one from here on.
             const int barrier = team * TEAM + set, mine_to_end = set == member;
@@ -619,17 +611,10 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                     gate += sh.reduce[member][team * TEAM + w][f][c];
                     lin += sh.reduce[member][team * TEAM + w][f + 8][c];
                 }
-                int row, t = c;
-                float w;
-                if (own) {
-                    const ActiveExpert& ex = sh.plan.of[a];
-                    t = (int)(ex.list >> (4 * c)) & 15;
-                    row = t * p.top + ((int)(ex.choice >> (4 * t)) & 15);
-                    w = z[t * z_row + ex.expert];
-                } else {
-                    row = p.n_tokens * p.top + t;
-                    w = sh.gate[t];
-                }
+                const int t = (int)(list >> (4 * c)) & 15;
+                const ActiveExpert& ex = sh.plan.of[it.a];
+                const int row = it.own ? t * p.top + ((int)(ex.choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+                const float w = it.own ? z[t * z_row + ex.expert] : sh.gate[t];
                 if (CODES) {
                     const float back = unscaling_of(sh.exponent[t]);
                     gate *= back;
@@ -640,13 +625,13 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                     lin = lin > p.limit ? p.limit : lin < -p.limit ? -p.limit : lin;
                 }
                 const float v = glu_gate(gate, p.slope) * (lin + p.shift) * w;
-                const long long at = (long long)row * p.h_row + f0 + f;
+                const long long at = (long long)row * p.h_row + it.f0 + f;
                 if (CODES) {
                     p.h[at] = v;
                     unsigned e = __float_as_uint(v) >> 23 & 255u;           // of the eight lanes
 #pragma unroll
                     for (int o = 4; o > 0; o >>= 1) e = max(e, __shfl_xor_sync(0xffu << (lane & 24), e, o));
-                    if (f == 0) p.h_top[row * p.top_row + f0 / 8] = (unsigned char)e;
+                    if (f == 0) p.h_top[row * p.top_row + it.f0 / 8] = (unsigned char)e;
                 } else {
                     const bf16 hi = __float2bfloat16_rn(v);
                     p.h_hi[at] = hi;
@@ -700,8 +685,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK, n_chunks = shared_chunks + sh.plan.n_active * own_chunks;
     auto active_of = [&](int chunk) { return quotient(chunk - shared_chunks, p.own_chunks_magic); };
     const int step = parts * L_WARPS, first = rank * L_WARPS + warp;
-    constexpr int AHEAD = CODES ? 4 : 2, PER = CODES ? 16 : 8;              // 64 registers of chunks that are held or on their way
-    const int rounds = max(1, (n_chunks + step - 1) / step), turns = (rounds + AHEAD - 1) / AHEAD * AHEAD;       // (empty chunks fill the last turn)
+    constexpr int PER = CODES ? 16 : 8;
+    const int rounds = max(1, (n_chunks + step - 1) / step);
     struct Place {              // a chunk: which active expert's (or the shared one's), and where in its k
         bool own;
         int a, kb;
@@ -718,57 +703,58 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
         const Place at = place_of(chunk);
         const LayerMatrix& m = at.own ? p.down : p.shared_down;
         const int e = at.own ? sh.plan.of[at.a].expert : 0, r0 = min(group * 16 + g, p.width - 1), r1 = min(group * 16 + g + 8, p.width - 1);
-        const unsigned char* base = m.w + e * m.stack_bytes + (long long)at.kb * LK * (CODES ? 1 : 2);
-        load_chunk<CODES>(c, base + r0 * m.row_bytes, base + r1 * m.row_bytes, (at.own ? p.inner : p.inner_shared) - at.kb * LK, lane);
+        const unsigned char* base = m.w + e * m.stack_bytes;
+        load_chunk<CODES>(c, base + r0 * m.row_bytes, base + r1 * m.row_bytes, at.kb * LK, at.own ? p.inner : p.inner_shared, lane);
         if (CODES) {
             const float* s = m.scales + (long long)e * m.row_blocks * m.k_blocks + at.kb;
             c.scale[0] = s[(long long)(r0 / LK) * m.k_blocks];
             c.scale[1] = s[(long long)(r1 / LK) * m.k_blocks];
         }
     };
-    Chunk<CODES> held[AHEAD];
-#pragma unroll
-    for (int i = 0; i < AHEAD; ++i)
-        if (blockIdx.x / parts < n_groups) load(held[i], blockIdx.x / parts, first + i * step);
+    Chunk<CODES> held[2];           // this round's and the next one's
+    if (blockIdx.x / parts < n_groups) {
+        load(held[0], blockIdx.x / parts, first);
+        load(held[1], blockIdx.x / parts, first + step);
+    }
 #pragma unroll 1
     for (int group = blockIdx.x / parts; group < n_groups; group += clusters) {
         float acc[2][4] = {};
+        const bool more = group + clusters < n_groups;
 #pragma unroll 1
-        for (int round = 0; round < turns; round += AHEAD) {
-            const bool last = round + AHEAD >= turns, more = !last || group + clusters < n_groups;
-            const int next_group = last ? group + clusters : group, next_round = last ? 0 : round + AHEAD;
+        for (int round = 0; round < rounds; round += 2) {
 #pragma unroll
-            for (int i = 0; i < AHEAD; ++i) {
+            for (int i = 0; i < 2; ++i) {
                 const int chunk = first + (round + i) * step;
                 if (chunk < n_chunks) {
-                    // the columns: h's rows (both halves) of the tokens that chose the chunk's expert, from the second-level cache
+                    // the columns: h's rows of the tokens that chose the chunk's expert, from the second-level cache (the others': the row of zeros behind h's)
                     const Place at = place_of(chunk);
-                    const int whole = (at.own ? p.inner : p.inner_shared) - at.kb * LK, left = whole >= LK ? LK : whole - (lane & 3) * PER;
                     const unsigned seen = at.own ? sh.plan.of[at.a].tokens : (1u << p.n_tokens) - 1u;
                     const unsigned long long choice = at.own ? sh.plan.of[at.a].choice : 0ull;
-#pragma unroll
+                    auto row_of = [&](int t) {
+                        return !(seen >> t & 1u) ? p.n_tokens * (p.top + 1) : at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+                    };
+#pragma unroll 1
                     for (int n = 0; n < GROUPS; ++n) {
-                        if ((seen >> (8 * n) & 0xffu) == 0u) continue;
-                        // (the others' columns: the row of zeros behind h's)
-                        auto row_of = [&](int t) {
-                            return !(seen >> t & 1u) ? p.n_tokens * (p.top + 1) : at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
-                        };
-                        const int row = row_of(n * 8 + g);
-                        const long long from = (long long)row * p.h_row + at.kb * LK + (lane & 3) * PER;
-                        if constexpr (CODES) {
-                            Column<CODES> b[1];
-                            load_column(b[0], p.h + from, left, scaling_of(sh.exponent[row]));
-                            multiply<CODES, 1>(held[i], b, acc[n], unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2)]),
-                                               unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2 + 1)]));
-                        } else {
-                            Column<CODES> b[2];
-                            load_column<CODES>(b[0], p.h_hi + from, left);
-                            load_column<CODES>(b[1], p.h_lo + from, left);
-                            multiply<CODES, 2>(held[i], b, acc[n]);
+                        if ((seen >> (8 * n) & 0xffu) != 0u) {
+                            const int row = row_of(n * 8 + g);
+                            const long long from = (long long)row * p.h_row + at.kb * LK + (lane & 3) * PER;
+                            if constexpr (CODES) {
+                                Column<CODES> b[1];
+                                load_column(b[0], p.h + from, scaling_of(sh.exponent[row]));
+                                multiply<CODES, 1>(held[i], b, acc[0], unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2)]),
+                                                   unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2 + 1)]));
+                            } else {
+                                Column<CODES> b[2];
+                                load_column<CODES>(b[0], p.h_hi + from);
+                                load_column<CODES>(b[1], p.h_lo + from);
+                                multiply<CODES, 2>(held[i], b, acc[0]);
+                            }
                         }
+                        if (GROUPS > 1) swap_sums(acc[0], acc[1]);
                     }
                 }
-                if (more) load(held[i], next_group, first + (next_round + i) * step);
+                if (round + 2 < rounds) load(held[i], group, chunk + 2 * step);
+                else if (more) load(held[i], group + clusters, first + i * step);
             }
         }
         const int col = (lane & 3) * 2;
@@ -868,18 +854,19 @@ namespace {
 // Where a call's parts of the workspace lie; `bytes` of it in all.
 struct LayerSpace {
     long long h, top, x, bytes;
-    int h_row, top_row;
+    int h_row, top_row, x_row;
 };
 LayerSpace space_of(int n_tokens, int top, int width, int inner, int inner_shared, bool codes, int sms) {
     LayerSpace s;
     const int most = inner > inner_shared ? inner : inner_shared;
     const long long rows = (long long)n_tokens * (top + 1) + 1;
-    s.h_row = (most + 7) / 8 * 8;
+    s.h_row = (most + LK - 1) / LK * LK;
+    s.x_row = (width + LK - 1) / LK * LK + TEAM * LK;          // (a chunk more for a team's second chunks)
     s.top_row = (s.h_row / 8 + 15) / 16 * 16;
     s.h = (sizeof(LayerPlan) + 15) / 16 * 16;
     s.top = s.h + 4 * rows * s.h_row;
     s.x = s.top + (codes ? rows * s.top_row : 0);
-    s.bytes = s.x + (codes ? (long long)(sms / L_CLUSTER + 1) * n_tokens * width * 2 : 0);
+    s.bytes = s.x + (long long)(sms / L_CLUSTER + 1) * n_tokens * s.x_row * 2;
     return s;
 }
 int layer_sms() {
@@ -956,7 +943,8 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     p.h_lo = p.h_hi + ((long long)a->n_tokens * (a->top + 1) + 1) * p.h_row;
     p.h = reinterpret_cast<float*>(work + space.h);
     p.h_top = work + space.top;
-    p.x_scaled = reinterpret_cast<__half*>(work + space.x);
+    p.x_copy = reinterpret_cast<bf16*>(work + space.x);
+    p.x_row = space.x_row;
     p.out = static_cast<bf16*>(a->out);
     auto magic = [](int d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; };
     p.per_expert_magic = magic(a->inner / 8);
