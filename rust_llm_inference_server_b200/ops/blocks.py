@@ -48,6 +48,13 @@ class BlockRows:
     shape = property(lambda self: self.values.shape)
     device = property(lambda self: self.values.device)
 
+    @classmethod
+    def _made(cls, values: torch.Tensor, scales: torch.Tensor, stride: int):
+        """Of tensors that are known to be right."""
+        new = cls.__new__(cls)
+        new.values, new.scales, new.stride = values, scales, stride
+        return new
+
 
 class BlockMatrix:
     """A matrix [N, K], or a stack of them [E, N, K], in blocks: `values` e4m3 and `scales` float32 [.., ceil(N / 128), ceil(K / 128)]."""
@@ -64,53 +71,63 @@ class BlockMatrix:
 
     shape = property(lambda self: self.values.shape)
     device = property(lambda self: self.values.device)
+    _made = classmethod(BlockRows._made.__func__)
 
 
-def _room(shape: tuple, device) -> torch.Tensor:
-    """A new tensor of codes whose rows start at multiples of 16 bytes."""
+def _room(shape: tuple, device) -> tuple:
+    """A new tensor of codes whose rows start at multiples of 16 bytes, and the bytes from one to the next."""
     K = shape[-1]
-    room = torch.empty(shape[:-1] + (-(-K // 16) * 16,), dtype=CODES, device=device)
-    return room if room.shape[-1] == K else room[..., :K]
+    if K % 16 == 0:
+        return torch.empty(shape, dtype=CODES, device=device), K
+    stride = -(-K // 16) * 16
+    return torch.empty(shape[:-1] + (stride,), dtype=CODES, device=device)[..., :K], stride
 
 
-def _plain(x: torch.Tensor, dims: tuple, what: str) -> None:
+_FLOATS = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _plain(x: torch.Tensor, dims: tuple, what: str) -> int:
+    """Checks rows of plain values; their element type's code."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise KernelError(f"{what}: expected a CUDA tensor; there is no CPU path")
-    _code(x.dtype)
+    code = _FLOATS.get(x.dtype)
+    if code is None:
+        _code(x.dtype)
     if x.dim() not in dims or x.shape[-1] < 1 or (x.stride(-1) != 1 and x.shape[-1] > 1):
         raise KernelError(f"{what}: expected rows with unit stride, got {tuple(x.shape)} with strides {x.stride()}")
+    return code
 
 
 def quantize_rows(x: torch.Tensor) -> BlockRows:
     """Rows x [T, K] (bfloat16 or float32; may be a column slice of wider rows) in blocks of 128 of a row."""
-    _plain(x, (2,), "quantize_rows")
+    code = _plain(x, (2,), "quantize_rows")
     if x.get_device() != _device():
         with torch.cuda.device(x.device):
             return quantize_rows(x)
     T, K = x.shape
-    values = _room((T, K), x.device)
-    scales = torch.empty((-(-K // BLOCK), T), dtype=torch.float32, device=x.device)
-    rows = BlockRows(values, scales)
-    check(lib().rlis_quantize_rows(x.data_ptr(), x.stride(0), values.data_ptr(), rows.stride, scales.data_ptr(), T, K, _code(x.dtype), _stream()), "quantize_rows")
+    dev = x.device
+    values, stride = _room((T, K), dev)
+    scales = torch.empty((-(-K // BLOCK), T), dtype=torch.float32, device=dev)
+    check(lib().rlis_quantize_rows(x.data_ptr(), x.stride(0), values.data_ptr(), stride, scales.data_ptr(), T, K, code, _stream()), "quantize_rows")
     _count("quantize_rows")
-    return rows
+    return BlockRows._made(values, scales, stride)
 
 
 def quantize_matrix(w: torch.Tensor) -> BlockMatrix:
     """A weight [N, K], or a stack of them [E, N, K] (bfloat16 or float32, rows and matrices any distance apart), in blocks of 128 x 128."""
-    _plain(w, (2, 3), "quantize_matrix")
+    code = _plain(w, (2, 3), "quantize_matrix")
     if w.get_device() != _device():
         with torch.cuda.device(w.device):
             return quantize_matrix(w)
-    N, K = w.shape[-2:]
-    E = w.shape[0] if w.dim() == 3 else 1
-    values = _room(tuple(w.shape), w.device)
-    scales = torch.empty(tuple(w.shape[:-2]) + (-(-N // BLOCK), -(-K // BLOCK)), dtype=torch.float32, device=w.device)
-    matrix = BlockMatrix(values, scales)
-    check(lib().rlis_quantize_matrix(w.data_ptr(), w.stride(-2), w.stride(0) if w.dim() == 3 else 0, values.data_ptr(), matrix.stride, scales.data_ptr(), E, N, K,
-                                     _code(w.dtype), _stream()), "quantize_matrix")
+    shape, dev = tuple(w.shape), w.device
+    N, K = shape[-2:]
+    E = shape[0] if len(shape) == 3 else 1
+    values, stride = _room(shape, dev)
+    scales = torch.empty(shape[:-2] + (-(-N // BLOCK), -(-K // BLOCK)), dtype=torch.float32, device=dev)
+    check(lib().rlis_quantize_matrix(w.data_ptr(), w.stride(-2), w.stride(0) if len(shape) == 3 else 0, values.data_ptr(), stride, scales.data_ptr(), E, N, K, code,
+                                     _stream()), "quantize_matrix")
     _count("quantize_matrix")
-    return matrix
+    return BlockMatrix._made(values, scales, stride)
 
 
 def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> torch.Tensor:
@@ -120,25 +137,29 @@ def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> 
     `early`: w is a weight that no kernel still in flight writes, so that its first tiles may be asked for before the kernels before have finished."""
     if not isinstance(w, BlockMatrix) or w.values.dim() != 2:
         raise KernelError("linear_blocks: expected a BlockMatrix [N, K]")
+    weight = w.values
     plain = not isinstance(x, BlockRows)
-    if plain:
-        _plain(x, (2,), "linear_blocks")
-    N, K = w.values.shape
-    if x.shape[1] != K or x.device != w.values.device:
-        raise KernelError(f"linear_blocks: rows {tuple(x.shape)} on {x.device} and a matrix {(N, K)} on {w.device} do not go together")
-    out_code = _code(out_dtype or (x.dtype if plain else torch.bfloat16))
-    if w.values.get_device() != _device():
-        with torch.cuda.device(w.device):
+    code = _plain(x, (2,), "linear_blocks") if plain else 1
+    T, K = x.shape
+    N = weight.shape[0]
+    device = weight.get_device()
+    if weight.shape[1] != K or (x if plain else x.values).get_device() != device:
+        raise KernelError(f"linear_blocks: rows {tuple(x.shape)} on {x.device} and a matrix {tuple(weight.shape)} on {w.device} do not go together")
+    out_code = code if out_dtype is None else _FLOATS.get(out_dtype)
+    if out_code is None:
+        _code(out_dtype)
+    if device != _device():
+        with torch.cuda.device(device):
             return linear_blocks(x, w, out_dtype, early=early)
-    T = x.shape[0]
-    out = torch.empty((T, N), dtype=torch.bfloat16 if out_code else torch.float32, device=w.values.device)
+    dev = weight.device
+    out = torch.empty((T, N), dtype=torch.bfloat16 if out_code else torch.float32, device=dev)
     if plain:
-        scratch = torch.empty((T * (-(-K // 16) * 16 + 4 * -(-K // BLOCK)),), dtype=torch.uint8, device=w.values.device)
-        check(lib().rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), _code(x.dtype), scratch.data_ptr(), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(),
-                                          T, N, K, out_code, _stream()), "linear_blocks")
+        scratch = torch.empty((T * (-(-K // 16) * 16 + 4 * -(-K // BLOCK)),), dtype=torch.uint8, device=dev)
+        check(lib().rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), code, scratch.data_ptr(), weight.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
+                                          out_code, _stream()), "linear_blocks")
         _count("quantize_rows")
     else:
-        check(lib().rlis_blocks_gemm(x.values.data_ptr(), x.stride, x.scales.data_ptr(), w.values.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
+        check(lib().rlis_blocks_gemm(x.values.data_ptr(), x.stride, x.scales.data_ptr(), weight.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
                                      out_code, int(early), _stream()), "linear_blocks")
     _count("linear_blocks")
     return out
