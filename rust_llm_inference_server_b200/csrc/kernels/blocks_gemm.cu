@@ -18,6 +18,7 @@
 // meet and free their tensor memory.
 #include "blocks.cuh"
 #include "tcgen05_utils.cuh"
+#include <algorithm>
 
 namespace {
 using namespace tc;
@@ -28,13 +29,15 @@ constexpr int BG_THREADS = 384, BG_WARPS = 8;           // three groups of four 
 constexpr int BG_REGS_LAUNCH = 168, BG_REGS_FIRST = 56, BG_REGS_EPILOGUE = 224;
 static_assert(BG_REGS_FIRST + 2 * BG_REGS_EPILOGUE <= 3 * BG_REGS_LAUNCH && BG_THREADS * BG_REGS_LAUNCH <= 65536, "a split above what the launch holds waits for good");
 constexpr int BG_MAX_STAGES = 6, BG_MAX_BUFFERS = 4;
+constexpr int BG_MAX_SPLITS = 3;                        // the first pair's stages hold the others' sums
 constexpr int BG_STAGING = 8192;                        // bytes of results that an epilogue warp keeps for its stores at most
 
 template <int BN> __host__ __device__ constexpr int bg_stage_bytes() { return BG_A_BYTES + BN / 2 * QB; }
 template <int BN> __host__ __device__ constexpr int bg_stages() { return BN == 128 ? 6 : 5; }
+static_assert((BG_MAX_SPLITS - 1) * 128 * BG_M * 4 <= bg_stages<128>() * bg_stage_bytes<128>(), "room for the other pairs' sums");
 template <int BN> __host__ __device__ constexpr int bg_buffers() { return BN == 128 ? 4 : 2; }
-// Columns that one store takes: 128 bytes of a row, or 64 where a warp's 96 columns are no multiple of that.
-template <int BN, typename OutT> __host__ __device__ constexpr int bg_store_cols() { return BN == 192 ? 32 : 128 / (int)sizeof(OutT); }
+// Columns that one store takes: 128 bytes of a row.
+template <typename OutT> __host__ __device__ constexpr int bg_store_cols() { return 128 / (int)sizeof(OutT); }
 template <int BN, typename OutT> __host__ __device__ constexpr int bg_staging() {
     return BN / 2 * 32 * (int)sizeof(OutT) < BG_STAGING ? BN / 2 * 32 * (int)sizeof(OutT) : BG_STAGING;
 }
@@ -96,8 +99,8 @@ __device__ __forceinline__ void umma_e4m3_pair(uint32_t tmem_d, uint64_t adesc, 
         : "memory");
 }
 // An arrival at the barrier at this offset in both CTAs of the pair once the products issued so far are done.
-__device__ __forceinline__ void bg_commit_pair(uint64_t* bar) {
-    const unsigned short both = 3;
+__device__ __forceinline__ void bg_commit_pair(uint64_t* bar, uint32_t leader) {
+    const unsigned short both = (unsigned short)(3u << leader);
     asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
                  ::"r"(smem_u32(bar)), "h"(both) : "memory");
 }
@@ -131,19 +134,20 @@ __device__ __forceinline__ unsigned long long twice(float s) {
     asm("mov.b64 %0, {%1, %1};" : "=l"(r) : "r"(__float_as_uint(s)));
     return r;
 }
+__device__ __forceinline__ void add2(unsigned long long& acc, float a, float b) {
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
+    asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc) : "l"(v));
+}
 __device__ __forceinline__ float2 two_of(unsigned long long v) {
     uint32_t a, b;
     asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
     return make_float2(__uint_as_float(a), __uint_as_float(b));
 }
 
-// COLS sums of each of a warp's 32 rows (a row a lane) on their way out, in the layout that a bulk tensor copy of 32 rows reads: rows of 128 bytes in 16-byte pieces,
-// piece c of row r at c ^ (r % 8), or rows of 64 bytes, piece c at c ^ (r / 2 % 4); a quarter of a warp's lanes meet in no bank either way.
-template <int COLS, typename OutT>
-__device__ __forceinline__ int staged_piece(int row, int piece) {
-    if constexpr (COLS * sizeof(OutT) == 128) return row * 8 + (piece ^ (row & 7));
-    else return row * 4 + (piece ^ ((row >> 1) & 3));
-}
+// COLS sums (128 bytes) of each of a warp's 32 rows (a row a lane) on their way out, in the layout that a bulk tensor copy of 32 rows reads: 16-byte pieces, piece c of
+// row r at c ^ (r % 8), so that a quarter of a warp's lanes meet in no bank.
+__device__ __forceinline__ int staged_piece(int row, int piece) { return row * 8 + (piece ^ (row & 7)); }
 template <int COLS, typename OutT>
 __device__ __forceinline__ void stage_sums(const unsigned long long* acc, uint4* to) {
     const int lane = threadIdx.x & 31;
@@ -157,7 +161,7 @@ __device__ __forceinline__ void stage_sums(const unsigned long long* acc, uint4*
             const float2 a = two_of(acc[2 * v]), b = two_of(acc[2 * v + 1]);
             pk = make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
         }
-        to[staged_piece<COLS, OutT>(lane, v)] = pk;
+        to[staged_piece(lane, v)] = pk;
     }
 }
 // The same for results whose rows start anywhere: value by value.
@@ -168,19 +172,20 @@ __device__ __forceinline__ void store_staged(const uint4* from, OutT* __restrict
     for (int r = 0; r < 32 && row0 + r < M; ++r)
 #pragma unroll
         for (int c = lane; c < COLS; c += 32)
-            if (col + c < N) y[(size_t)(row0 + r) * N + col + c] = reinterpret_cast<const OutT*>(from)[staged_piece<COLS, OutT>(r, c / PER) * PER + c % PER];
+            if (col + c < N) y[(size_t)(row0 + r) * N + col + c] = reinterpret_cast<const OutT*>(from)[staged_piece(r, c / PER) * PER + c % PER];
 }
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
 }
 
 // Persistent: pair p works on tiles p, p + pairs, ...; tile t -> (n tile t / m_tiles, m tile t % m_tiles), so that the pairs that run together share a few
-// rows of w and all of x in L2.
+// rows of w and all of x in L2.  With few tiles the pairs of a cluster share one tile's k instead (splits of them, a tile a cluster): the others hand their sums to
+// the first through its shared memory, which adds them in the order of the splits.
 template <int BN, typename OutT>
 __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                                                                     const __grid_constant__ CUtensorMap map_y, const float* __restrict__ sx,
-                                                                    const float* __restrict__ sw, OutT* __restrict__ y, int M, int N, int k_blocks, int m_tiles,
-                                                                    int num_tiles, int bulk_stores, int early) {
+                                                                    const float* __restrict__ sw, OutT* __restrict__ y, int M, int N, int k_blocks, int per, int m_tiles,
+                                                                    int num_tiles, int splits, int bulk_stores, int early) {
     constexpr int STAGES = bg_stages<BN>(), BUFFERS = bg_buffers<BN>(), B_BYTES = BN / 2 * QB, HALF = BN / 2;
     constexpr uint32_t IDESC = idesc_e4m3(2 * BG_M, BN);
     extern __shared__ unsigned char bg_smem_raw[];
@@ -189,8 +194,9 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
     unsigned char *a_tiles = base, *b_tiles = base + STAGES * BG_A_BYTES, *staging = b_tiles + STAGES * B_BYTES;
     BgCtrl* ctrl = reinterpret_cast<BgCtrl*>(staging + BG_WARPS * bg_staging<BN, OutT>());
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = bg_cta_rank();
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    constexpr bool SPLIT = BN == 128;
+    const uint32_t cta = bg_cta_rank(), rank = SPLIT ? cta & 1u : cta, leader = SPLIT ? cta & ~1u : 0u;         // of the cluster, of its pair, and the pair's first
+    const int split = (int)(cta >> 1), kb0 = SPLIT ? split * per : 0, n_kb = SPLIT ? min(per, k_blocks - kb0) : k_blocks, pair = blockIdx.y, pairs = gridDim.y;
 
     if (threadIdx.x == 0) {
         ctrl->abort = 0;
@@ -219,21 +225,22 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
         if (warp == 0) {
             if (lane == 0) {
                 // the first stages' tiles of w before the kernel before this one has finished, where the caller says that it does not write them
-                const int first = early ? min(STAGES, k_blocks) : 0;
+                const int first = early ? min(STAGES, n_kb) : 0;
+                const uint32_t full = bg_in_cta(&ctrl->full[0], leader);
                 auto ask_w = [&](int s, int n0, int kb) {
                     if (rank == 0) bar_expect_tx(&ctrl->full[s], 2 * (BG_A_BYTES + B_BYTES));
-                    bg_load_pair(b_tiles + s * B_BYTES, &map_w, kb * QB, n0 + (int)rank * HALF, bg_in_cta(&ctrl->full[s], 0));
+                    bg_load_pair(b_tiles + s * B_BYTES, &map_w, (kb0 + kb) * QB, n0 + (int)rank * HALF, full + (uint32_t)s * 8u);
                 };
                 for (int kb = 0; kb < first; ++kb) ask_w(kb, (pair / m_tiles) * BN, kb);
                 pdl_wait();
                 int it = 0;
                 for (int tile = pair; tile < num_tiles && !ctrl->abort; tile += pairs) {
                     const int n0 = (tile / m_tiles) * BN, m0 = (tile % m_tiles) * 2 * BG_M;
-                    for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                    for (int kb = 0; kb < n_kb; ++kb, ++it) {
                         const int s = it % STAGES;
                         if (it >= STAGES && !bar_wait(&ctrl->empty[s], ((it / STAGES) - 1) & 1, &ctrl->abort)) break;
                         if (it >= first) ask_w(s, n0, kb);
-                        bg_load_pair(a_tiles + s * BG_A_BYTES, &map_x, kb * QB, m0 + (int)rank * BG_M, bg_in_cta(&ctrl->full[s], 0));
+                        bg_load_pair(a_tiles + s * BG_A_BYTES, &map_x, (kb0 + kb) * QB, m0 + (int)rank * BG_M, full + (uint32_t)s * 8u);
                     }
                 }
             }
@@ -243,7 +250,7 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
                 int it = 0;
                 bool fine = true;
                 for (int tile = pair; tile < num_tiles && fine; tile += pairs) {
-                    for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+                    for (int kb = 0; kb < n_kb; ++kb, ++it) {
                         const int s = it % STAGES, buf = it % BUFFERS;
                         if (!bar_wait_warp(&ctrl->full[s], (it / STAGES) & 1, &ctrl->abort)) { fine = false; break; }
                         const uint64_t adesc = smem_desc_sw128(a_tiles + s * BG_A_BYTES), bdesc = smem_desc_sw128(b_tiles + s * B_BYTES);
@@ -253,13 +260,18 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
     #pragma unroll
                             for (int k = 0; k < QB / 32; ++k)          // 32 codes further along the swizzled row
                                 umma_e4m3_pair(tmem_base + (uint32_t)(buf * BN), adesc + (uint64_t)(k * 32 >> 4), bdesc + (uint64_t)(k * 32 >> 4), IDESC, k != 0 ? 1u : 0u);
-                            bg_commit_pair(&ctrl->empty[s]);
-                            bg_commit_pair(&ctrl->acc_full[buf]);
+                            bg_commit_pair(&ctrl->empty[s], leader);
+                            bg_commit_pair(&ctrl->acc_full[buf], leader);
                         }
                         __syncwarp();
                     }
                 }
             }
+        }
+        if (SPLIT && splits > 1) {          // the epilogue's two meetings
+            __syncwarp();
+            cluster_sync_all();
+            cluster_sync_all();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(BG_REGS_EPILOGUE));
@@ -267,37 +279,33 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
         // epilogue: warp w may touch TMEM lanes 32 * (w % 4) .. + 31; two warps share them, half of the columns each
         const int q = warp & 3, half = (warp - 4) / 4;
         const int n_blocks = (N + QB - 1) / QB;
-        constexpr int COLS = bg_store_cols<BN, OutT>(), STORE_BYTES = COLS * 32 * (int)sizeof(OutT), STAGED = bg_staging<BN, OutT>() / STORE_BYTES;
+        constexpr int COLS = bg_store_cols<OutT>(), STORE_BYTES = COLS * 32 * (int)sizeof(OutT), STAGED = bg_staging<BN, OutT>() / STORE_BYTES;
         unsigned char* mine = staging + (warp - 4) * bg_staging<BN, OutT>();
-        const uint32_t released = bg_in_cta(&ctrl->acc_empty[0], 0);
+        const uint32_t released = bg_in_cta(&ctrl->acc_empty[0], leader);
         int it = 0;
         bool fine = true;
         for (int tile = pair; tile < num_tiles && fine; tile += pairs) {
             const int col0 = (tile / m_tiles) * BN + half * HALF, row0 = (tile % m_tiles) * 2 * BG_M + (int)rank * BG_M + q * 32, row = row0 + lane;
-            // this warp's columns lie in one block of w's rows, or (BN 192) in two that meet at a multiple of 32
-            const int nb = min(col0 / QB, n_blocks - 1), nb1 = min((col0 + HALF - 1) / QB, n_blocks - 1);
-            const int border = BN == 192 ? (col0 / QB + 1) * QB - col0 : HALF;
-            const float *pw = sw + (size_t)nb * k_blocks, *pw1 = sw + (size_t)nb1 * k_blocks, *px = sx + min(row, M - 1);
+            // this warp's columns lie in one block of w's rows
+            const float *pw = sw + (size_t)min(col0 / QB, n_blocks - 1) * k_blocks + kb0, *px = sx + min(row, M - 1) + (size_t)kb0 * M;
             unsigned long long acc[HALF / 2];
 #pragma unroll
             for (int i = 0; i < HALF / 2; ++i) acc[i] = 0ull;
             // the scales of two blocks ahead are on their way: a block takes less time than a load from memory
-            float a[2], b[2], b1[2];
+            float a[2], b[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const int kb = min(i, k_blocks - 1);
+                const int kb = min(i, n_kb - 1);
                 a[i] = px[(size_t)kb * M];
                 b[i] = pw[kb];
-                b1[i] = BN == 192 ? pw1[kb] : 0.f;
             }
 #pragma unroll 2
-            for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+            for (int kb = 0; kb < n_kb; ++kb, ++it) {
                 const int buf = it % BUFFERS;
-                const unsigned long long s2 = twice(a[kb & 1] * b[kb & 1]), s2b = BN == 192 ? twice(a[kb & 1] * b1[kb & 1]) : 0ull;
-                if (kb + 2 < k_blocks) {
+                const unsigned long long s2 = twice(a[kb & 1] * b[kb & 1]);
+                if (kb + 2 < n_kb) {
                     a[kb & 1] = px[(size_t)(kb + 2) * M];
                     b[kb & 1] = pw[kb + 2];
-                    if (BN == 192) b1[kb & 1] = pw1[kb + 2];
                 }
                 if (!bar_wait_warp(&ctrl->acc_full[buf], (it / BUFFERS) & 1, &ctrl->abort)) { fine = false; break; }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -306,7 +314,6 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
                 for (int c = 0; c < HALF / 32; ++c) {
                     uint32_t r[32];
                     tmem_ld32_pinned(from + (uint32_t)(c * 32), r);
-                    const unsigned long long s = BN == 192 && c * 32 >= border ? s2b : s2;
                     if (c + 1 == HALF / 32) {
                         // this warp has read its lanes of the accumulator: CTA 0's product warp may write it again
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -314,7 +321,30 @@ __global__ __launch_bounds__(BG_THREADS, 1) void blocks_gemm_kernel(const __grid
                         if (lane == 0) bg_arrive_cluster(released + (uint32_t)buf * 8u);
                     }
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], r[2 * i], r[2 * i + 1], s);
+                    for (int i = 0; i < 16; ++i) fma2(acc[c * 16 + i], r[2 * i], r[2 * i + 1], s2);
+                }
+            }
+            if (SPLIT && splits > 1) {
+                // every pair is done with its products and copies: the first one's stages hold the others' sums, [split][4 columns][row][column of 4]
+                cluster_sync_all();
+                float4* sums = reinterpret_cast<float4*>(base) + ((half * (HALF / 4)) * BG_M + q * 32 + lane);
+                if (split > 0) {
+                    const uint32_t to = bg_in_cta(sums + (size_t)(split - 1) * (BN / 4) * BG_M, rank);
+#pragma unroll
+                    for (int c = 0; c < HALF / 4; ++c) {
+                        const float2 v = two_of(acc[2 * c]), w = two_of(acc[2 * c + 1]);
+                        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(to + (uint32_t)(c * BG_M * 16)), "f"(v.x), "f"(v.y), "f"(w.x), "f"(w.y) : "memory");
+                    }
+                }
+                cluster_sync_all();
+                if (split > 0) break;
+                for (int o = 1; o < splits; ++o) {
+#pragma unroll
+                    for (int c = 0; c < HALF / 4; ++c) {
+                        const float4 v = sums[((size_t)(o - 1) * (BN / 4) + c) * BG_M];
+                        add2(acc[2 * c], v.x, v.y);
+                        add2(acc[2 * c + 1], v.z, v.w);
+                    }
                 }
             }
             if (!fine) break;
@@ -363,13 +393,13 @@ template <typename OutT> bool make_result_map(CUtensorMap* map, void* y, int M, 
     const cuuint32_t box[2] = {(cuuint32_t)cols, 32u};
     const cuuint32_t estr[2] = {1, 1};
     return fn(map, sizeof(OutT) == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              cols * sizeof(OutT) == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int BN, typename OutT>
-int launch_blocks_gemm(const void* x, long long ldx, const float* sx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int early, int sms,
-                       cudaStream_t stream) {
+int launch_blocks_gemm(const void* x, long long ldx, const float* sx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int splits,
+                       int early, int sms, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed{0};
     const cudaError_t e = rlis_allow_smem(blocks_gemm_kernel<BN, OutT>, (int)bg_smem<BN, OutT>(), allowed);
     if (e != cudaSuccess) return (int)e;
@@ -378,10 +408,13 @@ int launch_blocks_gemm(const void* x, long long ldx, const float* sx, const void
     // rows of the result that start at multiples of 16 bytes leave by bulk tensor copies
     const bool bulk = ((long long)N * (int)sizeof(OutT)) % 16 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
     map_y = map_x;
-    if (bulk && !make_result_map<OutT>(&map_y, y, M, N, bg_store_cols<BN, OutT>())) return RLIS_ERR_UNSUPPORTED;
-    const int m_tiles = (M + 2 * BG_M - 1) / (2 * BG_M), num_tiles = m_tiles * ((N + BN - 1) / BN), pairs = num_tiles < sms / 2 ? num_tiles : sms / 2;
-    rlis_launch_cluster(blocks_gemm_kernel<BN, OutT>, dim3((unsigned)(2 * pairs)), dim3(BG_THREADS), bg_smem<BN, OutT>(), stream, dim3(2, 1, 1), map_x, map_w, map_y, sx,
-                        sw, (OutT*)y, M, N, (K + QB - 1) / QB, m_tiles, num_tiles, bulk ? 1 : 0, early);
+    if (bulk && !make_result_map<OutT>(&map_y, y, M, N, bg_store_cols<OutT>())) return RLIS_ERR_UNSUPPORTED;
+    const int m_tiles = (M + 2 * BG_M - 1) / (2 * BG_M), num_tiles = m_tiles * ((N + BN - 1) / BN), k_blocks = (K + QB - 1) / QB;
+    const int per = (k_blocks + splits - 1) / splits;
+    splits = (k_blocks + per - 1) / per;                // none without a block
+    const int pairs = splits > 1 || num_tiles < sms / 2 ? num_tiles : sms / 2;
+    rlis_launch_cluster(blocks_gemm_kernel<BN, OutT>, dim3(2u * splits, (unsigned)pairs), dim3(BG_THREADS), bg_smem<BN, OutT>(), stream, dim3(2u * splits, 1, 1), map_x,
+                        map_w, map_y, sx, sw, (OutT*)y, M, N, k_blocks, per, m_tiles, num_tiles, splits, bulk ? 1 : 0, early);
     return RLIS_LAUNCH_CHECK();
 }
 }  // namespace
@@ -417,13 +450,21 @@ extern "C" int rlis_blocks_gemm(const void* x, long long ldx, const float* sx, c
         return M <= 16 ? RLIS_BF(16) : M <= 32 ? RLIS_BF(32) : M <= 64 ? RLIS_BF(64) : RLIS_BF(128);
 #undef RLIS_BF
     }
-    // The width of a tile: the one whose rounds over the pairs of SMs come to the fewest columns (a round of narrow tiles is shorter), the widest of equals.
-    const long long m_tiles = (M + 2 * BG_M - 1) / (2 * BG_M);
-    auto columns = [&](int bn) { const long long tiles = m_tiles * ((N + bn - 1) / bn); return (tiles + sms / 2 - 1) / (sms / 2) * bn; };
-    const int bn = columns(256) <= columns(192) && columns(256) <= columns(128) ? 256 : columns(192) <= columns(128) ? 192 : 128;
-#define RLIS_BG(BN) (f32 ? launch_blocks_gemm<BN, float>(x, ldx, sx, w, ldw, sw, y, M, N, K, early, sms, stream) \
-                         : launch_blocks_gemm<BN, bf16>(x, ldx, sx, w, ldw, sw, y, M, N, K, early, sms, stream))
-    return bn == 256 ? RLIS_BG(256) : bn == 192 ? RLIS_BG(192) : RLIS_BG(128);
+    // The width of a tile: a round of 128 columns over the pairs of SMs takes 0.8 of one of 256 (as many steps along k, each waiting for the sums before it), so the
+    // narrow ones pay only where they need no more rounds (us in 128 / 256 columns: 512 x 4,096 of K 4096, one round either way, 14.9 / 17.8; 509 x 6,100 of K 4000,
+    // two rounds or one, 29.5 / 21.4; 1,024 x 14,336 of K 4096 73.4 / 61.1; 192 columns were slower than one of the two at all of 13 sizes).
+    const long long m_tiles = (M + 2 * BG_M - 1) / (2 * BG_M), pairs = sms / 2;
+    auto rounds = [&](int bn) { return (m_tiles * ((N + bn - 1) / bn) + pairs - 1) / pairs; };
+    const bool wide = 4 * rounds(128) >= 5 * rounds(256);
+    // The pairs that a round of narrow tiles leaves idle take shares of k, where that shortens it by 12 blocks or more: a block is 0.3 us, the meeting of the sums 3
+    // (us in 1 / 2 / 3 shares: 129 x 4,096 of K 14336 37.2 / 25.3 / more than the pairs; 256 x 2,048 of K 8192 23.2 / 17.2 / 15.4; 129 x 1,024 of K 4096 13.5 / 11.5 /
+    // 10.9; 300 x 2,048 of K 2048, where 2 shares save 8 blocks, 9.2 / 9.8).
+    const int k_blocks = (K + QB - 1) / QB;
+    int splits = wide ? 1 : (int)std::min<long long>(BG_MAX_SPLITS, std::max<long long>(1, pairs / (m_tiles * ((N + 127) / 128))));
+    if (k_blocks - (k_blocks + splits - 1) / splits < 12) splits = 1;
+#define RLIS_BG(BN) (f32 ? launch_blocks_gemm<BN, float>(x, ldx, sx, w, ldw, sw, y, M, N, K, splits, early, sms, stream) \
+                         : launch_blocks_gemm<BN, bf16>(x, ldx, sx, w, ldw, sw, y, M, N, K, splits, early, sms, stream))
+    return wide ? RLIS_BG(256) : RLIS_BG(128);
 #undef RLIS_BG
 }
 
