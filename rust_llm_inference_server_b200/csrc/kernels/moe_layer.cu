@@ -70,7 +70,7 @@ struct LayerArgs {
     LayerMatrix up, down, shared_up, shared_down;
     float slope, limit, shift;
     LayerPlan* plan;
-    bf16 *h_hi, *h_lo;                  // [tokens * top + tokens + 1, h_row]: the pairs', the shared expert's, a row of zeros; or, beside codes, float32:
+    bf16 *h_hi, *h_lo;                  // [tokens * top + tokens, h_row]: the pairs', the shared expert's; or, beside codes, float32:
     float* h;
     unsigned char* h_top;               // the largest exponent of every eight of a row, rows top_row apart
     bf16* x_copy;                       // [cluster of the up kernel][tokens][x_row] (float16 beside codes)
@@ -158,10 +158,11 @@ __device__ __forceinline__ void load_column(Column<true>& c, const float* row, f
                                    pack_half(f[2 * v + 1].x * scaling, f[2 * v + 1].y * scaling), pack_half(f[2 * v + 1].z * scaling, f[2 * v + 1].w * scaling));
     }
 }
-// acc += chunk * the sum of the columns (COLS of each of eight tokens), times `back0` and `back1` in the lane's two columns.  Neighbouring instructions add to different sums: one waits some 35 cycles for the one before
-// it on the same.
+// acc += chunk * the sum of the columns (COLS of each of eight tokens), times `back0` and `back1` in the lane's two columns, of those that are `wanted` (bits 0 and 1: a
+// weight that is no number must not reach a token that did not choose the expert).  Neighbouring instructions add to different sums: one waits some 35 cycles
+// for the one before it on the same.
 template <bool CODES, int COLS>
-__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<CODES> (&cols)[COLS], float (&acc)[4], float back0 = 1.f, float back1 = 1.f) {
+__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<CODES> (&cols)[COLS], float (&acc)[4], unsigned wanted = 3u, float back0 = 1.f, float back1 = 1.f) {
     float part[2][4] = {};
 #pragma unroll
     for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
@@ -184,10 +185,14 @@ __device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<COD
         }
     }
     const float s0 = CODES ? c.scale[0] : 1.f, s1 = CODES ? c.scale[1] : 1.f;
-    acc[0] = fmaf((part[0][0] + part[1][0]) * back0, s0, acc[0]);
-    acc[1] = fmaf((part[0][1] + part[1][1]) * back1, s0, acc[1]);
-    acc[2] = fmaf((part[0][2] + part[1][2]) * back0, s1, acc[2]);
-    acc[3] = fmaf((part[0][3] + part[1][3]) * back1, s1, acc[3]);
+    if (wanted & 1u) {
+        acc[0] = fmaf((part[0][0] + part[1][0]) * back0, s0, acc[0]);
+        acc[2] = fmaf((part[0][2] + part[1][2]) * back0, s1, acc[2]);
+    }
+    if (wanted & 2u) {
+        acc[1] = fmaf((part[0][1] + part[1][1]) * back1, s0, acc[1]);
+        acc[3] = fmaf((part[0][3] + part[1][3]) * back1, s1, acc[3]);
+    }
 }
 
 // A loop over eights of tokens works on the first sums and puts them behind the others.
@@ -495,10 +500,10 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
         const int words = (int)(offsetof(LayerPlan, of) + (size_t)n_active * sizeof(ActiveExpert)) / 8;
         for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(p.plan)[i] = reinterpret_cast<const unsigned long long*>(&sh.plan)[i];
     }
-    if (blockIdx.x == 1) {              // (a cluster has more than one)  What no item writes of h: the row of zeros, and the rows' ends
+    if (blockIdx.x == 1) {              // (a cluster has more than one)  What no item writes of h: the rows' ends
         const int pairs = p.n_tokens * p.top, rows = pairs + p.n_tokens;
-        for (int row = warp; row <= rows; row += L_WARPS)
-            for (int i = (row == rows ? 0 : row < pairs ? p.inner : p.inner_shared) + lane; i < p.h_row; i += 32) {
+        for (int row = warp; row < rows; row += L_WARPS)
+            for (int i = (row < pairs ? p.inner : p.inner_shared) + lane; i < p.h_row; i += 32) {
                 const long long at = (long long)row * p.h_row + i;
                 if (CODES) p.h[at] = 0.f;
                 else p.h_hi[at] = p.h_lo[at] = __float2bfloat16_rn(0.f);
@@ -647,7 +652,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
 struct DownShared {
     float reduce[L_WARPS][16][LT + 1];
     float cluster[16][LT];
-    int exponent[L_MAX_PAIRS + LT + 1];         // beside codes: of h's rows
+    int exponent[L_MAX_PAIRS + LT];             // beside codes: of h's rows
     LayerPlan plan;
 };
 
@@ -679,7 +684,6 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
             for (int o = 4; o > 0; o >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
             if ((lane & 7) == 0 && row < n_rows) sh.exponent[row] = max((int)e, LEAST_EXPONENT);
         }
-        if (threadIdx.x == 0) sh.exponent[n_rows] = LEAST_EXPONENT;
         __syncthreads();
     }
     const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK, n_chunks = shared_chunks + sh.plan.n_active * own_chunks;
@@ -726,28 +730,29 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
             for (int i = 0; i < 2; ++i) {
                 const int chunk = first + (round + i) * step;
                 if (chunk < n_chunks) {
-                    // the columns: h's rows of the tokens that chose the chunk's expert, from the second-level cache (the others': the row of zeros behind h's)
+                    // the columns: h's rows of the tokens that chose the chunk's expert, from the second-level cache (the others': any row)
                     const Place at = place_of(chunk);
                     const unsigned seen = at.own ? sh.plan.of[at.a].tokens : (1u << p.n_tokens) - 1u;
                     const unsigned long long choice = at.own ? sh.plan.of[at.a].choice : 0ull;
                     auto row_of = [&](int t) {
-                        return !(seen >> t & 1u) ? p.n_tokens * (p.top + 1) : at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+                        return !(seen >> t & 1u) ? 0 : at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
                     };
 #pragma unroll 1
                     for (int n = 0; n < GROUPS; ++n) {
                         if ((seen >> (8 * n) & 0xffu) != 0u) {
                             const int row = row_of(n * 8 + g);
+                            const unsigned wanted = seen >> (n * 8 + (lane & 3) * 2);
                             const long long from = (long long)row * p.h_row + at.kb * LK + (lane & 3) * PER;
                             if constexpr (CODES) {
                                 Column<CODES> b[1];
                                 load_column(b[0], p.h + from, scaling_of(sh.exponent[row]));
-                                multiply<CODES, 1>(held[i], b, acc[0], unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2)]),
+                                multiply<CODES, 1>(held[i], b, acc[0], wanted, unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2)]),
                                                    unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2 + 1)]));
                             } else {
                                 Column<CODES> b[2];
                                 load_column<CODES>(b[0], p.h_hi + from);
                                 load_column<CODES>(b[1], p.h_lo + from);
-                                multiply<CODES, 2>(held[i], b, acc[0]);
+                                multiply<CODES, 2>(held[i], b, acc[0], wanted);
                             }
                         }
                         if (GROUPS > 1) swap_sums(acc[0], acc[1]);
@@ -859,7 +864,7 @@ struct LayerSpace {
 LayerSpace space_of(int n_tokens, int top, int width, int inner, int inner_shared, bool codes, int sms) {
     LayerSpace s;
     const int most = inner > inner_shared ? inner : inner_shared;
-    const long long rows = (long long)n_tokens * (top + 1) + 1;
+    const long long rows = (long long)n_tokens * (top + 1);
     s.h_row = (most + LK - 1) / LK * LK;
     s.x_row = (width + LK - 1) / LK * LK + TEAM * LK;          // (a chunk more for a team's second chunks)
     s.top_row = (s.h_row / 8 + 15) / 16 * 16;
@@ -940,7 +945,7 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     p.h_row = space.h_row;
     p.top_row = space.top_row;
     p.h_hi = reinterpret_cast<bf16*>(work + space.h);
-    p.h_lo = p.h_hi + ((long long)a->n_tokens * (a->top + 1) + 1) * p.h_row;
+    p.h_lo = p.h_hi + (long long)a->n_tokens * (a->top + 1) * p.h_row;
     p.h = reinterpret_cast<float*>(work + space.h);
     p.h_top = work + space.top;
     p.x_copy = reinterpret_cast<bf16*>(work + space.x);

@@ -152,6 +152,29 @@ def test_a_token_that_is_no_number_leaves_the_others(blocks):
     assert torch.equal(call(m, 2)[[0, 8]], clean[[0, 8]])
 
 
+@pytest.mark.parametrize("T", [5, 13])
+@pytest.mark.parametrize("blocks", [False, True])
+def test_weights_that_are_no_numbers_reach_only_who_chose_them(blocks, T):
+    from rust_llm_inference_server_b200 import ops
+    m = make(T, 144, 80, 6, 32, blocks=blocks)
+    clean, (_, _, chosen) = call(m, 2), plain(m, 2)
+    e = next(e for e in range(6) if 0 < sum(e in c for c in chosen) < T)
+    who = torch.tensor([e in c for c in chosen], device="cuda")
+    for name, at in (("up", (e, 70, 143)), ("down", (e, 33, 79)), ("down", (e, 16, 0))):
+        bad = dict(m)
+        if blocks:
+            codes = m[name].values.clone().view(torch.uint8)
+            codes[at] = 127
+            bad[name] = ops.BlockMatrix(codes.view(torch.float8_e4m3fn), m[name].scales)
+        else:
+            bad[name] = m[name].clone()
+            bad[name][at] = float("inf") if at[1] == 16 else float("nan")
+        y = call(bad, 2)
+        assert torch.equal(y[~who], clean[~who])
+        touched = y[who] if name == "up" else y[who][:, at[1]]
+        assert not bool(touched.isfinite().any())
+
+
 @pytest.mark.parametrize("size", [1e-30, 1e-6, 1e4, 1e12])
 @pytest.mark.parametrize("blocks", [False, True])
 def test_activations_of_any_size(blocks, size):
