@@ -72,10 +72,8 @@ struct LayerArgs {
     LayerPlan* plan;
     bf16 *h_hi, *h_lo;                  // [tokens * top + tokens, h_row]: the pairs', the shared expert's; or, beside codes, float32:
     float* h;
-    unsigned char* h_top;               // the largest exponent of every eight of a row, rows top_row apart
     bf16* x_copy;                       // [cluster of the up kernel][tokens][x_row] (float16 beside codes)
-    int top_row, x_row;
-    int h_row;
+    int x_row, h_row;
     unsigned per_expert_magic, own_chunks_magic;        // see quotient()
     bf16* out;
 };
@@ -87,25 +85,6 @@ __device__ __forceinline__ uint4 stream16(const void* p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
     return v;
-}
-
-// 128 k of rows g and g + 8 of a warp's 16 (g = lane / 4): lane % 4 holds every fourth 16 bytes.
-template <bool CODES> struct Chunk {
-    static constexpr int STEPS = CODES ? 2 : 4;
-    uint4 a[STEPS][2];
-    float scale[2];             // codes: of row g, of row g + 8
-};
-// `row0`, `row1`: this lane's rows of K; the chunk is k0 .. k0 + 127.  What lies past the row's end is its last 16 bytes again, which meet zeros: the columns' rows
-// are padded with them, so that no chunk needs code of its own.
-template <bool CODES>
-__device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char* row0, const unsigned char* row1, int k0, int K, int lane) {
-    constexpr int PER = CODES ? 16 : 8;
-#pragma unroll
-    for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
-        const int at = min(k0 + (s * 4 + (lane & 3)) * PER, K - PER) * (16 / PER);
-        c.a[s][0] = stream16(row0 + at);
-        c.a[s][1] = stream16(row1 + at);
-    }
 }
 
 // Four codes as float16, in their order.
@@ -124,6 +103,39 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], const uint32_t (&a)
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+template <bool CODES> __device__ __forceinline__ void mma_step(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (CODES) mma_f16_16816(d, a, b0, b1);
+    else mma_bf16_16816(d, a, b0, b1);
+}
+
+// 128 k of rows g and g + 8 of a warp's 16 (g = lane / 4): lane % 4 holds every fourth 16 bytes.
+template <bool CODES> struct Chunk {
+    static constexpr int STEPS = CODES ? 2 : 4, PARTS = CODES ? 4 : 2;         // instructions a step
+    uint4 a[STEPS][2];
+    float scale[2];             // codes: of row g, of row g + 8
+    __device__ __forceinline__ void operand(int s, int j, uint32_t (&to)[4]) const {
+        const uint32_t r0[4] = {a[s][0].x, a[s][0].y, a[s][0].z, a[s][0].w}, r1[4] = {a[s][1].x, a[s][1].y, a[s][1].z, a[s][1].w};
+        if constexpr (CODES) {
+            widen_codes(r0[j], to[0], to[2]);
+            widen_codes(r1[j], to[1], to[3]);
+        } else {
+            to[0] = r0[2 * j], to[1] = r1[2 * j], to[2] = r0[2 * j + 1], to[3] = r1[2 * j + 1];
+        }
+    }
+};
+// `row0`, `row1`: this lane's rows of K; the chunk is k0 .. k0 + 127.  What lies past the row's end is its last 16 bytes again, which meet zeros: the columns' rows
+// are padded with them, so that no chunk needs code of its own.
+template <bool CODES>
+__device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char* row0, const unsigned char* row1, int k0, int K, int lane) {
+    constexpr int PER = CODES ? 16 : 8;
+#pragma unroll
+    for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
+        const int at = min(k0 + (s * 4 + (lane & 3)) * PER, K - PER) * (16 / PER);
+        c.a[s][0] = stream16(row0 + at);
+        c.a[s][1] = stream16(row1 + at);
+    }
+}
+
 // The powers of two that bring a row whose largest float32 exponent is e (biased) to 2^14 .. 2^15 and back; rows below 2^-112 stay below that.
 constexpr int LEAST_EXPONENT = 15;
 __device__ __forceinline__ float scaling_of(int e) { return __uint_as_float((unsigned)(268 - e) << 23); }
@@ -145,64 +157,24 @@ template <bool CODES> __device__ __forceinline__ void load_column(Column<CODES>&
 #pragma unroll
         for (int v = 0; v < Column<CODES>::VECS; ++v) c.b[s][v] = *reinterpret_cast<const uint4*>(row + s * (CODES ? 64 : 32) + v * 8);
 }
-// The same of a row of float32, scaled.
-__device__ __forceinline__ void load_column(Column<true>& c, const float* row, float scaling) {
-#pragma unroll
-    for (int s = 0; s < Chunk<true>::STEPS; ++s) {
-        float4 f[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) f[v] = *reinterpret_cast<const float4*>(row + s * 64 + v * 4);
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-            c.b[s][v] = make_uint4(pack_half(f[2 * v].x * scaling, f[2 * v].y * scaling), pack_half(f[2 * v].z * scaling, f[2 * v].w * scaling),
-                                   pack_half(f[2 * v + 1].x * scaling, f[2 * v + 1].y * scaling), pack_half(f[2 * v + 1].z * scaling, f[2 * v + 1].w * scaling));
-    }
-}
-// acc += chunk * the sum of the columns (COLS of each of eight tokens), times `back0` and `back1` in the lane's two columns, of those that are `wanted` (bits 0 and 1: a
-// weight that is no number must not reach a token that did not choose the expert).  Neighbouring instructions add to different sums: one waits some 35 cycles
-// for the one before it on the same.
-template <bool CODES, int COLS>
-__device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<CODES> (&cols)[COLS], float (&acc)[4], unsigned wanted = 3u, float back0 = 1.f, float back1 = 1.f) {
+// acc += chunk * column.  Neighbouring instructions add to different sums: one waits some 35 cycles for the one before it on the same.
+template <bool CODES> __device__ __forceinline__ void multiply(const Chunk<CODES>& c, const Column<CODES>& col, float (&acc)[4]) {
     float part[2][4] = {};
 #pragma unroll
     for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
-        const uint32_t r0[4] = {c.a[s][0].x, c.a[s][0].y, c.a[s][0].z, c.a[s][0].w}, r1[4] = {c.a[s][1].x, c.a[s][1].y, c.a[s][1].z, c.a[s][1].w};
 #pragma unroll
-        for (int j = 0; j < (CODES ? 4 : 2); ++j) {
+        for (int j = 0; j < Chunk<CODES>::PARTS; ++j) {
             uint32_t a[4];
-            if constexpr (CODES) {
-                widen_codes(r0[j], a[0], a[2]);
-                widen_codes(r1[j], a[1], a[3]);
-            } else {
-                a[0] = r0[2 * j], a[1] = r1[2 * j], a[2] = r0[2 * j + 1], a[3] = r1[2 * j + 1];
-            }
-#pragma unroll
-            for (int i = 0; i < COLS; ++i) {
-                const uint4 b = cols[i].b[s][CODES ? j / 2 : 0];
-                if constexpr (CODES) mma_f16_16816(part[(j + i) & 1], a, j & 1 ? b.z : b.x, j & 1 ? b.w : b.y);
-                else mma_bf16_16816(part[(j + i) & 1], a, j & 1 ? b.z : b.x, j & 1 ? b.w : b.y);
-            }
+            c.operand(s, j, a);
+            const uint4 b = col.b[s][CODES ? j / 2 : 0];
+            mma_step<CODES>(part[j & 1], a, j & 1 ? b.z : b.x, j & 1 ? b.w : b.y);
         }
     }
     const float s0 = CODES ? c.scale[0] : 1.f, s1 = CODES ? c.scale[1] : 1.f;
-    if (wanted & 1u) {
-        acc[0] = fmaf((part[0][0] + part[1][0]) * back0, s0, acc[0]);
-        acc[2] = fmaf((part[0][2] + part[1][2]) * back0, s1, acc[2]);
-    }
-    if (wanted & 2u) {
-        acc[1] = fmaf((part[0][1] + part[1][1]) * back1, s0, acc[1]);
-        acc[3] = fmaf((part[0][3] + part[1][3]) * back1, s1, acc[3]);
-    }
-}
-
-// A loop over eights of tokens works on the first sums and puts them behind the others.
-__device__ __forceinline__ void swap_sums(float (&a)[4], float (&b)[4]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float t = a[i];
-        a[i] = b[i];
-        b[i] = t;
-    }
+    acc[0] = fmaf(part[0][0] + part[1][0], s0, acc[0]);
+    acc[1] = fmaf(part[0][1] + part[1][1], s0, acc[1]);
+    acc[2] = fmaf(part[0][2] + part[1][2], s1, acc[2]);
+    acc[3] = fmaf(part[0][3] + part[1][3], s1, acc[3]);
 }
 
 // ---- the choice ------------------------------------------------------------------------------------------------------------------------
@@ -500,15 +472,6 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
         const int words = (int)(offsetof(LayerPlan, of) + (size_t)n_active * sizeof(ActiveExpert)) / 8;
         for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(p.plan)[i] = reinterpret_cast<const unsigned long long*>(&sh.plan)[i];
     }
-    if (blockIdx.x == 1) {              // (a cluster has more than one)  What no item writes of h: the rows' ends
-        const int pairs = p.n_tokens * p.top, rows = pairs + p.n_tokens;
-        for (int row = warp; row < rows; row += L_WARPS)
-            for (int i = (row < pairs ? p.inner : p.inner_shared) + lane; i < p.h_row; i += 32) {
-                const long long at = (long long)row * p.h_row + i;
-                if (CODES) p.h[at] = 0.f;
-                else p.h_hi[at] = p.h_lo[at] = __float2bfloat16_rn(0.f);
-            }
-    }
     pdl_trigger();
 
     // items: eight features for up to eight tokens, of the shared expert, then of the active ones; a team's warp takes every TEAM-th chunk of their k, a round each
@@ -583,11 +546,11 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                 for (int u = 0; u < UNITS; ++u, x += UNIT * TEAM * LK) {
                     if (member + (round + u * UNIT) * TEAM < n_chunks) {
                         // (a unit's second chunk that is not there is the last one again and meets zeros)
-                        Column<CODES> columns[UNIT][1];
+                        Column<CODES> columns[UNIT];
 #pragma unroll
-                        for (int i = 0; i < UNIT; ++i) load_column<CODES>(columns[i][0], x + i * TEAM * LK);
+                        for (int i = 0; i < UNIT; ++i) load_column<CODES>(columns[i], x + i * TEAM * LK);
 #pragma unroll
-                        for (int i = 0; i < UNIT; ++i) multiply<CODES, 1>(held[u][i], columns[i], acc);
+                        for (int i = 0; i < UNIT; ++i) multiply<CODES>(held[u][i], columns[i], acc);
                     }
                     if (more) load(held[u], last ? u * UNIT : round + TURN + u * UNIT);
                 }
@@ -633,10 +596,6 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                 const long long at = (long long)row * p.h_row + it.f0 + f;
                 if (CODES) {
                     p.h[at] = v;
-                    unsigned e = __float_as_uint(v) >> 23 & 255u;           // of the eight lanes
-#pragma unroll
-                    for (int o = 4; o > 0; o >>= 1) e = max(e, __shfl_xor_sync(0xffu << (lane & 24), e, o));
-                    if (f == 0) p.h_top[row * p.top_row + it.f0 / 8] = (unsigned char)e;
                 } else {
                     const bf16 hi = __float2bfloat16_rn(v);
                     p.h_hi[at] = hi;
@@ -649,192 +608,274 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
 
 // ---- down ------------------------------------------------------------------------------------------------------------------------------
 
+constexpr int PARTS = 4;                                    // CTAs of a cluster: they share the chunks
+constexpr int LEAST_TEAMS = 2, MOST_TEAMS = 4;              // of a CTA: each has 16 output features of its own, and its warps share the CTA's chunks
+constexpr int HELD = 2;                                     // chunks that a warp has on their way
+template <bool CODES> __host__ __device__ constexpr int slot_bytes() { return CODES ? LK * 2 : LK * 4; }
+
 struct DownShared {
     float reduce[L_WARPS][16][LT + 1];
-    float cluster[16][LT];
-    int exponent[L_MAX_PAIRS + LT];             // beside codes: of h's rows
     LayerPlan plan;
+    int n_slots, next;                                      // of h's pieces that are in shared memory, and the first chunk whose are not
 };
+// Behind it, for `cap` slots: h's pieces (128 k of a token's row), then what brings a slot's sums back, where a slot's piece lies in h (row * 128 + chunk of its k),
+// and the first slot of a chunk.
+template <bool CODES> constexpr size_t down_smem_bytes(int cap) { return sizeof(DownShared) + (size_t)cap * (slot_bytes<CODES>() + 4 + 2 + 2); }
+template <bool CODES> constexpr int most_slots() { return (int)((227 * 1024 - sizeof(DownShared)) / (slot_bytes<CODES>() + 8)) / 8 * 8; }
+static_assert(sizeof(DownShared) % 16 == 0, "vectors of 16 bytes behind it");
+static_assert(most_slots<false>() >= LT * L_WARPS / LEAST_TEAMS * HELD, "a turn of all warps' chunks with all tokens");
+static_assert((L_MAX_PAIRS + LT) * (MOST_K / LK) <= 65536, "a piece's place in 16 bits");
 
-// CTA r of a cluster of `parts` takes its share of the chunks of 16 output features; a cluster takes features 16 (blockIdx / parts), ...
+// Where unit u of eight k lies within a slot: the four lanes of a load side by side (beside codes a lane takes 16 k, two units, at a time), the halves of odd slots
+// exchanged, so that the two slots that a quarter of a warp reads meet in no bank.
+template <bool CODES> __device__ __forceinline__ int unit_of(int u, int slot) {
+    const int at = CODES ? (u & 8) | (u & 1) << 2 | (u >> 1 & 3) : u;
+    return at ^ (slot & 1) << 2;
+}
+
+// A cluster takes 16 * teams output features at a time; the chunks (of the shared expert, then of the active ones) go round its CTAs, and round the warps of a
+// team.
 template <bool CODES, int GROUPS>
-__global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const LayerArgs p, int parts) {
+__global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const LayerArgs p, int teams, int cap) {
     extern __shared__ __align__(16) unsigned char down_smem[];
     DownShared& sh = *reinterpret_cast<DownShared*>(down_smem);
+    constexpr int SLOT = slot_bytes<CODES>();
+    unsigned char* pieces = down_smem + sizeof(DownShared);
+    float* back = reinterpret_cast<float*>(pieces + (size_t)cap * SLOT);
+    unsigned short *place = reinterpret_cast<unsigned short*>(back + cap), *slot_of = place + cap;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
-    const int rank = blockIdx.x % parts, clusters = gridDim.x / parts, n_groups = (p.width + 15) / 16;
+    const int rank = blockIdx.x % PARTS, n_groups = (p.width + 15) / 16, clusters = gridDim.x / PARTS;
+    const int members = L_WARPS / teams, team = warp / members, member = warp % members;
     pdl_wait();
     // (as much of the plan as the step can have: its length comes with it)
     const int words = (int)(offsetof(LayerPlan, of) + (size_t)min(p.n_tokens * p.top, p.n_real) * sizeof(ActiveExpert)) / 8;
     for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(&sh.plan)[i] = reinterpret_cast<const unsigned long long*>(p.plan)[i];
     __syncthreads();
     pdl_trigger();
-    if (CODES) {
-        // eight lanes a row
-        const int n_rows = p.n_tokens * (p.top + 1);
-#pragma unroll 1
-        for (int row = threadIdx.x >> 3; row < (n_rows + 3) / 4 * 4; row += L_THREADS / 8) {
-            const int n = (row < p.n_tokens * p.top ? p.inner : p.inner_shared) / 16;
-            const unsigned short* tops = reinterpret_cast<const unsigned short*>(p.h_top + min(row, n_rows - 1) * p.top_row);
-            unsigned e = 0u;
-#pragma unroll 8
-            for (int i = lane & 7; i < n; i += 8) e = __vmaxu4(e, tops[i]);
-            e = max(e & 255u, e >> 8);
-#pragma unroll
-            for (int o = 4; o > 0; o >>= 1) e = max(e, __shfl_xor_sync(0xffffffffu, e, o));
-            if ((lane & 7) == 0 && row < n_rows) sh.exponent[row] = max((int)e, LEAST_EXPONENT);
-        }
-        __syncthreads();
-    }
-    const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK, n_chunks = shared_chunks + sh.plan.n_active * own_chunks;
-    auto active_of = [&](int chunk) { return quotient(chunk - shared_chunks, p.own_chunks_magic); };
-    const int step = parts * L_WARPS, first = rank * L_WARPS + warp;
-    constexpr int PER = CODES ? 16 : 8;
-    const int rounds = max(1, (n_chunks + step - 1) / step);
+    // this CTA's chunks: number i is chunk rank + PARTS * i of all
+    const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK, all_chunks = shared_chunks + sh.plan.n_active * own_chunks;
+    const int n_chunks = (all_chunks - rank + PARTS - 1) / PARTS;
     struct Place {              // a chunk: which active expert's (or the shared one's), and where in its k
         bool own;
         int a, kb;
+        unsigned tokens;
     };
-    auto place_of = [&](int chunk) {
+    auto place_of = [&](int i) {
+        const int chunk = rank + PARTS * i;
         Place at;
         at.own = chunk >= shared_chunks;
         at.a = at.own ? quotient(chunk - shared_chunks, p.own_chunks_magic) : 0;
         at.kb = at.own ? (chunk - shared_chunks) - at.a * own_chunks : chunk;
+        at.tokens = at.own ? sh.plan.of[at.a].tokens : (1u << p.n_tokens) - 1u;
         return at;
     };
-    auto load = [&](Chunk<CODES>& c, int group, int chunk) {
-        if (chunk >= n_chunks) return;
-        const Place at = place_of(chunk);
+    auto load = [&](Chunk<CODES>& c, int group, int i) {
+        if (i >= n_chunks) return;
+        const Place at = place_of(i);
         const LayerMatrix& m = at.own ? p.down : p.shared_down;
         const int e = at.own ? sh.plan.of[at.a].expert : 0, r0 = min(group * 16 + g, p.width - 1), r1 = min(group * 16 + g + 8, p.width - 1);
         const unsigned char* base = m.w + e * m.stack_bytes;
         load_chunk<CODES>(c, base + r0 * m.row_bytes, base + r1 * m.row_bytes, at.kb * LK, at.own ? p.inner : p.inner_shared, lane);
-        if (CODES) {
-            const float* s = m.scales + (long long)e * m.row_blocks * m.k_blocks + at.kb;
-            c.scale[0] = s[(long long)(r0 / LK) * m.k_blocks];
-            c.scale[1] = s[(long long)(r1 / LK) * m.k_blocks];
-        }
+        if (CODES)      // (sixteen rows lie in one block)
+            c.scale[0] = m.scales[((long long)e * m.row_blocks + r0 / LK) * m.k_blocks + at.kb];
     };
-    Chunk<CODES> held[2];           // this round's and the next one's
-    if (blockIdx.x / parts < n_groups) {
-        load(held[0], blockIdx.x / parts, first);
-        load(held[1], blockIdx.x / parts, first + step);
-    }
-#pragma unroll 1
-    for (int group = blockIdx.x / parts; group < n_groups; group += clusters) {
-        float acc[2][4] = {};
-        const bool more = group + clusters < n_groups;
-#pragma unroll 1
-        for (int round = 0; round < rounds; round += 2) {
+    // The pieces of h that the chunks from `from` on meet, as many as there are slots for (whole turns of all warps), into shared memory; beside codes scaled.
+    auto fill = [&](int from) {
+        __syncthreads();                // nobody reads the last ones any more
+        if (warp == 0) {
+            int used = 0, i = from;
+            for (bool room = true; room && i < n_chunks;) {
+                const bool have = i + lane < n_chunks;
+                const Place at = place_of(have ? i + lane : from);
+                const int n = have ? __popc(at.tokens) : 0;
+                int upto = n;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int chunk = first + (round + i) * step;
-                if (chunk < n_chunks) {
-                    // the columns: h's rows of the tokens that chose the chunk's expert, from the second-level cache (the others': any row)
-                    const Place at = place_of(chunk);
-                    const unsigned seen = at.own ? sh.plan.of[at.a].tokens : (1u << p.n_tokens) - 1u;
-                    const unsigned long long choice = at.own ? sh.plan.of[at.a].choice : 0ull;
-                    auto row_of = [&](int t) {
-                        return !(seen >> t & 1u) ? 0 : at.own ? t * p.top + ((int)(choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
-                    };
-#pragma unroll 1
-                    for (int n = 0; n < GROUPS; ++n) {
-                        if ((seen >> (8 * n) & 0xffu) != 0u) {
-                            const int row = row_of(n * 8 + g);
-                            const unsigned wanted = seen >> (n * 8 + (lane & 3) * 2);
-                            const long long from = (long long)row * p.h_row + at.kb * LK + (lane & 3) * PER;
-                            if constexpr (CODES) {
-                                Column<CODES> b[1];
-                                load_column(b[0], p.h + from, scaling_of(sh.exponent[row]));
-                                multiply<CODES, 1>(held[i], b, acc[0], wanted, unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2)]),
-                                                   unscaling_of(sh.exponent[row_of(n * 8 + (lane & 3) * 2 + 1)]));
-                            } else {
-                                Column<CODES> b[2];
-                                load_column<CODES>(b[0], p.h_hi + from);
-                                load_column<CODES>(b[1], p.h_lo + from);
-                                multiply<CODES, 2>(held[i], b, acc[0], wanted);
-                            }
-                        }
-                        if (GROUPS > 1) swap_sums(acc[0], acc[1]);
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                const unsigned fits = __ballot_sync(0xffffffffu, have && used + upto <= cap);
+                int take = __popc(fits);
+                if (take < min(32, n_chunks - i)) {
+                    room = false;
+                    take -= (i + take - from) % (members * HELD);           // (no less than none: see the assertion above)
+                }
+                const int first = used + upto - n;
+                if (lane < take) {
+                    slot_of[i + lane - from] = (unsigned short)first;
+                    int k = first;
+                    for (unsigned m = at.tokens; m != 0u; m &= m - 1u, ++k) {
+                        const int t = __ffs((int)m) - 1;
+                        const int row = at.own ? t * p.top + ((int)(sh.plan.of[at.a].choice >> (4 * t)) & 15) : p.n_tokens * p.top + t;
+                        place[k] = (unsigned short)(row * (MOST_K / LK) + at.kb);
                     }
                 }
-                if (round + 2 < rounds) load(held[i], group, chunk + 2 * step);
-                else if (more) load(held[i], group + clusters, first + i * step);
+                used = take > 0 ? __shfl_sync(0xffffffffu, used + upto, take - 1) : used;
+                i += take;
+            }
+            if (lane == 0) {
+                sh.n_slots = used;
+                sh.next = i;
+            }
+        }
+        __syncthreads();
+        const int n_slots = sh.n_slots;
+#pragma unroll 4
+        for (int slot = warp; slot < n_slots; slot += L_WARPS) {
+            const int row = place[slot] / (MOST_K / LK), k0 = place[slot] % (MOST_K / LK) * LK, inner = row < p.n_tokens * p.top ? p.inner : p.inner_shared;
+            unsigned char* to = pieces + (size_t)slot * SLOT;
+            if constexpr (CODES) {
+                const int k = k0 + lane * 4;
+                const float4 v = k < inner ? *reinterpret_cast<const float4*>(p.h + (long long)row * p.h_row + k) : make_float4(0, 0, 0, 0);
+                const unsigned top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
+                                         max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
+                const int e = max((int)(__reduce_max_sync(0xffffffffu, top) >> 23), LEAST_EXPONENT);
+                const float scaling = scaling_of(e);
+                *reinterpret_cast<uint2*>(to + unit_of<CODES>(lane >> 1, slot) * 16 + (lane & 1) * 8) =
+                    make_uint2(pack_half(v.x * scaling, v.y * scaling), pack_half(v.z * scaling, v.w * scaling));
+                if (lane == 0) back[slot] = unscaling_of(e);
+            } else {
+                const int k = k0 + (lane & 15) * 8;
+                *reinterpret_cast<uint4*>(to + (lane >> 4) * (LK * 2) + unit_of<CODES>(lane & 15, slot) * 16) =
+                    k < inner ? *reinterpret_cast<const uint4*>((lane < 16 ? p.h_hi : p.h_lo) + (long long)row * p.h_row + k) : make_uint4(0, 0, 0, 0);
+            }
+        }
+        __syncthreads();
+    };
+
+    Chunk<CODES> held[HELD];
+    int group = (blockIdx.x / PARTS) * teams + team;
+#pragma unroll
+    for (int u = 0; u < HELD; ++u) load(held[u], group, member + u * members);
+    int from = 0, upto = 0;             // the chunks whose pieces are in shared memory: all of them, as a rule
+#pragma unroll 1
+    for (int group0 = group - team; group0 < n_groups; group0 += clusters * teams, group += clusters * teams) {
+        float acc[GROUPS][4] = {};
+#pragma unroll 1
+        for (int turn = 0; turn < n_chunks; turn += HELD * members) {
+            if (turn < from || turn >= upto) {
+                fill(turn);
+                from = turn;
+                upto = sh.next;
+            }
+#pragma unroll
+            for (int u = 0; u < HELD; ++u) {
+                const int i = turn + u * members + member;
+                if (i < n_chunks) {
+                    const Place at = place_of(i);
+                    const int first = slot_of[i - from];
+                    uint32_t a[Chunk<CODES>::STEPS][Chunk<CODES>::PARTS][4];
+#pragma unroll
+                    for (int s = 0; s < Chunk<CODES>::STEPS; ++s)
+#pragma unroll
+                        for (int j = 0; j < Chunk<CODES>::PARTS; ++j) held[u].operand(s, j, a[s][j]);
+                    const float scale = CODES ? held[u].scale[0] : 1.f;
+#pragma unroll
+                    for (int n = 0; n < GROUPS; ++n) {
+                        if (GROUPS > 1 && (at.tokens >> (8 * n) & 0xffu) == 0u) continue;
+                        // the columns: the tokens that chose the chunk's expert (the others': any of them; their sums are left out, so that a weight that is no
+                        // number does not reach them)
+                        const int t = n * 8 + g, slot = first + (at.tokens >> t & 1u ? __popc(at.tokens & ((1u << t) - 1u)) : 0);
+                        const unsigned char* piece = pieces + (size_t)slot * SLOT;
+                        const int flip = (slot & 1) << 6;
+                        float part[2][4] = {};
+#pragma unroll
+                        for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
+#pragma unroll
+                            for (int v = 0; v < 2; ++v) {           // codes: the halves of the step's k; else h's two numbers
+                                const uint4 b = *reinterpret_cast<const uint4*>(
+                                    piece + ((CODES ? s * 128 + v * 64 : v * (LK * 2) + s * 64) + (lane & 3) * 16 ^ flip));
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    const int q = CODES ? 2 * v + j : j;
+                                    mma_step<CODES>(part[(j + (CODES ? 0 : v)) & 1], a[s][q], j ? b.z : b.x, j ? b.w : b.y);
+                                }
+                            }
+                        }
+                        const int t0 = n * 8 + (lane & 3) * 2;
+#pragma unroll
+                        for (int c = 0; c < 2; ++c)
+                            if (at.tokens >> (t0 + c) & 1u) {
+                                const float by = CODES ? back[first + __popc(at.tokens & ((1u << (t0 + c)) - 1u))] : 1.f;
+                                acc[n][c] = fmaf((part[0][c] + part[1][c]) * by, scale, acc[n][c]);
+                                acc[n][2 + c] = fmaf((part[0][2 + c] + part[1][2 + c]) * by, scale, acc[n][2 + c]);
+                            }
+                    }
+                }
+                if (turn + HELD * members < n_chunks) load(held[u], group, i + HELD * members);
+                else if (group0 + clusters * teams < n_groups) load(held[u], group + clusters * teams, member + u * members);
             }
         }
         const int col = (lane & 3) * 2;
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < GROUPS; ++n) {
             sh.reduce[warp][g][n * 8 + col] = acc[n][0];
             sh.reduce[warp][g][n * 8 + col + 1] = acc[n][1];
             sh.reduce[warp][g + 8][n * 8 + col] = acc[n][2];
             sh.reduce[warp][g + 8][n * 8 + col + 1] = acc[n][3];
         }
-        __syncthreads();
-        const int f = threadIdx.x & 15, t = threadIdx.x >> 4;
-        float v = 0.f;
-        if (t < p.n_tokens) {
-#pragma unroll
-            for (int i = 0; i < L_WARPS; ++i) v += sh.reduce[i][f][t];
-            if (parts > 1) sh.cluster[f][t] = v;
-        }
-        if (parts > 1) {
-            cluster_sync_all();
-            if (rank == 0 && t < p.n_tokens)
-                for (int r = 1; r < parts; ++r) v += ld_dsmem(&sh.cluster[f][t], (uint32_t)r);
-            cluster_sync_all();
-        } else {
-            __syncthreads();
-        }
-        const int feature = group * 16 + f;
-        if (rank == 0 && t < p.n_tokens && feature < p.width) {
+        cluster_sync_all();
+        // CTA r ends the features of team r: the sums of the four CTAs' teams, in order
+        const int f = threadIdx.x & 15, t = threadIdx.x >> 4, feature = (group0 + rank) * 16 + f;
+        if (rank < teams && t < p.n_tokens && feature < p.width) {
+            float v = 0.f;
+            for (int r = 0; r < PARTS; ++r)
+#pragma unroll 4
+                for (int m = 0; m < members; ++m) v += ld_dsmem(&sh.reduce[rank * members + m][f][t], (uint32_t)r);
             const float w = sh.plan.identity[t];
             if (p.n_out > p.n_real) v += w * __bfloat162float(p.x[(long long)t * p.ldx + feature]);
             p.out[(long long)t * p.width + feature] = __float2bfloat16_rn(v);
         }
+        cluster_sync_all();
     }
 }
 
 template <int GROUPS> size_t up_smem_bytes(const LayerArgs& p) { return sizeof(UpShared<GROUPS>) + (size_t)LT * (p.n_out + 1) * 4 + (size_t)LT * (p.n_out + p.n_groups) * 4; }
 
-// Clusters of the up kernel that the device holds at once (asked for once a device): a grid that needs a second round would route twice.
-template <bool CODES, int GROUPS> int up_clusters(size_t smem, int sms) {
-    static std::atomic<int> known[64];
+// Clusters of `size` CTAs that the device holds at once, one CTA to an SM (asked for once a device): the clusters of a grid that come in a second round begin when the
+// others are done.
+template <typename... KArgs> int clusters_at_once(void (*kernel)(KArgs...), int size, size_t smem, int sms, std::atomic<int> (&known)[64]) {
     int dev = 0, n = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 1;
     if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(64 * L_CLUSTER);
+    cfg.gridDim = dim3(64 * size);
     cfg.blockDim = dim3(L_THREADS);
     cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = L_CLUSTER;
+    attr[0].val.clusterDim.x = size;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, moe_layer_up_kernel<CODES, GROUPS>, &cfg) != cudaSuccess || n < 1) n = 1;
-    if (n > sms / L_CLUSTER) n = sms / L_CLUSTER > 0 ? sms / L_CLUSTER : 1;           // (what the workspace has room for)
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) n = 1;
+    if (n > sms / size) n = sms / size > 0 ? sms / size : 1;            // (what the workspace has room for)
     if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
     return n;
 }
 
 template <bool CODES, int GROUPS> int launch_layer(const LayerArgs& p, int sms, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed_up{0}, allowed_down{0};
+    static std::atomic<int> known_up[64], known_down[64];
     static_assert(sizeof(UpShared<2>) + (size_t)LT * (L_MAX_OUT + 1) * 4 + (size_t)LT * 2 * L_MAX_OUT * 4 <= 227 * 1024, "the most router outputs and groups");
     cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES, GROUPS>, 227 * 1024, allowed_up);
-    if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES, GROUPS>, (int)sizeof(DownShared), allowed_down);
+    if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES, GROUPS>, 227 * 1024, allowed_down);
     if (e != cudaSuccess) return (int)e;
-    const int clusters = up_clusters<CODES, GROUPS>(up_smem_bytes<GROUPS>(p), sms);
-    rlis_launch_cluster(moe_layer_up_kernel<CODES, GROUPS>, dim3((unsigned)(clusters * L_CLUSTER)), dim3(L_THREADS), up_smem_bytes<GROUPS>(p), stream, dim3(L_CLUSTER, 1, 1), p);
+    const size_t up_smem = up_smem_bytes<GROUPS>(p);
+    const int up_clusters = clusters_at_once(moe_layer_up_kernel<CODES, GROUPS>, L_CLUSTER, up_smem, sms, known_up);
+    rlis_launch_cluster(moe_layer_up_kernel<CODES, GROUPS>, dim3((unsigned)(up_clusters * L_CLUSTER)), dim3(L_THREADS), up_smem, stream, dim3(L_CLUSTER, 1, 1), p);
     const int rc = RLIS_LAUNCH_CHECK();
     if (rc != 0) return rc;
+    // as many slots as the pieces of a CTA's chunks can take, up to what its shared memory holds
+    const auto share = [](int k) { return ((k + LK - 1) / LK + PARTS - 1) / PARTS; };
+    const int all = p.n_tokens * (p.top * share(p.inner) + share(p.inner_shared)), cap = all < most_slots<CODES>() ? (all + 7) / 8 * 8 : most_slots<CODES>();
     const int groups = (p.width + 15) / 16;
-    int parts = 1;
-    while (parts < 4 && groups * parts * 4 < 3 * sms) parts *= 2;
-    const int at_once = sms / parts < groups ? sms / parts : groups;
-    rlis_launch_cluster(moe_layer_down_kernel<CODES, GROUPS>, dim3((unsigned)(at_once * parts)), dim3(L_THREADS), sizeof(DownShared), stream, dim3((unsigned)parts, 1, 1), p, parts);
+    const int teams = (groups + MOST_TEAMS - 1) / MOST_TEAMS * PARTS * 4 >= 3 * sms ? MOST_TEAMS : LEAST_TEAMS;
+    const int most = clusters_at_once(moe_layer_down_kernel<CODES, GROUPS>, PARTS, down_smem_bytes<CODES>(most_slots<CODES>()), sms, known_down);
+    const int clusters = (groups + teams - 1) / teams < most ? (groups + teams - 1) / teams : most;
+    rlis_launch_cluster(moe_layer_down_kernel<CODES, GROUPS>, dim3((unsigned)(clusters * PARTS)), dim3(L_THREADS), down_smem_bytes<CODES>(cap), stream, dim3(PARTS, 1, 1), p,
+                        teams, cap);
     return RLIS_LAUNCH_CHECK();
 }
 }  // namespace
@@ -858,19 +899,16 @@ struct RlisMoeLayer {
 namespace {
 // Where a call's parts of the workspace lie; `bytes` of it in all.
 struct LayerSpace {
-    long long h, top, x, bytes;
-    int h_row, top_row, x_row;
+    long long h, x, bytes;
+    int h_row, x_row;
 };
-LayerSpace space_of(int n_tokens, int top, int width, int inner, int inner_shared, bool codes, int sms) {
+LayerSpace space_of(int n_tokens, int top, int width, int inner, int inner_shared, int sms) {
     LayerSpace s;
-    const int most = inner > inner_shared ? inner : inner_shared;
     const long long rows = (long long)n_tokens * (top + 1);
-    s.h_row = (most + LK - 1) / LK * LK;
+    s.h_row = inner > inner_shared ? inner : inner_shared;
     s.x_row = (width + LK - 1) / LK * LK + TEAM * LK;          // (a chunk more for a team's second chunks)
-    s.top_row = (s.h_row / 8 + 15) / 16 * 16;
     s.h = (sizeof(LayerPlan) + 15) / 16 * 16;
-    s.top = s.h + 4 * rows * s.h_row;
-    s.x = s.top + (codes ? rows * s.top_row : 0);
+    s.x = s.h + 4 * rows * s.h_row;
     s.bytes = s.x + (long long)(sms / L_CLUSTER + 1) * n_tokens * s.x_row * 2;
     return s;
 }
@@ -882,9 +920,9 @@ int layer_sms() {
 }  // namespace
 
 // Bytes of workspace of a call on the current device (0: a size that is not taken).
-extern "C" long long rlis_moe_layer_bytes(int n_tokens, int top, int width, int inner, int inner_shared, int codes) {
+extern "C" long long rlis_moe_layer_bytes(int n_tokens, int top, int width, int inner, int inner_shared) {
     if (n_tokens < 0 || n_tokens > LT || top < 0 || top > L_MAX_PAIRS / LT || width < 0 || inner < 0 || inner_shared < 0) return 0;
-    return space_of(n_tokens, top, width, inner, inner_shared, codes != 0, layer_sms()).bytes;
+    return space_of(n_tokens, top, width, inner, inner_shared, layer_sms()).bytes;
 }
 
 extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
@@ -940,14 +978,12 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     p.shift = a->shift;
     p.plan = static_cast<LayerPlan*>(a->workspace);
     const int sms = layer_sms();
-    const LayerSpace space = space_of(a->n_tokens, a->top, a->width, a->inner, a->inner_shared, codes, sms);
+    const LayerSpace space = space_of(a->n_tokens, a->top, a->width, a->inner, a->inner_shared, sms);
     unsigned char* work = static_cast<unsigned char*>(a->workspace);
     p.h_row = space.h_row;
-    p.top_row = space.top_row;
     p.h_hi = reinterpret_cast<bf16*>(work + space.h);
     p.h_lo = p.h_hi + (long long)a->n_tokens * (a->top + 1) * p.h_row;
     p.h = reinterpret_cast<float*>(work + space.h);
-    p.h_top = work + space.top;
     p.x_copy = reinterpret_cast<bf16*>(work + space.x);
     p.x_row = space.x_row;
     p.out = static_cast<bf16*>(a->out);

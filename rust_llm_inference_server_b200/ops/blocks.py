@@ -258,7 +258,7 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
         raise KernelError(f"moe_layer: out: expected contiguous bfloat16 {(T, W)} on {dev}")
     if T == 0:
         return out
-    work = torch.empty((lib().rlis_moe_layer_bytes(T, int(top), W, I2 // 2, S2 // 2, 1 if blocks else 0),), dtype=torch.uint8, device=dev)
+    work = torch.empty((lib().rlis_moe_layer_bytes(T, int(top), W, I2 // 2, S2 // 2),), dtype=torch.uint8, device=dev)
     call = _MoeLayer(x.data_ptr(), x.stride(0) if T > 1 else W, w_router.data_ptr(), _layer_vector(correction, n_out, dev, "correction"),
                      _layer_vector(router_bias, n_out, dev, "router_bias"), up, down, shared_up, shared_down, work.data_ptr(), out.data_ptr(), T, W, I2 // 2, S2 // 2, E,
                      int(n_identity), int(top), _SCORING[scoring], int(n_groups), int(keep), 1 if normalize else 0, 1 if shared_gate else 0, int(interleave),

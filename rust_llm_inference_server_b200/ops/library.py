@@ -115,7 +115,7 @@ SIGNATURES = {
     "rlis_stream_gemm_timeline": [I],
     "rlis_stream_gemm_timeline_read": [P, P],
     "rlis_attention_decode_last_variant": [],
-    "rlis_moe_layer_bytes": [I, I, I, I, I, I],
+    "rlis_moe_layer_bytes": [I, I, I, I, I],
     "rlis_moe_layer": [P, P],
     "rlis_quantize_rows": [P, LL, P, LL, P, I, I, I, P],
     "rlis_quantize_matrix": [P, LL, LL, P, LL, P, I, I, I, I, P],
