@@ -615,6 +615,7 @@ template <bool CODES> __host__ __device__ constexpr int slot_bytes() { return CO
 
 struct DownShared {
     float reduce[L_WARPS][16][LT + 1];
+    float sums[2][PARTS][16][LT];                           // of the CTAs' teams, for the CTA that ends their features (in turn)
     LayerPlan plan;
     int n_slots, next;                                      // of h's pieces that are in shared memory, and the first chunk whose are not
 };
@@ -622,6 +623,7 @@ struct DownShared {
 // and the first slot of a chunk.
 template <bool CODES> constexpr size_t down_smem_bytes(int cap) { return sizeof(DownShared) + (size_t)cap * (slot_bytes<CODES>() + 4 + 2 + 2); }
 template <bool CODES> constexpr int most_slots() { return (int)((227 * 1024 - sizeof(DownShared)) / (slot_bytes<CODES>() + 8)) / 8 * 8; }
+static_assert(MOST_TEAMS <= PARTS && L_THREADS == 512, "a CTA for each team's end");
 static_assert(sizeof(DownShared) % 16 == 0, "vectors of 16 bytes behind it");
 static_assert(most_slots<false>() >= LT * L_WARPS / LEAST_TEAMS * HELD, "a turn of all warps' chunks with all tokens");
 static_assert((L_MAX_PAIRS + LT) * (MOST_K / LK) <= 65536, "a piece's place in 16 bits");
@@ -719,25 +721,36 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
             }
         }
         __syncthreads();
+        // (the loads of several slots are asked for before the first is used: they come from the second-level cache)
         const int n_slots = sh.n_slots;
-#pragma unroll 4
-        for (int slot = warp; slot < n_slots; slot += L_WARPS) {
-            const int row = place[slot] / (MOST_K / LK), k0 = place[slot] % (MOST_K / LK) * LK, inner = row < p.n_tokens * p.top ? p.inner : p.inner_shared;
-            unsigned char* to = pieces + (size_t)slot * SLOT;
-            if constexpr (CODES) {
-                const int k = k0 + lane * 4;
-                const float4 v = k < inner ? *reinterpret_cast<const float4*>(p.h + (long long)row * p.h_row + k) : make_float4(0, 0, 0, 0);
-                const unsigned top = max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu),
-                                         max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu));
-                const int e = max((int)(__reduce_max_sync(0xffffffffu, top) >> 23), LEAST_EXPONENT);
-                const float scaling = scaling_of(e);
-                *reinterpret_cast<uint2*>(to + unit_of<CODES>(lane >> 1, slot) * 16 + (lane & 1) * 8) =
-                    make_uint2(pack_half(v.x * scaling, v.y * scaling), pack_half(v.z * scaling, v.w * scaling));
-                if (lane == 0) back[slot] = unscaling_of(e);
-            } else {
-                const int k = k0 + (lane & 15) * 8;
-                *reinterpret_cast<uint4*>(to + (lane >> 4) * (LK * 2) + unit_of<CODES>(lane & 15, slot) * 16) =
-                    k < inner ? *reinterpret_cast<const uint4*>((lane < 16 ? p.h_hi : p.h_lo) + (long long)row * p.h_row + k) : make_uint4(0, 0, 0, 0);
+        constexpr int AT_ONCE = 6;
+        for (int slot0 = warp; slot0 < n_slots; slot0 += AT_ONCE * L_WARPS) {
+            uint4 v[AT_ONCE];
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int slot = slot0 + i * L_WARPS, at = slot < n_slots ? place[slot] : 0;
+                const int row = at / (MOST_K / LK), inner = row < p.n_tokens * p.top ? p.inner : p.inner_shared;
+                const int k = at % (MOST_K / LK) * LK + (CODES ? lane * 4 : (lane & 15) * 8);
+                const long long from = (long long)row * p.h_row + k;
+                v[i] = make_uint4(0, 0, 0, 0);
+                if (slot < n_slots && k < inner)
+                    v[i] = CODES ? *reinterpret_cast<const uint4*>(p.h + from) : *reinterpret_cast<const uint4*>((lane < 16 ? p.h_hi : p.h_lo) + from);
+            }
+#pragma unroll
+            for (int i = 0; i < AT_ONCE; ++i) {
+                const int slot = slot0 + i * L_WARPS;
+                if (slot >= n_slots) break;
+                unsigned char* to = pieces + (size_t)slot * SLOT;
+                if constexpr (CODES) {
+                    const unsigned top = max(max(v[i].x & 0x7fffffffu, v[i].y & 0x7fffffffu), max(v[i].z & 0x7fffffffu, v[i].w & 0x7fffffffu));
+                    const int e = max((int)(__reduce_max_sync(0xffffffffu, top) >> 23), LEAST_EXPONENT);
+                    const float scaling = scaling_of(e);
+                    auto two = [&](uint32_t a, uint32_t b) { return pack_half(__uint_as_float(a) * scaling, __uint_as_float(b) * scaling); };
+                    *reinterpret_cast<uint2*>(to + unit_of<CODES>(lane >> 1, slot) * 16 + (lane & 1) * 8) = make_uint2(two(v[i].x, v[i].y), two(v[i].z, v[i].w));
+                    if (lane == 0) back[slot] = unscaling_of(e);
+                } else {
+                    *reinterpret_cast<uint4*>(to + (lane >> 4) * (LK * 2) + unit_of<CODES>(lane & 15, slot) * 16) = v[i];
+                }
             }
         }
         __syncthreads();
@@ -747,7 +760,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     int group = (blockIdx.x / PARTS) * teams + team;
 #pragma unroll
     for (int u = 0; u < HELD; ++u) load(held[u], group, member + u * members);
-    int from = 0, upto = 0;             // the chunks whose pieces are in shared memory: all of them, as a rule
+    int set = 0, from = 0, upto = 0;    // the chunks whose pieces are in shared memory: all of them, as a rule
 #pragma unroll 1
     for (int group0 = group - team; group0 < n_groups; group0 += clusters * teams, group += clusters * teams) {
         float acc[GROUPS][4] = {};
@@ -814,19 +827,26 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
             sh.reduce[warp][g + 8][n * 8 + col] = acc[n][2];
             sh.reduce[warp][g + 8][n * 8 + col + 1] = acc[n][3];
         }
-        cluster_sync_all();
-        // CTA r ends the features of team r: the sums of the four CTAs' teams, in order
-        const int f = threadIdx.x & 15, t = threadIdx.x >> 4, feature = (group0 + rank) * 16 + f;
-        if (rank < teams && t < p.n_tokens && feature < p.width) {
+        __syncthreads();
+        // CTA r ends the features of team r: every CTA adds its team's sums in order and hands them over, and CTA r adds the four.  (Two sets: a CTA writes one again
+        // after the next meeting, to which everybody comes when they have read it.)
+        const int f = threadIdx.x & 15, t = threadIdx.x >> 4 & 15;
+        for (int to = threadIdx.x >> 8; to < teams; to += 2) {
             float v = 0.f;
-            for (int r = 0; r < PARTS; ++r)
-#pragma unroll 4
-                for (int m = 0; m < members; ++m) v += ld_dsmem(&sh.reduce[rank * members + m][f][t], (uint32_t)r);
+            for (int m = 0; m < members; ++m) v += sh.reduce[to * members + m][f][t];
+            st_cluster_f32(&sh.sums[set][rank][f][t], v, (uint32_t)to);
+        }
+        cluster_sync_all();
+        const int feature = (group0 + rank) * 16 + f;
+        if (threadIdx.x < 256 && rank < teams && t < p.n_tokens && feature < p.width) {
+            float v = 0.f;
+#pragma unroll
+            for (int r = 0; r < PARTS; ++r) v += sh.sums[set][r][f][t];
             const float w = sh.plan.identity[t];
             if (p.n_out > p.n_real) v += w * __bfloat162float(p.x[(long long)t * p.ldx + feature]);
             p.out[(long long)t * p.width + feature] = __float2bfloat16_rn(v);
         }
-        cluster_sync_all();
+        set ^= 1;
     }
 }
 
