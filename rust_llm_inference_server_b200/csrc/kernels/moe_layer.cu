@@ -622,7 +622,10 @@ struct DownShared {
 // Behind it, for `cap` slots: h's pieces (128 k of a token's row), then what brings a slot's sums back, where a slot's piece lies in h (row * 128 + chunk of its k),
 // and the first slot of a chunk.
 template <bool CODES> constexpr size_t down_smem_bytes(int cap) { return sizeof(DownShared) + (size_t)cap * (slot_bytes<CODES>() + 4 + 2 + 2); }
-template <bool CODES> constexpr int most_slots() { return (int)((227 * 1024 - sizeof(DownShared)) / (slot_bytes<CODES>() + 8)) / 8 * 8; }
+// What a CTA takes of shared memory at most: the rest is the first-level cache, through which the weights on their way go (16 tokens, 50 experts of 1,408 of width 2,048
+// and a shared one, in bfloat16, whose pieces would fill it: 353, 214 and 179 us with 227, 195 and 163 KB, the pieces in one, two and two goes).
+constexpr int DOWN_SMEM = 163 * 1024;
+template <bool CODES> constexpr int most_slots() { return (int)((DOWN_SMEM - sizeof(DownShared)) / (slot_bytes<CODES>() + 8)) / 8 * 8; }
 static_assert(MOST_TEAMS <= PARTS && L_THREADS == 512, "a CTA for each team's end");
 static_assert(sizeof(DownShared) % 16 == 0, "vectors of 16 bytes behind it");
 static_assert(most_slots<false>() >= LT * L_WARPS / LEAST_TEAMS * HELD, "a turn of all warps' chunks with all tokens");
@@ -880,7 +883,7 @@ template <bool CODES, int GROUPS> int launch_layer(const LayerArgs& p, int sms, 
     static std::atomic<int> known_up[64], known_down[64];
     static_assert(sizeof(UpShared<2>) + (size_t)LT * (L_MAX_OUT + 1) * 4 + (size_t)LT * 2 * L_MAX_OUT * 4 <= 227 * 1024, "the most router outputs and groups");
     cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES, GROUPS>, 227 * 1024, allowed_up);
-    if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES, GROUPS>, 227 * 1024, allowed_down);
+    if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES, GROUPS>, DOWN_SMEM, allowed_down);
     if (e != cudaSuccess) return (int)e;
     const size_t up_smem = up_smem_bytes<GROUPS>(p);
     const int up_clusters = clusters_at_once(moe_layer_up_kernel<CODES, GROUPS>, L_CLUSTER, up_smem, sms, known_up);

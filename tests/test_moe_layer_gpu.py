@@ -106,6 +106,15 @@ def test_layers(blocks, T, W, I, E, top, S):
     assert torch.equal(call(m, top, 2.5, shared_gate=S > 0), y)             # no order that timing decides
 
 
+# more of the experts' results than shared memory holds at a time: one go of output features, and two; and experts that fill it alone
+@pytest.mark.parametrize("blocks", [False, True])
+@pytest.mark.parametrize("T,W,I,E,top,S", [(16, 64, 4096, 16, 8, 0), (16, 2304, 2048, 4, 4, 1040), (9, 48, 16384, 2, 2, 0), (16, 32, 4112, 1, 1, 8192)])
+def test_layers_in_several_goes(blocks, T, W, I, E, top, S):
+    m = make(T, W, I, E, S, blocks=blocks, scale=0.02)
+    want, size, _ = plain(m, top)
+    close(call(m, top), dict(m, x=torch.empty(1, max(W, I, S))), want, size, top)
+
+
 @pytest.mark.parametrize("blocks", [False, True])
 @pytest.mark.parametrize("how", [
     dict(scoring="softmax"), dict(scoring="softmax", normalize=True, correction=True), dict(scoring="softmax_chosen", router_bias=True), dict(normalize=True, router_bias=True),
