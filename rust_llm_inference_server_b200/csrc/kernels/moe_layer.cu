@@ -282,7 +282,10 @@ constexpr int TEAM = 4, TEAMS = L_WARPS / TEAM;             // warps that share 
 static_assert(TEAM * TEAMS <= 16, "a barrier for each team and set");
 
 template <int GROUPS> struct UpShared {
-    float reduce[TEAM][L_WARPS][16][8 * GROUPS + 1];        // the warps' sums of 16 rows (sets in turn); before that the router's
+    union {                                     // the warps' sums of 16 rows, sets in turn
+        float router[2][L_WARPS][16][8 * GROUPS + 1];
+        float reduce[TEAM][L_WARPS][16][8 + 1];
+    };
     LayerPlan plan;
     float gate[LT];
     int exponent[LT];                           // beside codes: the largest exponent of a token's row
@@ -348,7 +351,7 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUP
                 }
             }
         }
-        auto& sums = sh.reduce[tile & 1][warp];
+        auto& sums = sh.router[tile & 1][warp];
         const int col = (lane & 3) * 2;
 #pragma unroll
         for (int n = 0; n < GROUPS; ++n) {
@@ -367,7 +370,7 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUP
             if (tile * 16 + r < mine && t < p.n_tokens) {
                 float v = 0.f;
 #pragma unroll
-                for (int i = 0; i < L_WARPS; ++i) v += sh.reduce[tile & 1][i][r][t];
+                for (int i = 0; i < L_WARPS; ++i) v += sh.router[tile & 1][i][r][t];
                 for (int c = 0; c < cluster; ++c) st_cluster_f32(z + t * z_row + first + tile * 16 + r, v, (uint32_t)c);
             }
         }
