@@ -105,8 +105,22 @@ template <typename T> __device__ __forceinline__ uint2 codes8(const Eight<T>& e,
     return make_uint2(pack_codes(q), pack_codes(q + 4));
 }
 
-// Their codes, into a row that starts at a multiple of 16 bytes and has room for K rounded up to 16.
+// Their codes, into a row that starts at a multiple of 16 bytes.
 template <typename T> __device__ __forceinline__ void store8(unsigned char* row, int k, int K, const Eight<T>& e, const Coding& c) {
-    if (k < K) *reinterpret_cast<uint2*>(row + k) = codes8<T>(e, c);
+    if (k >= K) return;
+    const uint2 v = codes8<T>(e, c);
+    if (k + 8 <= K) {
+        *reinterpret_cast<uint2*>(row + k) = v;
+    } else {
+        uint32_t w = v.x;
+        row += k;
+        int left = K - k;
+        if (left >= 4) {
+            *reinterpret_cast<uint32_t*>(row) = w;
+            w = v.y, row += 4, left -= 4;
+        }
+#pragma unroll 1
+        for (; left > 0; --left, ++row, w >>= 8) *row = (unsigned char)w;
+    }
 }
 }  // namespace

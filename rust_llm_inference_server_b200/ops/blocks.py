@@ -74,13 +74,17 @@ class BlockMatrix:
     _made = classmethod(BlockRows._made.__func__)
 
 
-def _room(shape: tuple, device) -> tuple:
-    """A new tensor of codes whose rows start at multiples of 16 bytes, and the bytes from one to the next."""
-    K = shape[-1]
-    if K % 16 == 0:
-        return torch.empty(shape, dtype=CODES, device=device), K
+# A new tensor on the current device.  (torch.empty takes 2.4 us, more than a small call's kernel; what it calls at the end 0.75.)
+_empty = getattr(getattr(getattr(torch._C, "_dynamo", None), "guards", None), "_empty_strided_cuda", None)
+if _empty is None:
+    def _empty(shape, stride, dtype):
+        return torch.empty_strided(shape, stride, dtype=dtype, device="cuda")
+
+
+def _room(N: int, K: int, E=None) -> tuple:
+    """A new tensor of codes [N, K] (or [E, N, K]) whose rows start at multiples of 16 bytes, and the bytes from one to the next."""
     stride = -(-K // 16) * 16
-    return torch.empty(shape[:-1] + (stride,), dtype=CODES, device=device)[..., :K], stride
+    return (_empty((N, K), (stride, 1), CODES) if E is None else _empty((E, N, K), (N * stride, stride, 1), CODES)), stride
 
 
 _FLOATS = {torch.float32: 0, torch.bfloat16: 1}
@@ -105,9 +109,8 @@ def quantize_rows(x: torch.Tensor) -> BlockRows:
         with torch.cuda.device(x.device):
             return quantize_rows(x)
     T, K = x.shape
-    dev = x.device
-    values, stride = _room((T, K), dev)
-    scales = torch.empty((-(-K // BLOCK), T), dtype=torch.float32, device=dev)
+    values, stride = _room(T, K)
+    scales = _empty((-(-K // BLOCK), T), (T, 1), torch.float32)
     check(lib().rlis_quantize_rows(x.data_ptr(), x.stride(0), values.data_ptr(), stride, scales.data_ptr(), T, K, code, _stream()), "quantize_rows")
     _count("quantize_rows")
     return BlockRows._made(values, scales, stride)
@@ -119,12 +122,13 @@ def quantize_matrix(w: torch.Tensor) -> BlockMatrix:
     if w.get_device() != _device():
         with torch.cuda.device(w.device):
             return quantize_matrix(w)
-    shape, dev = tuple(w.shape), w.device
-    N, K = shape[-2:]
-    E = shape[0] if len(shape) == 3 else 1
-    values, stride = _room(shape, dev)
-    scales = torch.empty(shape[:-2] + (-(-N // BLOCK), -(-K // BLOCK)), dtype=torch.float32, device=dev)
-    check(lib().rlis_quantize_matrix(w.data_ptr(), w.stride(-2), w.stride(0) if len(shape) == 3 else 0, values.data_ptr(), stride, scales.data_ptr(), E, N, K, code,
+    N, K = w.shape[-2:]
+    nb, kb = -(-N // BLOCK), -(-K // BLOCK)
+    stack = w.dim() == 3
+    E = w.shape[0] if stack else 1
+    values, stride = _room(N, K, E if stack else None)
+    scales = _empty((E, nb, kb), (nb * kb, kb, 1), torch.float32) if stack else _empty((nb, kb), (kb, 1), torch.float32)
+    check(lib().rlis_quantize_matrix(w.data_ptr(), w.stride(-2), w.stride(0) if stack else 0, values.data_ptr(), stride, scales.data_ptr(), E, N, K, code,
                                      _stream()), "quantize_matrix")
     _count("quantize_matrix")
     return BlockMatrix._made(values, scales, stride)
@@ -151,10 +155,9 @@ def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> 
     if device != _device():
         with torch.cuda.device(device):
             return linear_blocks(x, w, out_dtype, early=early)
-    dev = weight.device
-    out = torch.empty((T, N), dtype=torch.bfloat16 if out_code else torch.float32, device=dev)
+    out = _empty((T, N), (N, 1), torch.bfloat16 if out_code else torch.float32)
     if plain:
-        scratch = torch.empty((T * (-(-K // 16) * 16 + 4 * -(-K // BLOCK)),), dtype=torch.uint8, device=dev)
+        scratch = _empty((T * (-(-K // 16) * 16 + 4 * -(-K // BLOCK)),), (1,), torch.uint8)
         check(lib().rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), code, scratch.data_ptr(), weight.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
                                           out_code, _stream()), "linear_blocks")
         _count("quantize_rows")
@@ -253,12 +256,12 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
         raise KernelError(f"moe_layer: expected a contiguous float32 router [{n_out + (1 if shared_gate else 0)}, {W}] on {dev}, got {w_router.dtype} {tuple(w_router.shape)}")
     n_groups, keep = groups if groups is not None else (1, 1)
     if out is None:
-        out = torch.empty((T, W), dtype=torch.bfloat16, device=dev)
+        out = _empty((T, W), (W, 1), torch.bfloat16)
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, W) or not out.is_contiguous() or out.device != dev:
         raise KernelError(f"moe_layer: out: expected contiguous bfloat16 {(T, W)} on {dev}")
     if T == 0:
         return out
-    work = torch.empty((lib().rlis_moe_layer_bytes(T, int(top), W, I2 // 2, S2 // 2),), dtype=torch.uint8, device=dev)
+    work = _empty((lib().rlis_moe_layer_bytes(T, int(top), W, I2 // 2, S2 // 2),), (1,), torch.uint8)
     call = _MoeLayer(x.data_ptr(), x.stride(0) if T > 1 else W, w_router.data_ptr(), _layer_vector(correction, n_out, dev, "correction"),
                      _layer_vector(router_bias, n_out, dev, "router_bias"), up, down, shared_up, shared_down, work.data_ptr(), out.data_ptr(), T, W, I2 // 2, S2 // 2, E,
                      int(n_identity), int(top), _SCORING[scoring], int(n_groups), int(keep), 1 if normalize else 0, 1 if shared_gate else 0, int(interleave),
