@@ -278,10 +278,10 @@ __device__ __forceinline__ void st_cluster_f32(float* local, float v, uint32_t r
 
 // ---- up --------------------------------------------------------------------------------------------------------------------------------
 
-constexpr int TEAM = 4, TEAMS = L_WARPS / TEAM;             // warps that share an item's k
-static_assert(TEAM * TEAMS <= 16, "a barrier for each team and set");
+constexpr int MOST_TEAM = 8;                                // warps that share an item's k: 4 or 8 (see launch_layer)
+static_assert(L_WARPS <= 16, "a barrier for each team and set");
 
-template <int GROUPS> struct UpShared {
+template <int GROUPS, int TEAM> struct UpShared {
     union {                                     // the warps' sums of 16 rows, sets in turn
         float router[2][L_WARPS][16][8 * GROUPS + 1];
         float reduce[TEAM][L_WARPS][16][8 + 1];
@@ -297,8 +297,8 @@ template <int GROUPS> struct UpShared {
 
 // This CTA's rows of the router against all tokens, into every CTA's z [LT][z_row].  Sixteen rows at a time; the warps share k: a warp takes 128 k of the
 // sixteen rows as three bfloat16 each.
-template <int GROUPS>
-__device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUPS>& sh, float* z, int z_row, int rank, int cluster) {
+template <int GROUPS, int TEAM>
+__device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUPS, TEAM>& sh, float* z, int z_row, int rank, int cluster) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int rows = p.n_out + p.shared_gate, per = (rows + cluster - 1) / cluster, first = rank * per, mine = max(0, min(per, rows - first));
     const int tiles = (per + 15) / 16, n_chunks = (p.width + LK - 1) / LK;
@@ -378,8 +378,8 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUP
 }
 
 // The cluster's copy of the tokens' rows, padded with zeros to x_row; beside codes as scaled float16, and their exponents in every CTA.  Eight warps a token.
-template <bool CODES, int GROUPS>
-__device__ __forceinline__ void copy_rows(const LayerArgs& p, UpShared<GROUPS>& sh, bf16* to, int rank) {
+template <bool CODES, int GROUPS, int TEAM>
+__device__ __forceinline__ void copy_rows(const LayerArgs& p, UpShared<GROUPS, TEAM>& sh, bf16* to, int rank) {
     static_assert(L_CLUSTER * 2 >= LT && L_WARPS == 16, "two tokens a CTA at the most");
     const int warp = threadIdx.x >> 5, t = rank + L_CLUSTER * (warp >> 3), i0 = threadIdx.x & 255;
     const bf16* x = p.x + (long long)min(t, p.n_tokens - 1) * p.ldx;
@@ -410,11 +410,13 @@ __device__ __forceinline__ void copy_rows(const LayerArgs& p, UpShared<GROUPS>& 
     if (CODES && i0 < L_CLUSTER) st_cluster_f32(reinterpret_cast<float*>(&sh.exponent[t]), __int_as_float(e), (uint32_t)i0);
 }
 
-template <bool CODES, int GROUPS /* of eight tokens */>
+template <bool CODES, int GROUPS /* of eight tokens */, int TEAM>
 __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerArgs p) {
     extern __shared__ __align__(16) unsigned char up_smem[];
-    UpShared<GROUPS>& sh = *reinterpret_cast<UpShared<GROUPS>*>(up_smem);
-    float* z = reinterpret_cast<float*>(up_smem + sizeof(UpShared<GROUPS>));                     // [LT][z_row]: logits, later the weights of what was chosen
+    constexpr int TEAMS = L_WARPS / TEAM;
+    using Shared = UpShared<GROUPS, TEAM>;
+    Shared& sh = *reinterpret_cast<Shared*>(up_smem);
+    float* z = reinterpret_cast<float*>(up_smem + sizeof(Shared));                     // [LT][z_row]: logits, later the weights of what was chosen
     const int z_row = p.n_out + 1;
     unsigned* keys = reinterpret_cast<unsigned*>(z + LT * z_row);                        // [LT][n_out + n_groups]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
@@ -424,9 +426,9 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
         sh.choice[e] = 0ull;
     }
     pdl_wait();
-    router_logits<GROUPS>(p, sh, z, z_row, blockIdx.x % L_CLUSTER, L_CLUSTER);
+    router_logits(p, sh, z, z_row, blockIdx.x % L_CLUSTER, L_CLUSTER);
     bf16* x_copy = p.x_copy + (long long)(blockIdx.x / L_CLUSTER) * p.n_tokens * p.x_row;
-    copy_rows<CODES, GROUPS>(p, sh, x_copy, blockIdx.x % L_CLUSTER);
+    copy_rows<CODES>(p, sh, x_copy, blockIdx.x % L_CLUSTER);
     cluster_sync_all();
 
     if (warp < p.n_tokens) {
@@ -856,7 +858,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     }
 }
 
-template <int GROUPS> size_t up_smem_bytes(const LayerArgs& p) { return sizeof(UpShared<GROUPS>) + (size_t)LT * (p.n_out + 1) * 4 + (size_t)LT * (p.n_out + p.n_groups) * 4; }
+template <int GROUPS, int TEAM> size_t up_smem_bytes(const LayerArgs& p) { return sizeof(UpShared<GROUPS, TEAM>) + (size_t)LT * (p.n_out + 1) * 4 + (size_t)LT * (p.n_out + p.n_groups) * 4; }
 
 // Clusters of `size` CTAs that the device holds at once, one CTA to an SM (asked for once a device): the clusters of a grid that come in a second round begin when the
 // others are done.
@@ -881,16 +883,16 @@ template <typename... KArgs> int clusters_at_once(void (*kernel)(KArgs...), int 
     return n;
 }
 
-template <bool CODES, int GROUPS> int launch_layer(const LayerArgs& p, int sms, cudaStream_t stream) {
+template <bool CODES, int GROUPS, int TEAM> int launch_layer(const LayerArgs& p, int sms, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed_up{0}, allowed_down{0};
     static std::atomic<int> known_up[64], known_down[64];
-    static_assert(sizeof(UpShared<2>) + (size_t)LT * (L_MAX_OUT + 1) * 4 + (size_t)LT * 2 * L_MAX_OUT * 4 <= 227 * 1024, "the most router outputs and groups");
-    cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES, GROUPS>, 227 * 1024, allowed_up);
+    static_assert(sizeof(UpShared<GROUPS, TEAM>) + (size_t)LT * (L_MAX_OUT + 1) * 4 + (size_t)LT * 2 * L_MAX_OUT * 4 <= 227 * 1024, "the most router outputs and groups");
+    cudaError_t e = rlis_allow_smem(moe_layer_up_kernel<CODES, GROUPS, TEAM>, 227 * 1024, allowed_up);
     if (e == cudaSuccess) e = rlis_allow_smem(moe_layer_down_kernel<CODES, GROUPS>, DOWN_SMEM, allowed_down);
     if (e != cudaSuccess) return (int)e;
-    const size_t up_smem = up_smem_bytes<GROUPS>(p);
-    const int up_clusters = clusters_at_once(moe_layer_up_kernel<CODES, GROUPS>, L_CLUSTER, up_smem, sms, known_up);
-    rlis_launch_cluster(moe_layer_up_kernel<CODES, GROUPS>, dim3((unsigned)(up_clusters * L_CLUSTER)), dim3(L_THREADS), up_smem, stream, dim3(L_CLUSTER, 1, 1), p);
+    const size_t up_smem = up_smem_bytes<GROUPS, TEAM>(p);
+    const int up_clusters = clusters_at_once(moe_layer_up_kernel<CODES, GROUPS, TEAM>, L_CLUSTER, up_smem, sms, known_up);
+    rlis_launch_cluster(moe_layer_up_kernel<CODES, GROUPS, TEAM>, dim3((unsigned)(up_clusters * L_CLUSTER)), dim3(L_THREADS), up_smem, stream, dim3(L_CLUSTER, 1, 1), p);
     const int rc = RLIS_LAUNCH_CHECK();
     if (rc != 0) return rc;
     // as many slots as the pieces of a CTA's chunks can take, up to what its shared memory holds
@@ -932,7 +934,7 @@ LayerSpace space_of(int n_tokens, int top, int width, int inner, int inner_share
     LayerSpace s;
     const long long rows = (long long)n_tokens * (top + 1);
     s.h_row = inner > inner_shared ? inner : inner_shared;
-    s.x_row = (width + LK - 1) / LK * LK + TEAM * LK;          // (a chunk more for a team's second chunks)
+    s.x_row = (width + LK - 1) / LK * LK + MOST_TEAM * LK;     // (a chunk more for a team's second chunks)
     s.h = (sizeof(LayerPlan) + 15) / 16 * 16;
     s.x = s.h + 4 * rows * s.h_row;
     s.bytes = s.x + (long long)(sms / L_CLUSTER + 1) * n_tokens * s.x_row * 2;
@@ -1016,6 +1018,11 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
     auto magic = [](int d) { return d > 1 ? (unsigned)(((1ull << 32) + d - 1) / d) : 0u; };
     p.per_expert_magic = magic(a->inner / 8);
     p.own_chunks_magic = magic((a->inner + LK - 1) / LK);
-    if (p.n_tokens <= 8) return codes ? launch_layer<true, 1>(p, sms, stream) : launch_layer<false, 1>(p, sms, stream);
-    return codes ? launch_layer<true, 2>(p, sms, stream) : launch_layer<false, 2>(p, sms, stream);
+    // Where teams of four warps would take two items each at the most, many would take one while others take two: teams of eight take twice as many half as long ones,
+    // as long as a warp has two chunks of each (one token, 4 of 32 experts of 1,024 of width 2,048 and a shared one: 25.5 -> 24.2 us, in blocks 21.3 -> 20.8; 8 tokens, 22
+    // experts: 63.6 -> 62.8, but in blocks 46.4 -> 50.1).
+    const int items = (p.n_tokens * p.top * p.inner + p.inner_shared) / 8, teams = sms / L_CLUSTER * L_CLUSTER * (L_WARPS / 4);
+    if (p.n_tokens <= 8 && items <= 2 * teams && p.width > 15 * LK) return codes ? launch_layer<true, 1, 8>(p, sms, stream) : launch_layer<false, 1, 8>(p, sms, stream);
+    if (p.n_tokens <= 8) return codes ? launch_layer<true, 1, 4>(p, sms, stream) : launch_layer<false, 1, 4>(p, sms, stream);
+    return codes ? launch_layer<true, 2, 4>(p, sms, stream) : launch_layer<false, 2, 4>(p, sms, stream);
 }

@@ -95,7 +95,7 @@ def close(y, m, want, size, top):
 # one token, the edge of the first eight columns and of the tokens; widths that end inside a chunk and a warp's turn; experts fewer than a cluster's CTAs and more than
 # eight for each; one feature group and a few
 @pytest.mark.parametrize("blocks", [False, True])
-@pytest.mark.parametrize("T,W,I,E,top,S", [(1, 16, 16, 1, 1, 0), (1, 256, 128, 8, 2, 0), (3, 272, 48, 5, 5, 32), (8, 512, 256, 32, 4, 256), (9, 128, 64, 40, 3, 0),
+@pytest.mark.parametrize("T,W,I,E,top,S", [(1, 16, 16, 1, 1, 0), (1, 2048, 128, 6, 2, 64), (3, 2064, 48, 5, 2, 0), (8, 1936, 16, 8, 4, 16), (1, 256, 128, 8, 2, 0), (3, 272, 48, 5, 5, 32), (8, 512, 256, 32, 4, 256), (9, 128, 64, 40, 3, 0),
                                            (16, 384, 96, 70, 8, 160), (16, 2304, 32, 3, 2, 16), (7, 4112, 16, 9, 1, 0), (2, 1024, 144, 512, 16, 0)])
 def test_layers(blocks, T, W, I, E, top, S):
     m = make(T, W, I, E, S, gate=S > 0, blocks=blocks)
