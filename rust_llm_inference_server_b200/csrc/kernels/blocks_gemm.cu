@@ -14,6 +14,11 @@
 // epilogues; warps 4-11 are the epilogue, a quarter of the rows and half of the columns each, and tell CTA 0 when they have read an accumulator.
 // Few rows: blocks_few.cuh.
 //
+// What bounds it (2,048 x 16,384 of K 2048, 63.3 us, 2,172 TFLOP/s; the nominal e4m3 rate would be 31): the tiles' way from the second-level cache (what is left without
+// products and sums takes 44 us, in tiles of 128 columns 73, 11 TB/s), the epilogue's sums (55 without them) and the products (55 with a quarter of them) are of one
+// size, and none hides the others whole.  (The hand-over of an accumulator by an arrive that releases waited for the loads of scales on their way, 1,050 to 1,300
+// cycles a block: 132 us; the widths of loads from tensor memory make no difference.)
+//
 // Every mbarrier wait is bounded (tcgen05_utils.cuh); a wait that runs out sets the error word, every role runs to its end without further waits, the CTAs
 // meet and free their tensor memory.
 #include "blocks.cuh"
@@ -470,12 +475,28 @@ extern "C" int rlis_blocks_gemm(const void* x, long long ldx, const float* sx, c
 
 extern "C" int rlis_quantize_rows(const void* x, long long ldx, void* codes, long long ldc, float* scales, int n_tokens, int K, int dtype, cudaStream_t stream);
 
-// The same for plain rows x [M, K] of `dtype` (ldx elements apart): rlis_quantize_rows and the product.  scratch: M * ceil(K / 16) * 16 bytes of codes and behind them
-// M * ceil(K / 128) floats, 16-byte aligned.  (The first kernel lets the second start once all kernels before itself have finished; none but itself is in
-// flight then, and it does not write w: w's first tiles are always read early.)
+// The bytes of scratch that rlis_blocks_gemm_rows wants on the current device: 0 where the product puts the rows into blocks itself.
+extern "C" long long rlis_blocks_gemm_scratch(int M, int N, int K) {
+    if (M <= 0 || N <= 0 || K <= 0 || plain_rows_fit(M, N, K, sms_of_device())) return 0;
+    return M * ((K + 15LL) / 16 * 16 + 4LL * ((K + QB - 1) / QB));
+}
+
+// The same for plain rows x [M, K] of `dtype` (ldx elements apart), which the product puts into blocks itself or rlis_quantize_rows before it.  scratch: 16-byte aligned,
+// M * ceil(K / 16) * 16 bytes of codes and behind them M * ceil(K / 128) floats.  (Of two kernels the first lets the second start once all kernels before itself have
+// finished; none but itself is in flight then, and it does not write w: w's first tiles are always read early.)
 extern "C" int rlis_blocks_gemm_rows(const void* x, long long ldx, int dtype, void* scratch, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K,
                                      int out_dtype, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
+    if (K <= 0) return RLIS_ERR_UNSUPPORTED;
+    const int sms = sms_of_device();
+    if (plain_rows_fit(M, N, K, sms)) {
+        if ((dtype != RLIS_F32 && dtype != RLIS_BF16) || (out_dtype != RLIS_F32 && out_dtype != RLIS_BF16) || !codes_fit(w, ldw, K)) return RLIS_ERR_UNSUPPORTED;
+#define RLIS_BP(T) (out_dtype == RLIS_F32 ? launch_blocks_few_plain<T, float>(x, ldx, w, ldw, sw, y, M, N, K, sms, stream) \
+                                          : launch_blocks_few_plain<T, bf16>(x, ldx, w, ldw, sw, y, M, N, K, sms, stream))
+        return dtype == RLIS_F32 ? RLIS_BP(float) : RLIS_BP(bf16);
+#undef RLIS_BP
+    }
+    if (scratch == nullptr) return RLIS_ERR_UNSUPPORTED;
     const long long ldc = (K + 15LL) / 16 * 16;
     float* sx = reinterpret_cast<float*>(static_cast<unsigned char*>(scratch) + M * ldc);
     const int e = rlis_quantize_rows(x, ldx, scratch, ldc, sx, M, K, dtype, stream);

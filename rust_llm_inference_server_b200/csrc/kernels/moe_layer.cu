@@ -4,25 +4,31 @@
 //         h[t, s, :] = gate[t] glu(..) of the shared expert
 //   down: out[t, :] = sum over e of W_down_e h[t, e, :] (+ W_down_s h[t, s, :]) + sum of the weights of t's identity experts * x_t
 //
-// With so few tokens the layer is a stream of the chosen experts' weights from memory (8 tokens, 4 of 32 experts of 2,048 x 1,024 and a shared one: 278 MB, 42 us
-// at the rate of a copy).  So every weight is read once, by 16-byte loads of 16 rows side by side straight into the registers of mma.sync m16n8k16, no
-// shared memory between: a sum over k may take k in any order, so a thread's 16 bytes of a row, eight neighbouring k, serve as its k slots of two
-// instructions, and the tokens' rows, which stay in the caches, are read in the same order.  A warp takes 128 k of 16 rows at a time (a chunk, a block's edge; for
-// weights in e4m3 blocks a chunk's sums are scaled before they join the others) and has the next chunks, of the next rows if need be, on their way while it
-// works on one.  Four warps (up) or a CTA's sixteen (down) take different k of the same rows and add their sums in shared memory in the order of the
-// warps, so results do not depend on timing.  (Chunks by asynchronous copies through 180 KB of shared memory: 65 -> 99 us for the layer above; the first-level
-// cache that is left holds no tokens' rows.)
+// With so few tokens the layer is a stream of the chosen experts' weights from memory (8 tokens, 4 of 32 experts of 2,048 x 1,024 and a shared one: 290 MB, 44 us
+// at the rate of a copy; the two kernels take 63).  So every weight is read once, by 16-byte loads of 16 rows side by side straight into the registers of mma.sync
+// m16n8k16, no shared memory between: a sum over k may take k in any order, so a thread's 16 bytes of a row, eight neighbouring k, serve as its k slots of two
+// instructions, and the tokens' rows are read in the same order.  A warp takes 128 k of 16 rows at a time (a chunk, a block's edge; for weights in e4m3 blocks a
+// chunk's sums are scaled before they join the others) and has the next chunks, of the next rows if need be, on their way while it works on one.  The warps of a
+// team take different k of the same rows and add their sums in shared memory in the order of the warps, so results do not depend on timing.  In flight the loads
+// take room in the first-level cache, which is what shared memory leaves: chunks by asynchronous copies through 180 KB of shared memory took 99 us for 65, and the
+// down kernel with 227 KB instead of 163 353 for 179.
 //
 // Routing sits in the up kernel: the CTAs of a cluster share the router's rows, hand each other the logits (distributed shared memory), and each chooses
-// for all tokens itself: no launch of its own, no grid-wide barrier, no workspace but h and the plan, which the first CTA leaves for the down kernel.  The
-// router's float32 rows go through the same instructions as three bfloat16 numbers each, whose sum they are to 2^-24 (a token's logits are sums of exact
-// products in float32, as a chain of FMAs would give them; as FMAs, 128 rows against 16 tokens took 20 us).
+// for all tokens itself: no launch of its own, no grid-wide barrier, no workspace but h, the plan, which the first CTA leaves for the down kernel, and a copy of
+// the tokens' rows for each cluster, which the caches hold.  The router's float32 rows go through the same instructions as three bfloat16 numbers each, whose sum
+// they are to 2^-24 (a token's logits are sums of exact products in float32, as a chain of FMAs would give them; as FMAs, 128 rows against 16 tokens took 20 us).
 //
 // The weights of the choice are multiplied into h in float32; the down product is then one long sum over the chosen experts' k, with the step's tokens as columns
-// whoever chose them.  Nothing but the result is rounded to the activations' type: beside bfloat16 weights h is two bfloat16 numbers (their sum is h to 2^-17).
-// Codes become float16 by one instruction a pair (as bfloat16, which has none, a word of four took 10 cycles of a scheduler instead of 5, and the products waited
-// for it), so the tokens' rows and h's meet them as float16 of eleven bits, each row times the power of two that brings its largest value to 2^14 .. 2^15: x is
-// that exactly down to 2^-31 of the largest, h to 2^-11 of every value, an eighth of what the result is rounded by.
+// whoever chose them.  Its CTAs bring the pieces of h that their chunks meet into shared memory first (read from the second-level cache chunk by chunk they took
+// more of the load units than the weights: 16 tokens, 83 of 128 experts of 768 in blocks 135 us, 111 so).  Nothing but the result is rounded to the activations'
+// type: beside bfloat16 weights h is two bfloat16 numbers (their sum is h to 2^-17).  Codes become float16 by one instruction a pair (as bfloat16, which has none,
+// a word of four took 10 cycles of a scheduler instead of 5, and the products waited for it), so the tokens' rows and h's meet them as float16 of eleven bits, each
+// row (of h each piece of 128) times the power of two that brings its largest value to 2^14 .. 2^15: x is that exactly down to 2^-31 of the largest, h to 2^-11 of
+// every value, an eighth of what the result is rounded by.
+//
+// What bounds it: memory in the two loops (8 tokens in bfloat16: 6.8 TB/s), and what comes before and between them, when memory is idle: 8 us from the launch
+// to the first expert's weights (the router's rows, the meeting of the cluster, the choice), 4 from the first CTA's last item to the down kernel's plan, 4 to its first
+// product, 2 for the last sums.
 #include "common.cuh"
 #include "mma_utils.cuh"
 #include <cuda_fp16.h>

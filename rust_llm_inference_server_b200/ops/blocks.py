@@ -157,10 +157,13 @@ def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> 
             return linear_blocks(x, w, out_dtype, early=early)
     out = _empty((T, N), (N, 1), torch.bfloat16 if out_code else torch.float32)
     if plain:
-        scratch = _empty((T * (-(-K // 16) * 16 + 4 * -(-K // BLOCK)),), (1,), torch.uint8)
-        check(lib().rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), code, scratch.data_ptr(), weight.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
+        kernels = lib()
+        room = kernels.rlis_blocks_gemm_scratch(T, N, K)
+        scratch = _empty((room,), (1,), torch.uint8) if room else None
+        check(kernels.rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), code, scratch.data_ptr() if room else None, weight.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
                                           out_code, _stream()), "linear_blocks")
-        _count("quantize_rows")
+        if room:
+            _count("quantize_rows")
     else:
         check(lib().rlis_blocks_gemm(x.values.data_ptr(), x.stride, x.scales.data_ptr(), weight.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
                                      out_code, int(early), _stream()), "linear_blocks")

@@ -119,6 +119,7 @@ SIGNATURES = {
     "rlis_moe_layer": [P, P],
     "rlis_quantize_rows": [P, LL, P, LL, P, I, I, I, P],
     "rlis_quantize_matrix": [P, LL, LL, P, LL, P, I, I, I, I, P],
+    "rlis_blocks_gemm_scratch": [I, I, I],
     "rlis_blocks_gemm_rows": [P, LL, I, P, P, LL, P, P, I, I, I, I, P],
     "rlis_blocks_gemm": [P, LL, P, P, LL, P, P, I, I, I, I, I, P],
 }
@@ -166,7 +167,7 @@ def lib():
             fn = getattr(handle, name)
             fn.argtypes = []
             fn.restype = c_int
-        handle.rlis_moe_layer_bytes.restype = LL
+        handle.rlis_moe_layer_bytes.restype = handle.rlis_blocks_gemm_scratch.restype = LL
         handle.rlis_debug_set.argtypes = [ctypes.c_char_p, c_int]
         handle.rlis_debug_set.restype = c_int
         _lib = handle

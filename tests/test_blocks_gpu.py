@@ -109,6 +109,7 @@ def close(y, r, m, out_dtype):
 
 SIZES = [(1, 1, 1), (1, 128, 128), (3, 40, 130), (8, 2048, 2048), (8, 1000, 4100), (16, 130, 1000), (17, 300, 513), (33, 257, 384), (64, 4096, 256), (65, 128, 1280), (100, 1, 700),
          (128, 640, 1024), (129, 255, 128), (200, 384, 129), (257, 513, 2048), (300, 2056, 640), (1, 20000, 256), (1000, 7, 64), (513, 1024, 15),
+         (2, 2000, 300), (16, 2048, 2048), (16, 700, 1400), (4, 18000, 2000), (1, 300, 8000), (1, 37000, 300), (15, 260, 90),          # put into blocks by the product
          (129, 300, 3000), (130, 4100, 4100), (2000, 257, 2500), (256, 1, 1700)]          # k in shares: 3, 2, 3 and, of 14 blocks, none
 
 
