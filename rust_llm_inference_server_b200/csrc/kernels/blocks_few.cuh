@@ -11,7 +11,7 @@
 // after a cluster barrier CTA r adds the rows r, r + splits, .. of all CTAs in the order of the splits: the result does not depend on timing.  The number of
 // splits depends on N and K alone up to 64 rows (few_splits), so a row has the same bits whatever other rows there are.
 // 8 rows x 16,384 of K 2048 from rows in blocks 8.3 us (4.0 TB/s; plain rows, put into blocks by the product, 10.3), 64 x 4,096 of K 14336
-// 17.5, one row x 2,048 of K 2048 3.4 (plain 3.9): a launch, the first tiles' way from memory and the cluster's meeting before anything else.
+// 15.9, one row x 2,048 of K 2048 3.4 (plain 3.9): a launch, the first tiles' way from memory and the cluster's meeting before anything else.
 // (Included by blocks_gemm.cu, whose error word it shares.)
 #pragma once
 
@@ -261,10 +261,12 @@ template <int NT> int few_splits(int tiles, int k_blocks, int sms) {
     const int most = k_blocks / 2;
     return s < most ? s : most < 1 ? 1 : most;
 }
-// Stages of the ring: six for a CTA that has an SM to itself; four so that two CTAs fit, for clusters and where there are more CTAs than SMs; and as few as keep
-// tensor memory enough for many CTAs an SM where there are several for each (128,256 features of K 2048: 40.2, 41.4 and 45.2 us with 2, 4 and 6).
+// Stages of the ring: six for a CTA that has an SM to itself, which clusters of four find for nine tenths of the SMs (64 x 4,096 of K 14336, 128 CTAs: 15.9 us for 16.6 with
+// four, plain rows 19.7 for 24.2, since two CTAs on an SM while others wait for the launch before is what four allow); four so that two CTAs fit, for larger clusters and
+// where there are more CTAs than SMs; and as few as keep tensor memory enough for many CTAs an SM where there are several for each (128,256 features of K 2048: 40.2, 41.4
+// and 45.2 us with 2, 4 and 6).
 template <int NT> int few_stages(int tiles, int splits, int sms) {
-    if (NT == 128 || (splits == 1 && tiles <= sms)) return 6;
+    if (NT == 128 || (splits == 1 && tiles <= sms) || (splits > 1 && splits <= 4 && 10 * tiles * splits <= 9 * sms)) return 6;
     return splits > 1 || tiles <= 4 * sms || NT == 64 ? 4 : NT == 16 ? 2 : 3;
 }
 
