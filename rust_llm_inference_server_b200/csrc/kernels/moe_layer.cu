@@ -194,18 +194,18 @@ __device__ __forceinline__ unsigned order_of(float v) {
 __device__ __forceinline__ float logistic(float z) { return 1.0f / (1.0f + expf(-z)); }
 
 // One warp chooses for one token: z [n_out] logits in, scores out; `key` [n_out + n_groups] is scratch.  Lane k ends with choice k and its weight.
-__device__ __forceinline__ void choose(const LayerArgs& p, float* z, unsigned* key, int lane, int& chosen, float& weight) {
+__device__ __forceinline__ void choose(const LayerArgs& p, const float* correction, const float* bias, float* z, unsigned* key, int lane, int& chosen, float& weight) {
     const int n = p.n_out;
     float mx = -INFINITY;
     if (p.scoring == 2) {
 #pragma unroll 1
-        for (int e = lane; e < n; e += 32) mx = fmaxf(mx, z[e] + (p.router_bias != nullptr ? p.router_bias[e] : 0.f));
+        for (int e = lane; e < n; e += 32) mx = fmaxf(mx, z[e] + bias[e]);
         mx = warp_max(mx);
     }
     float sum = 0.f;
 #pragma unroll 1
     for (int e = lane; e < n; e += 32) {
-        float v = z[e] + (p.router_bias != nullptr ? p.router_bias[e] : 0.f);
+        float v = z[e] + bias[e];
         if (p.scoring != 1) v = expf(p.scoring == 2 ? v - mx : -v);
         if (p.scoring == 0) v = 1.0f / (1.0f + v);
         sum += v;
@@ -216,7 +216,7 @@ __device__ __forceinline__ void choose(const LayerArgs& p, float* z, unsigned* k
     for (int e = lane; e < n; e += 32) {
         const float v = p.scoring == 2 ? z[e] / sum : z[e];
         z[e] = v;
-        key[e] = order_of(v + (p.correction != nullptr ? p.correction[e] : 0.f));
+        key[e] = order_of(v + correction[e]);
     }
     __syncwarp();
     if (p.n_groups > 1) {
@@ -298,6 +298,7 @@ template <int GROUPS, int TEAM> struct UpShared {
     unsigned top[L_WARPS];
     unsigned long long choice[L_MAX_OUT];       // which of a token's choices an expert is, four bits a token
     unsigned tokens[L_MAX_OUT];                 // the tokens that chose an expert
+    float correction[L_MAX_OUT], bias[L_MAX_OUT];       // of the outputs (zeros where there are none): on their way with the router's rows
     unsigned short work[2 * L_MAX_PAIRS];       // active experts, with SECOND set for those after the first eight of an expert's tokens
 };
 
@@ -385,7 +386,7 @@ __device__ __forceinline__ void router_logits(const LayerArgs& p, UpShared<GROUP
 
 // The cluster's copy of the tokens' rows, padded with zeros to x_row; beside codes as scaled float16, and their exponents in every CTA.  Eight warps a token.
 template <bool CODES, int GROUPS, int TEAM>
-__device__ __forceinline__ void copy_rows(const LayerArgs& p, UpShared<GROUPS, TEAM>& sh, bf16* to, int rank) {
+__device__ __forceinline__ void copy_rows(const LayerArgs& p, UpShared<GROUPS, TEAM>& sh, bf16* to, int rank, const uint4 head) {
     static_assert(L_CLUSTER * 2 >= LT && L_WARPS == 16, "two tokens a CTA at the most");
     const int warp = threadIdx.x >> 5, t = rank + L_CLUSTER * (warp >> 3), i0 = threadIdx.x & 255;
     const bf16* x = p.x + (long long)min(t, p.n_tokens - 1) * p.ldx;
@@ -393,7 +394,7 @@ __device__ __forceinline__ void copy_rows(const LayerArgs& p, UpShared<GROUPS, T
     if (CODES) {
         unsigned m = 0u;
         for (int k = i0 * 8; k < p.width; k += 2048) {
-            const uint4 v = *reinterpret_cast<const uint4*>(x + k);
+            const uint4 v = k == i0 * 8 ? head : *reinterpret_cast<const uint4*>(x + k);
             m = __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)), __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
         }
         m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
@@ -406,7 +407,7 @@ __device__ __forceinline__ void copy_rows(const LayerArgs& p, UpShared<GROUPS, T
     const float scaling = scaling_of(e);
 #pragma unroll 1
     for (int k = i0 * 8; k < p.x_row; k += 2048) {
-        uint4 v = k < p.width ? *reinterpret_cast<const uint4*>(x + k) : make_uint4(0, 0, 0, 0);
+        uint4 v = k == i0 * 8 ? head : k < p.width ? *reinterpret_cast<const uint4*>(x + k) : make_uint4(0, 0, 0, 0);
         if (CODES) {
             auto two = [&](uint32_t w) { return pack_half(__uint_as_float(w << 16) * scaling, __uint_as_float(w & 0xffff0000u) * scaling); };
             v = make_uint4(two(v.x), two(v.y), two(v.z), two(v.w));
@@ -432,15 +433,22 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
         sh.choice[e] = 0ull;
     }
     pdl_wait();
+    for (int e = threadIdx.x; e < p.n_out; e += L_THREADS) {
+        sh.correction[e] = p.correction != nullptr ? p.correction[e] : 0.f;
+        sh.bias[e] = p.router_bias != nullptr ? p.router_bias[e] : 0.f;
+    }
+    // (the first of this thread's vectors of the tokens' rows that copy_rows copies: on its way meanwhile)
+    const int copied = min((int)(blockIdx.x % L_CLUSTER) + L_CLUSTER * (warp >> 3), p.n_tokens - 1), head_k = (threadIdx.x & 255) * 8;
+    const uint4 head = head_k < p.width ? *reinterpret_cast<const uint4*>(p.x + copied * p.ldx + head_k) : make_uint4(0, 0, 0, 0);
     router_logits(p, sh, z, z_row, blockIdx.x % L_CLUSTER, L_CLUSTER);
     bf16* x_copy = p.x_copy + (long long)(blockIdx.x / L_CLUSTER) * p.n_tokens * p.x_row;
-    copy_rows<CODES>(p, sh, x_copy, blockIdx.x % L_CLUSTER);
+    copy_rows<CODES>(p, sh, x_copy, blockIdx.x % L_CLUSTER, head);
     cluster_sync_all();
 
     if (warp < p.n_tokens) {
         int e;
         float w;
-        choose(p, z + warp * z_row, keys + warp * (p.n_out + p.n_groups), lane, e, w);
+        choose(p, sh.correction, sh.bias, z + warp * z_row, keys + warp * (p.n_out + p.n_groups), lane, e, w);
         const bool have = lane < p.top, real = have && e < p.n_real;
         const float identity = warp_sum(have && !real ? w : 0.f);
         if (real) {
