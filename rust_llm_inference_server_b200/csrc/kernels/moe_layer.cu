@@ -670,15 +670,9 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
     const int rank = blockIdx.x % PARTS, n_groups = (p.width + 15) / 16, clusters = gridDim.x / PARTS;
     const int members = L_WARPS / teams, team = warp / members, member = warp % members;
-    pdl_wait();
-    // (as much of the plan as the step can have: its length comes with it)
-    const int words = (int)(offsetof(LayerPlan, of) + (size_t)min(p.n_tokens * p.top, p.n_real) * sizeof(ActiveExpert)) / 8;
-    for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(&sh.plan)[i] = reinterpret_cast<const unsigned long long*>(p.plan)[i];
-    __syncthreads();
-    pdl_trigger();
-    // this CTA's chunks: number i is chunk rank + PARTS * i of all
-    const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK, all_chunks = shared_chunks + sh.plan.n_active * own_chunks;
-    const int n_chunks = (all_chunks - rank + PARTS - 1) / PARTS;
+    // this CTA's chunks: number i is chunk rank + PARTS * i of all, those of the shared expert first (until the plan is known, all)
+    const int own_chunks = (p.inner + LK - 1) / LK, shared_chunks = (p.inner_shared + LK - 1) / LK;
+    int n_chunks = (shared_chunks - rank + PARTS - 1) / PARTS;
     struct Place {              // a chunk: which active expert's (or the shared one's), and where in its k
         bool own;
         int a, kb;
@@ -780,8 +774,23 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
 
     Chunk<CODES> held[HELD];
     int group = (blockIdx.x / PARTS) * teams + team;
+    // The first chunks: those of the shared expert before the up kernel has finished (its CTAs have waited for what came before, so nobody writes a weight any more),
+    // the others when the plan is there.
+#pragma unroll 1
+    for (int known = 0, planned = 0;; planned = 1) {
 #pragma unroll
-    for (int u = 0; u < HELD; ++u) load(held[u], group, member + u * members);
+        for (int u = 0; u < HELD; ++u)
+            if (member + u * members >= known) load(held[u], group, member + u * members);
+        if (planned) break;
+        pdl_wait();
+        // (as much of the plan as the step can have: its length comes with it)
+        const int words = (int)(offsetof(LayerPlan, of) + (size_t)min(p.n_tokens * p.top, p.n_real) * sizeof(ActiveExpert)) / 8;
+        for (int i = threadIdx.x; i < words; i += L_THREADS) reinterpret_cast<unsigned long long*>(&sh.plan)[i] = reinterpret_cast<const unsigned long long*>(p.plan)[i];
+        __syncthreads();
+        pdl_trigger();
+        known = n_chunks;
+        n_chunks = (shared_chunks + sh.plan.n_active * own_chunks - rank + PARTS - 1) / PARTS;
+    }
     int set = 0, from = 0, upto = 0;    // the chunks whose pieces are in shared memory: all of them, as a rule
 #pragma unroll 1
     for (int group0 = group - team; group0 < n_groups; group0 += clusters * teams, group += clusters * teams) {

@@ -116,6 +116,22 @@ def test_a_weight_written_right_before_its_product():
             assert torch.equal(ops.linear_blocks(ops.quantize_rows(x), made), want)
 
 
+@pytest.mark.parametrize("blocks", [False, True])
+def test_experts_written_right_before_their_layer(blocks):
+    from rust_llm_inference_server_b200 import ops
+    T, W, I, E, S = 6, 1024, 256, 8, 512
+    x, router = rand(T, W), rand(E, W, scale=0.1, dtype=torch.float32)
+    plain = [rand(*s, scale=s[-1] ** -0.5) for s in ((E, 2 * I, W), (E, W, I), (2 * S, W), (W, S))]
+    make = lambda: [ops.quantize_matrix(w) if blocks else w.clone() for w in plain]
+    call = lambda up, down, a, b: ops.moe_layer(x, router, up, down, 2, shared=(a, b))
+    want = call(*make())
+    torch.cuda.synchronize()
+    for _ in range(20):
+        assert torch.equal(call(*make()), want)
+        made = make()[::-1]                                 # the last written is the first used
+        assert torch.equal(call(*made[::-1]), want)
+
+
 def test_tensors_without_rows():
     from rust_llm_inference_server_b200 import ops
     none = ops.quantize_matrix(rand(0, 96))
