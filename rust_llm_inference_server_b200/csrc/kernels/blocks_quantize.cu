@@ -1,6 +1,6 @@
 // Values into e4m3 with a float32 scale for each block (blocks.cuh says how): 128 of a row (activations), or 128 x 128 of a matrix (weights).
-// Both kernels read their input once and keep it in registers while the block's largest value is found.  2,048 rows of 14,336 (bfloat16): 20.8 us, 4.2 TB/s, nearly
-// bound by instructions (see blocks.cuh); a matrix of 16,384 x 2,048 32.4 us in float32 (5.2 TB/s), 20.3 in bfloat16; eight rows of 2,048 2.3 us, a launch.
+// Both kernels read their input once and keep it in registers while the block's largest value is found.  2,048 rows of 14,336 (bfloat16): 16.6 us, 5.3 TB/s, where
+// instructions still count beside memory (see blocks.cuh); a matrix of 16,384 x 2,048 31.2 us in float32 (5.4 TB/s), 19.5 in bfloat16; 64 rows of 4,096 1.9 us, a launch.
 #include "blocks.cuh"
 
 namespace {
@@ -25,15 +25,27 @@ __global__ __launch_bounds__(ROWS_THREADS) void quantize_rows_kernel(const T* __
         kb[u] = unit - r * k_blocks;
         v[u] = row[u] >= 0 ? load8<T, VEC>(x + row[u] * ldx, kb[u] * QB + lane * 8, K) : nothing8<T>();
     }
+    // a lane divides for one of the blocks, and the others take it over (all dividing for all: 20.8 us for 18.0 at 2,048 x 14,336)
+    unsigned amax[UNITS];
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) {
-        unsigned amax = amax_bits(v[u]);
+        amax[u] = amax_bits(v[u]);
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));      // within the sixteen lanes
-        if (row[u] < 0) continue;
-        const Coding c = coding_of(amax);
-        store8<T>(codes + row[u] * ldc, kb[u] * QB + lane * 8, K, v[u], c);
-        if (lane == 0) scales[(long long)kb[u] * n_tokens + row[u]] = c.scale;
+        for (int o = 8; o > 0; o >>= 1) amax[u] = max(amax[u], __shfl_xor_sync(0xffffffffu, amax[u], o));      // within the sixteen lanes
+    }
+    unsigned own = amax[0];
+    int own_row = row[0], own_kb = kb[0];
+#pragma unroll
+    for (int u = 1; u < UNITS; ++u)
+        if (lane == u) own = amax[u], own_row = row[u], own_kb = kb[u];
+    const Coding mine = coding_of(own);
+    if (lane < UNITS && own_row >= 0) scales[(long long)own_kb * n_tokens + own_row] = mine.scale;
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        Coding c;
+        c.a = least_of(amax[u]);
+        c.factor = __shfl_sync(0xffffffffu, mine.factor, u, 16);
+        if (row[u] >= 0) store8<T>(codes + row[u] * ldc, kb[u] * QB + lane * 8, K, v[u], c);
     }
 }
 
