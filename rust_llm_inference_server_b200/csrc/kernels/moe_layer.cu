@@ -668,6 +668,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
     float* back = reinterpret_cast<float*>(pieces + (size_t)cap * SLOT);
     unsigned short *place = reinterpret_cast<unsigned short*>(back + cap), *slot_of = place + cap;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2;
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     const int rank = blockIdx.x % PARTS, n_groups = (p.width + 15) / 16, clusters = gridDim.x / PARTS;
     const int members = L_WARPS / teams, team = warp / members, member = warp % members;
     // this CTA's chunks: number i is chunk rank + PARTS * i of all, those of the shared expert first (until the plan is known, all)
@@ -791,6 +792,9 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
         known = n_chunks;
         n_chunks = (shared_chunks + sh.plan.n_active * own_chunks - rank + PARTS - 1) / PARTS;
     }
+    // every CTA of the cluster has begun before its shared memory is written from another
+    __syncwarp();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     int set = 0, from = 0, upto = 0;    // the chunks whose pieces are in shared memory: all of them, as a rule
 #pragma unroll 1
     for (int group0 = group - team; group0 < n_groups; group0 += clusters * teams, group += clusters * teams) {
