@@ -207,6 +207,15 @@ void blocks_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
             }
         }
     }
+    // The sums are in registers: tensor memory goes back before the cluster meets.  A CTA that held it there would wait for CTAs that may wait for tensor memory, which
+    // another kernel's CTAs hold that wait for their own cluster in turn; so whoever holds some here waits for nothing but its own copies and products.
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncwarp();
+    __syncthreads();
+    if (warp == 1) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(COLS) : "memory");
+    }
     const int f_local = (warp & 3) * 32 + lane, f = n0 + f_local, group = (warp - 2) / 4, t0 = group * C;
     if (splits == 1) {
         if (taker && fine && f < N) {
@@ -220,7 +229,6 @@ void blocks_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
     } else {
         // the products and copies of this CTA are done, so its stages hold the sums now: [row][feature]
         float* part = reinterpret_cast<float*>(base);
-        __syncwarp();
         if (taker) {
 #pragma unroll
             for (int i = 0; i < C / 2; ++i) {
@@ -239,12 +247,6 @@ void blocks_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
             }
         }
         cluster_sync_all();         // nobody leaves while others read its sums
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (warp == 1) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(COLS) : "memory");
     }
 }
 

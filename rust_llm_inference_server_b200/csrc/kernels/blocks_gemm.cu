@@ -20,7 +20,9 @@
 // cycles a block: 132 us; the widths of loads from tensor memory make no difference.)
 //
 // Every mbarrier wait is bounded (tcgen05_utils.cuh); a wait that runs out sets the error word, every role runs to its end without further waits, the CTAs
-// meet and free their tensor memory.
+// meet and free their tensor memory.  The allocation of tensor memory and the cluster's barriers have no bound, so no CTA may hold the one while it waits for the other beside
+// a kernel that does the same.  Here the launch takes the registers of a whole SM, and no other CTA that has tensor memory fits beside it; blocks_few.cuh gives its back
+// before its cluster meets.
 #include "blocks.cuh"
 #include "tcgen05_utils.cuh"
 #include <algorithm>
@@ -33,6 +35,7 @@ constexpr int BG_THREADS = 384, BG_WARPS = 8;           // three groups of four 
 // Registers a thread: 168 at launch for every group; the epilogue's 128 sums a thread and two sets of loads want more, the first group gives them up.
 constexpr int BG_REGS_LAUNCH = 168, BG_REGS_FIRST = 56, BG_REGS_EPILOGUE = 224;
 static_assert(BG_REGS_FIRST + 2 * BG_REGS_EPILOGUE <= 3 * BG_REGS_LAUNCH && BG_THREADS * BG_REGS_LAUNCH <= 65536, "a split above what the launch holds waits for good");
+static_assert(65536 - BG_THREADS * BG_REGS_LAUNCH < 4 * 32 * 16, "a CTA that holds tensor memory has four warps at least, of sixteen registers and more a thread");
 constexpr int BG_MAX_STAGES = 6, BG_MAX_BUFFERS = 4;
 constexpr int BG_MAX_SPLITS = 3;                        // the first pair's stages hold the others' sums
 constexpr int BG_STAGING = 8192;                        // bytes of results that an epilogue warp keeps for its stores at most

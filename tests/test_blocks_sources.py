@@ -36,3 +36,18 @@ def test_the_routed_layer_s_clusters_arrive_once_for_each_wait():
     for kernel, wait in (("moe_layer_up_kernel", "router_logits"), ("moe_layer_down_kernel", "moe_layer_down_kernel")):
         text = source("moe_layer.cu")
         assert body(text, kernel).count("barrier.cluster.arrive.") == 1 and body(text, wait).count("barrier.cluster.wait.") == 1
+
+
+def test_no_cta_of_the_products_of_few_rows_holds_tensor_memory_where_its_cluster_meets():
+    """Neither the allocation of tensor memory nor a cluster's barrier is bounded.  CTAs that hold the first and wait at the second, beside another kernel's that do the
+    same, may wait for each other for good; so tensor memory is given back before the first meeting."""
+    text = body(source("blocks_few.cuh"), "blocks_few_kernel")
+    assert text.count("tcgen05.alloc.") == text.count("tcgen05.dealloc.") == 1
+    assert text.index("tcgen05.alloc.") < text.index("tcgen05.dealloc.") < text.index("cluster_sync_all()")
+
+
+def test_the_products_of_many_rows_have_an_sm_to_themselves():
+    """Their CTAs hold all of an SM's tensor memory while the pair meets: their registers leave no room for another CTA that allocates some (four warps or more)."""
+    text = source("blocks_gemm.cu")
+    number = lambda name: int(re.search(rf"\b{name} = (\d+)\b", text).group(1))
+    assert 65536 - number("BG_THREADS") * number("BG_REGS_LAUNCH") < 4 * 32 * 16
