@@ -23,8 +23,8 @@
 // more of the load units than the weights: 16 tokens, 83 of 128 experts of 768 in blocks 135 us, 111 so).  Nothing but the result is rounded to the activations'
 // type: beside bfloat16 weights h is two bfloat16 numbers (their sum is h to 2^-17).  Codes become float16 by one instruction a pair (as bfloat16, which has none,
 // a word of four took 10 cycles of a scheduler instead of 5, and the products waited for it), so the tokens' rows and h's meet them as float16 of eleven bits, each
-// row (of h each piece of 128) times the power of two that brings its largest value to 2^14 .. 2^15: x is that exactly down to 2^-31 of the largest, h to 2^-11 of
-// every value, an eighth of what the result is rounded by.
+// row (of h each piece of 128) times the power of two that brings its largest value to 2^14 .. 2^15: x is that exactly down to 2^-31 of the largest, h is two such
+// numbers, whose sum is h to 2^-22, or 2^-39 of the piece's largest.
 //
 // What bounds it: memory in the two loops (8 tokens in bfloat16: 6.8 TB/s), and what comes before and between them, when memory is idle: 8 us from the launch
 // to the first expert's weights (the router's rows, the meeting of the cluster, the choice), 4 from the first CTA's last item to the down kernel's plan, 4 to its first
@@ -149,6 +149,14 @@ __device__ __forceinline__ float unscaling_of(int e) { return __uint_as_float((u
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
     const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Two numbers as float16 and what these leave of them.
+__device__ __forceinline__ void split_half(float a, float b, uint32_t& first, uint32_t& rest) {
+    const __half2 v = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(v);
+    first = *reinterpret_cast<const uint32_t*>(&v);
+    rest = pack_half(a - f.x, b - f.y);
 }
 
 // This lane's part of a column's row over a chunk: the vectors of bfloat16 that its A vectors meet.
@@ -630,7 +638,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
 constexpr int PARTS = 4;                                    // CTAs of a cluster: they share the chunks
 constexpr int LEAST_TEAMS = 2, MOST_TEAMS = 4;              // of a CTA: each has 16 output features of its own, and its warps share the CTA's chunks
 constexpr int HELD = 2;                                     // chunks that a warp has on their way
-template <bool CODES> __host__ __device__ constexpr int slot_bytes() { return CODES ? LK * 2 : LK * 4; }
+constexpr int SLOT = LK * 4;                                // bytes of a piece: its first numbers, and behind them the second ones
 
 struct DownShared {
     float reduce[L_WARPS][16][LT + 1];
@@ -640,14 +648,14 @@ struct DownShared {
 };
 // Behind it, for `cap` slots: h's pieces (128 k of a token's row), then what brings a slot's sums back, where a slot's piece lies in h (row * 128 + chunk of its k),
 // and the first slot of a chunk.
-template <bool CODES> constexpr size_t down_smem_bytes(int cap) { return sizeof(DownShared) + (size_t)cap * (slot_bytes<CODES>() + 4 + 2 + 2); }
+constexpr size_t down_smem_bytes(int cap) { return sizeof(DownShared) + (size_t)cap * (SLOT + 4 + 2 + 2); }
 // What a CTA takes of shared memory at most: the rest is the first-level cache, through which the weights on their way go (16 tokens, 50 experts of 1,408 of width 2,048
 // and a shared one, in bfloat16, whose pieces would fill it: 353, 214 and 179 us with 227, 195 and 163 KB, the pieces in one, two and two goes).
 constexpr int DOWN_SMEM = 163 * 1024;
-template <bool CODES> constexpr int most_slots() { return (int)((DOWN_SMEM - sizeof(DownShared)) / (slot_bytes<CODES>() + 8)) / 8 * 8; }
+constexpr int MOST_SLOTS = (int)((DOWN_SMEM - sizeof(DownShared)) / (SLOT + 8)) / 8 * 8;
 static_assert(MOST_TEAMS <= PARTS && L_THREADS == 512, "a CTA for each team's end");
 static_assert(sizeof(DownShared) % 16 == 0, "vectors of 16 bytes behind it");
-static_assert(most_slots<false>() >= LT * L_WARPS / LEAST_TEAMS * HELD, "a turn of all warps' chunks with all tokens");
+static_assert(MOST_SLOTS >= LT * L_WARPS / LEAST_TEAMS * HELD, "a turn of all warps' chunks with all tokens");
 static_assert((L_MAX_PAIRS + LT) * (MOST_K / LK) <= 65536, "a piece's place in 16 bits");
 
 // Where unit u of eight k lies within a slot: the four lanes of a load side by side (beside codes a lane takes 16 k, two units, at a time), the halves of odd slots
@@ -663,7 +671,6 @@ template <bool CODES, int GROUPS>
 __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const LayerArgs p, int teams, int cap) {
     extern __shared__ __align__(16) unsigned char down_smem[];
     DownShared& sh = *reinterpret_cast<DownShared*>(down_smem);
-    constexpr int SLOT = slot_bytes<CODES>();
     unsigned char* pieces = down_smem + sizeof(DownShared);
     float* back = reinterpret_cast<float*>(pieces + (size_t)cap * SLOT);
     unsigned short *place = reinterpret_cast<unsigned short*>(back + cap), *slot_of = place + cap;
@@ -762,8 +769,12 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
                     const unsigned top = max(max(v[i].x & 0x7fffffffu, v[i].y & 0x7fffffffu), max(v[i].z & 0x7fffffffu, v[i].w & 0x7fffffffu));
                     const int e = max((int)(__reduce_max_sync(0xffffffffu, top) >> 23), LEAST_EXPONENT);
                     const float scaling = scaling_of(e);
-                    auto two = [&](uint32_t a, uint32_t b) { return pack_half(__uint_as_float(a) * scaling, __uint_as_float(b) * scaling); };
-                    *reinterpret_cast<uint2*>(to + unit_of<CODES>(lane >> 1, slot) * 16 + (lane & 1) * 8) = make_uint2(two(v[i].x, v[i].y), two(v[i].z, v[i].w));
+                    uint2 hi, lo;
+                    split_half(__uint_as_float(v[i].x) * scaling, __uint_as_float(v[i].y) * scaling, hi.x, lo.x);
+                    split_half(__uint_as_float(v[i].z) * scaling, __uint_as_float(v[i].w) * scaling, hi.y, lo.y);
+                    to += unit_of<CODES>(lane >> 1, slot) * 16 + (lane & 1) * 8;
+                    *reinterpret_cast<uint2*>(to) = hi;
+                    *reinterpret_cast<uint2*>(to + LK * 2) = lo;
                     if (lane == 0) back[slot] = unscaling_of(e);
                 } else {
                     *reinterpret_cast<uint4*>(to + (lane >> 4) * (LK * 2) + unit_of<CODES>(lane & 15, slot) * 16) = v[i];
@@ -818,6 +829,7 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
 #pragma unroll
                         for (int j = 0; j < Chunk<CODES>::PARTS; ++j) held[u].operand(s, j, a[s][j]);
                     const float scale = CODES ? held[u].scale[0] : 1.f;
+                    constexpr int VECS = Column<CODES>::VECS;
 #pragma unroll
                     for (int n = 0; n < GROUPS; ++n) {
                         if (GROUPS > 1 && (at.tokens >> (8 * n) & 0xffu) == 0u) continue;
@@ -830,13 +842,13 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
 #pragma unroll
                         for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
 #pragma unroll
-                            for (int v = 0; v < 2; ++v) {           // codes: the halves of the step's k; else h's two numbers
-                                const uint4 b = *reinterpret_cast<const uint4*>(
-                                    piece + ((CODES ? s * 128 + v * 64 : v * (LK * 2) + s * 64) + (lane & 3) * 16 ^ flip));
+                            for (int v = 0; v < VECS; ++v) {        // (codes: the halves of the step's k)
+                                const unsigned char* at_k = piece + ((s * VECS + v) * 64 + (lane & 3) * 16 ^ flip);
+                                const uint4 b = *reinterpret_cast<const uint4*>(at_k), c = *reinterpret_cast<const uint4*>(at_k + LK * 2);
 #pragma unroll
-                                for (int j = 0; j < 2; ++j) {
-                                    const int q = CODES ? 2 * v + j : j;
-                                    mma_step<CODES>(part[(j + (CODES ? 0 : v)) & 1], a[s][q], j ? b.z : b.x, j ? b.w : b.y);
+                                for (int j = 0; j < 2; ++j) {       // h's two numbers in turn
+                                    mma_step<CODES>(part[0], a[s][2 * v + j], j ? b.z : b.x, j ? b.w : b.y);
+                                    mma_step<CODES>(part[1], a[s][2 * v + j], j ? c.z : c.x, j ? c.w : c.y);
                                 }
                             }
                         }
@@ -924,12 +936,12 @@ template <bool CODES, int GROUPS, int TEAM> int launch_layer(const LayerArgs& p,
     if (rc != 0) return rc;
     // as many slots as the pieces of a CTA's chunks can take, up to what its shared memory holds
     const auto share = [](int k) { return ((k + LK - 1) / LK + PARTS - 1) / PARTS; };
-    const int all = p.n_tokens * (p.top * share(p.inner) + share(p.inner_shared)), cap = all < most_slots<CODES>() ? (all + 7) / 8 * 8 : most_slots<CODES>();
+    const int all = p.n_tokens * (p.top * share(p.inner) + share(p.inner_shared)), cap = all < MOST_SLOTS ? (all + 7) / 8 * 8 : MOST_SLOTS;
     const int groups = (p.width + 15) / 16;
     const int teams = (groups + MOST_TEAMS - 1) / MOST_TEAMS * PARTS * 4 >= 3 * sms ? MOST_TEAMS : LEAST_TEAMS;
-    const int most = clusters_at_once(moe_layer_down_kernel<CODES, GROUPS>, PARTS, down_smem_bytes<CODES>(most_slots<CODES>()), sms, known_down);
+    const int most = clusters_at_once(moe_layer_down_kernel<CODES, GROUPS>, PARTS, down_smem_bytes(MOST_SLOTS), sms, known_down);
     const int clusters = (groups + teams - 1) / teams < most ? (groups + teams - 1) / teams : most;
-    rlis_launch_cluster(moe_layer_down_kernel<CODES, GROUPS>, dim3((unsigned)(clusters * PARTS)), dim3(L_THREADS), down_smem_bytes<CODES>(cap), stream, dim3(PARTS, 1, 1), p,
+    rlis_launch_cluster(moe_layer_down_kernel<CODES, GROUPS>, dim3((unsigned)(clusters * PARTS)), dim3(L_THREADS), down_smem_bytes(cap), stream, dim3(PARTS, 1, 1), p,
                         teams, cap);
     return RLIS_LAUNCH_CHECK();
 }

@@ -224,8 +224,8 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
     shared expert in the same form; `interleave` (`shared_interleave`) as `moe_up` takes it (in blocks 0, 4 or a multiple of 8); the gating of `glu_act` with
     `slope`, `limit` and `up_shift`.  W, I and S are multiples of 8, in blocks of 16, and at most 16,384; the router has up to 512 outputs.
 
-    Scores and sums are float32; the experts' gated results go into the second product to 2^-17 of each (beside codes to 2^-11); a token's result is rounded
-    once."""
+    Scores and sums are float32; the experts' gated results go into the second product to 2^-17 of each (beside codes to 2^-22, or 2^-39 of the largest of 128 of
+    them); a token's result is rounded once."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
         raise KernelError("moe_layer: expected bfloat16 rows [T, W] with unit stride on the device; there is no CPU path")
     dev = x.device
