@@ -8,9 +8,9 @@
 // The quotient of two bfloat16 numbers often lies right between two e4m3 (2 to 3 of 1,000 codes), and p = x * fl(448 / a) is off by up to 2^-23 of it, to
 // either side: p alone would take one code or the other by chance.  A point between two codes has five significant bits at most, and a quotient 7 X / A of
 // integers of eight bits that is none of them is at least 2^-13 of it away.  So p rounded to 16 bits (off by 2^-17 at most) is that point where the quotient is,
-// and stays on its side where it is not: for bfloat16 its e4m3 is the quotient's.  A float32 x may come closer: where the 16 bits end in eleven zeros (one
-// of 2,048), the quotient is formed by a division.  (As divisions, all of them, the codes of 2,048 rows of 14,336 took 5 us more;
-// two values at a time in an instruction 1.4 less than one by one: 16.6.)
+// and stays on its side where it is not: for bfloat16 its e4m3 is the quotient's.  A float32 x may come closer: where the 16 bits may be such a point (one
+// of 4,096), the sign of 448 x - p a says on which side of them the quotient lies (to_its_side).  (As divisions, all of them, the
+// codes of 2,048 rows of 14,336 took 5 us more; two values at a time in an instruction 1.4 less than one by one: 16.6.)
 #pragma once
 #include "common.cuh"
 #include <cuda_fp8.h>
@@ -19,6 +19,7 @@ namespace {
 constexpr int QB = 128;                              // a block's edge
 constexpr unsigned LEAST_BITS = 0x0D800000u;         // 2^-100
 constexpr unsigned LARGE_BITS = 0x71800000u;         // 2^100
+constexpr unsigned SMALL_BITS = 0x3c800000u;         // 2^-6
 
 // What a block's values are turned to codes with.
 struct Coding {
@@ -104,23 +105,35 @@ template <typename T> __device__ __forceinline__ void widen(const Eight<T>& e, f
         else v[i] = __uint_as_float((i & 1) ? e.w[i >> 1] & 0xffff0000u : e.w[i >> 1] << 16);
     }
 }
+// q, to which p was rounded, goes a unit to the side of it on which 448 x / a lies, so that a q between two e4m3 takes the right one of them (any other stays between the
+// same two).  448 x - q a is formed exactly for a q of five bits: each product is a float32 and what its rounding left (x and a have 24 bits, 448 three), the products lie
+// next to each other, so their difference and that of the rests are numbers of a few bits.  `by` is 448, and beside an a above 2^100 both are 2^-20 of it.
+__device__ __forceinline__ float to_its_side(float q, float x, float by, float a) {
+    const float p = __fmul_rn(x, by), r = __fmul_rn(q, a);
+    const float d = __fadd_rn(__fsub_rn(p, r), __fsub_rn(__fmaf_rn(x, by, -p), __fmaf_rn(q, a, -r)));
+    const int unit = (__float_as_int(d) ^ __float_as_int(q)) >> 31 | 1;
+    return __int_as_float(__float_as_int(q) + (fabsf(d) > 0.f ? unit : 0));         // (a NaN stays one)
+}
 template <typename T> __device__ __forceinline__ uint2 codes8(const Eight<T>& e, const Coding& c) {
     float v[8], q[8];
     widen(e, v);
-    bool near = false;
     const unsigned long long factors = pair_of(c.factor, c.factor);
 #pragma unroll
     for (int i = 0; i < 8; i += 2) product_of_16_bits(v[i], v[i + 1], factors, q[i], q[i + 1]);
     if (sizeof(T) == 4) {
+        // a middle of two e4m3 has a one as its fifth bit and zeros behind it, or lies among those below 2^-6
+        unsigned middle = ~0u, small = ~0u;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) near |= (__float_as_uint(q[i]) & 0x7ffffu) == 0u && q[i] != 0.f;
-    }
-    if (sizeof(T) == 4 && near) {
-        // (above 2^100 both by 2^-20 less, so that 448 x stays finite)
-        const bool large = __float_as_uint(c.a) > LARGE_BITS;
-        const float mul = large ? 448.f * 0x1p-20f : 448.f, div = large ? c.a * 0x1p-20f : c.a;
+        for (int i = 0; i < 8; ++i) {
+            middle = min(middle, (__float_as_uint(q[i]) & 0xfffffu) ^ 0x80000u);
+            small = min(small, 2u * __float_as_uint(q[i]) - 2u);            // (a zero is none of them)
+        }
+        if (middle == 0u || small < 2u * SMALL_BITS - 2u) {
+            const bool large = __float_as_uint(c.a) > LARGE_BITS;
+            const float by = large ? 448.f * 0x1p-20f : 448.f, a = large ? c.a * 0x1p-20f : c.a;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = __fdiv_rn(v[i] * mul, div);
+            for (int i = 0; i < 8; ++i) q[i] = to_its_side(q[i], v[i], by, a);
+        }
     }
     return make_uint2(pack_codes(q), pack_codes(q + 4));
 }

@@ -1,6 +1,7 @@
 // Values into e4m3 with a float32 scale for each block (blocks.cuh says how): 128 of a row (activations), or 128 x 128 of a matrix (weights).
-// Both kernels read their input once and keep it in registers while the block's largest value is found.  2,048 rows of 14,336 (bfloat16): 16.6 us, 5.3 TB/s, where
-// instructions still count beside memory (see blocks.cuh); a matrix of 16,384 x 2,048 31.2 us in float32 (5.4 TB/s), 19.5 in bfloat16; 64 rows of 4,096 1.9 us, a launch.
+// Both kernels read their input once and keep it in registers while the block's largest value is found.  2,048 rows of 14,336 (bfloat16): 15.8 us, 5.6 TB/s, where
+// instructions still count beside memory (see blocks.cuh), in float32 27.5 (5.3 TB/s); a matrix of 16,384 x 2,048 33.7 us in float32 (5.0 TB/s), 18.9 in bfloat16; 64 rows
+// of 4,096 1.9 us, a launch.
 #include "blocks.cuh"
 
 namespace {
