@@ -624,7 +624,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_up_kernel(const LayerA
                 if (CODES) {
                     p.h[at] = v;
                 } else {
-                    const bf16 hi = __float2bfloat16_rn(v);
+                    bf16 hi = __float2bfloat16_rn(v);
+                    if (__hisinf(hi)) hi = __float2bfloat16_rz(v);          // (beyond the largest bfloat16 the second number makes up for it)
                     p.h_hi[at] = hi;
                     p.h_lo[at] = __float2bfloat16_rn(v - __bfloat162float(hi));
                 }
@@ -664,6 +665,9 @@ template <bool CODES> __device__ __forceinline__ int unit_of(int u, int slot) {
     const int at = CODES ? (u & 8) | (u & 1) << 2 | (u >> 1 & 3) : u;
     return at ^ (slot & 1) << 2;
 }
+
+// The sum of the products with h's first numbers and of those with the second: where the first is infinite, by an h or a weight that is, the second says nothing.
+__device__ __forceinline__ float joined(float first, float second) { return fabsf(first) < INFINITY ? first + second : first; }
 
 // A cluster takes 16 * teams output features at a time; the chunks (of the shared expert, then of the active ones) go round its CTAs, and round the warps of a
 // team.
@@ -857,8 +861,8 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
                         for (int c = 0; c < 2; ++c)
                             if (at.tokens >> (t0 + c) & 1u) {
                                 const float by = CODES ? back[first + __popc(at.tokens & ((1u << (t0 + c)) - 1u))] : 1.f;
-                                acc[n][c] = fmaf((part[0][c] + part[1][c]) * by, scale, acc[n][c]);
-                                acc[n][2 + c] = fmaf((part[0][2 + c] + part[1][2 + c]) * by, scale, acc[n][2 + c]);
+                                acc[n][c] = fmaf(joined(part[0][c], part[1][c]) * by, scale, acc[n][c]);
+                                acc[n][2 + c] = fmaf(joined(part[0][2 + c], part[1][2 + c]) * by, scale, acc[n][2 + c]);
                             }
                     }
                 }
