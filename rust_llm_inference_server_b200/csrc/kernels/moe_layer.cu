@@ -129,16 +129,23 @@ template <bool CODES> struct Chunk {
         }
     }
 };
-// `row0`, `row1`: this lane's rows of K; the chunk is k0 .. k0 + 127.  What lies past the row's end is its last 16 bytes again, which meet zeros: the columns' rows
-// are padded with them, so that no chunk needs code of its own.
+__device__ const uint4 NOTHING = {0u, 0u, 0u, 0u};
+// `row0`, `row1`: this lane's rows of K; the chunk is k0 .. k0 + 127.  The columns' rows are padded with zeros, so that no chunk needs code of its own: of what lies past
+// the row's end, codes are its last 16 bytes again (a NaN among them has made the sum one already), and bfloat16 are zeros (an infinity would make a NaN of it).
 template <bool CODES>
 __device__ __forceinline__ void load_chunk(Chunk<CODES>& c, const unsigned char* row0, const unsigned char* row1, int k0, int K, int lane) {
     constexpr int PER = CODES ? 16 : 8;
 #pragma unroll
     for (int s = 0; s < Chunk<CODES>::STEPS; ++s) {
-        const int at = min(k0 + (s * 4 + (lane & 3)) * PER, K - PER) * (16 / PER);
-        c.a[s][0] = stream16(row0 + at);
-        c.a[s][1] = stream16(row1 + at);
+        const int k = k0 + (s * 4 + (lane & 3)) * PER;
+        if (CODES) {
+            const int at = min(k, K - PER);
+            c.a[s][0] = stream16(row0 + at);
+            c.a[s][1] = stream16(row1 + at);
+        } else {
+            c.a[s][0] = stream16(k < K ? row0 + 2 * k : reinterpret_cast<const unsigned char*>(&NOTHING));
+            c.a[s][1] = stream16(k < K ? row1 + 2 * k : reinterpret_cast<const unsigned char*>(&NOTHING));
+        }
     }
 }
 

@@ -72,3 +72,23 @@ def test_an_infinite_weight(T):
         y = layer(x, up, down, False)
         assert bool((y[:, 3] == float("inf")).all()) and bool((y[:, 40] == float("-inf")).all()) and bool(y[:, :3].isfinite().all()) and bool(y[:, 41:].isfinite().all())
         assert bool((layer(-x, torch.cat([-up[:I], up[I:]]), down, False)[:, 3] == float("-inf")).all())
+
+
+@pytest.mark.parametrize("T", [1, 6, 14])
+def test_an_infinite_weight_at_its_row_s_end(T):
+    """Rows that end inside a chunk of 128: nothing past the end takes part."""
+    W, I = 200, 144
+    g = torch.Generator().manual_seed(T)
+    x, up = torch.rand(T, W, generator=g) + 0.5, torch.rand(2 * I, W, generator=g) + 0.5
+    down = torch.rand(W, I, generator=g) - 0.5
+    for at in (I - 8, I - 1):
+        bad = down.clone()
+        bad[3, at], bad[199, at] = float("inf"), float("-inf")
+        y = layer(x, up, bad, False)
+        assert bool((y[:, 3] == float("inf")).all()) and bool((y[:, 199] == float("-inf")).all()) and bool(y[:, :3].isfinite().all()) and bool(y[:, 4:199].isfinite().all())
+    for row in (20, I + 20):                # a gate's, a linear branch's
+        for at in (W - 8, W - 1):
+            bad = up.clone()
+            bad[row, at] = float("inf")
+            y, sign = layer(x, bad, down, False), down[:, 20].sign()
+            assert torch.equal(y, (sign * float("inf")).expand(T, W))
