@@ -867,9 +867,11 @@ __global__ __launch_bounds__(L_THREADS, 1) void moe_layer_down_kernel(const Laye
 #pragma unroll
                         for (int c = 0; c < 2; ++c)
                             if (at.tokens >> (t0 + c) & 1u) {
+                                // (of the two scales the large one first meets the small one, so that a sum leaves float32's range only if the result does)
                                 const float by = CODES ? back[first + __popc(at.tokens & ((1u << (t0 + c)) - 1u))] : 1.f;
-                                acc[n][c] = fmaf(joined(part[0][c], part[1][c]) * by, scale, acc[n][c]);
-                                acc[n][2 + c] = fmaf(joined(part[0][2 + c], part[1][2 + c]) * by, scale, acc[n][2 + c]);
+                                const float one = by > 1.f ? by * scale : by, two = by > 1.f ? 1.f : scale;
+                                acc[n][c] = fmaf(joined(part[0][c], part[1][c]) * one, two, acc[n][c]);
+                                acc[n][2 + c] = fmaf(joined(part[0][2 + c], part[1][2 + c]) * one, two, acc[n][2 + c]);
                             }
                     }
                 }

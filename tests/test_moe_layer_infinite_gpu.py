@@ -47,15 +47,16 @@ def test_an_infinite_gated_result(T, blocks):
     assert bool((layer(x, up, down, blocks) == -y).all())
 
 
+@pytest.mark.parametrize("blocks", [False, True])
 @pytest.mark.parametrize("T", [1, 6, 14])
-def test_a_gated_result_beyond_the_largest_bfloat16(T):
-    """2^127 (2 - 2^-9) is a float32, and nearest to it is the bfloat16 infinity."""
+def test_a_gated_result_beyond_the_largest_bfloat16(T, blocks):
+    """2^127 (2 - 2^-9) is a float32, and nearest to it is the bfloat16 infinity.  (In blocks the second product's largest code is 4, four times its weight's.)"""
     W, I = 48, 144
     x, up = inputs(T, W, I, 2.0 ** 64, 2.0 ** 63 * 255 / 128, 2.0 ** 63 * (1 / 128 - 2.0 ** -9))
     down = torch.zeros(W, I)
     down[:, 5] = 2.0 ** -10
     down[1::2, 5] = -2.0 ** -20
-    y = layer(x, up, down, False)
+    y = layer(x, up, down, blocks)
     want = (down[:, 5].double() * 2.0 ** 127 * (2 - 2.0 ** -9)).bfloat16().float()
     assert torch.equal(y, want.expand(T, W))
 
