@@ -321,7 +321,7 @@ bool plain_rows_fit(int M, int N, int K, int sms) {
     return M * f.per <= 2 * PLAIN_AT_ONCE * plain_warps(f, sms) && smem <= PLAIN_SMEM && f.tiles * f.splits <= (smem <= PLAIN_TWICE ? 2 * sms : sms);
 }
 template <typename T, typename OutT>
-int launch_blocks_few_plain(const void* x, long long ldx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int sms, cudaStream_t stream) {
+int launch_blocks_few_plain(const void* x, long long ldx, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K, int early, int sms, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed{0}, wide{0};
     constexpr int NT = PLAIN_NT;
     using Rows = PlainRows<T>;
@@ -334,7 +334,7 @@ int launch_blocks_few_plain(const void* x, long long ldx, const void* w, long lo
     const int vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (M == 1 || (ldx * (long long)sizeof(T)) % 16 == 0) ? 1 : 0;
     rlis_launch_cluster(blocks_few_kernel<NT, OutT, Rows>, dim3((unsigned)f.tiles, (unsigned)f.splits), 64 + 32 * plain_warps(f, sms),
                         (size_t)plain_smem(f), stream, dim3(1, (unsigned)f.splits, 1), map_w, map_w,
-                        Rows{static_cast<const T*>(x), ldx, K, vec}, (const float*)nullptr, sw, (OutT*)y, M, N, f.k_blocks, f.per, f.stages, 0);
+                        Rows{static_cast<const T*>(x), ldx, K, vec}, (const float*)nullptr, sw, (OutT*)y, M, N, f.k_blocks, f.per, f.stages, early);
     return RLIS_LAUNCH_CHECK();
 }
 }  // namespace

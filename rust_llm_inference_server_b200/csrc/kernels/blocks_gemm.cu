@@ -485,17 +485,17 @@ extern "C" long long rlis_blocks_gemm_scratch(int M, int N, int K) {
 }
 
 // The same for plain rows x [M, K] of `dtype` (ldx elements apart), which the product puts into blocks itself or rlis_quantize_rows before it.  scratch: 16-byte aligned,
-// M * ceil(K / 16) * 16 bytes of codes and behind them M * ceil(K / 128) floats.  (Of two kernels the first lets the second start once all kernels before itself have
-// finished; none but itself is in flight then, and it does not write w: w's first tiles are always read early.)
+// M * ceil(K / 16) * 16 bytes of codes and behind them M * ceil(K / 128) floats.  early: as above for one kernel.  (Of two the first lets the second start once all
+// kernels before itself have finished; none but itself is in flight then, and it does not write w: w's first tiles are always read early.)
 extern "C" int rlis_blocks_gemm_rows(const void* x, long long ldx, int dtype, void* scratch, const void* w, long long ldw, const float* sw, void* y, int M, int N, int K,
-                                     int out_dtype, cudaStream_t stream) {
+                                     int out_dtype, int early, cudaStream_t stream) {
     if (M <= 0 || N <= 0) return 0;
     if (K <= 0) return RLIS_ERR_UNSUPPORTED;
     const int sms = sms_of_device();
     if (plain_rows_fit(M, N, K, sms)) {
         if ((dtype != RLIS_F32 && dtype != RLIS_BF16) || (out_dtype != RLIS_F32 && out_dtype != RLIS_BF16) || !codes_fit(w, ldw, K)) return RLIS_ERR_UNSUPPORTED;
-#define RLIS_BP(T) (out_dtype == RLIS_F32 ? launch_blocks_few_plain<T, float>(x, ldx, w, ldw, sw, y, M, N, K, sms, stream) \
-                                          : launch_blocks_few_plain<T, bf16>(x, ldx, w, ldw, sw, y, M, N, K, sms, stream))
+#define RLIS_BP(T) (out_dtype == RLIS_F32 ? launch_blocks_few_plain<T, float>(x, ldx, w, ldw, sw, y, M, N, K, early, sms, stream) \
+                                          : launch_blocks_few_plain<T, bf16>(x, ldx, w, ldw, sw, y, M, N, K, early, sms, stream))
         return dtype == RLIS_F32 ? RLIS_BP(float) : RLIS_BP(bf16);
 #undef RLIS_BP
     }

@@ -161,7 +161,7 @@ def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> 
         room = kernels.rlis_blocks_gemm_scratch(T, N, K)
         scratch = _empty((room,), (1,), torch.uint8) if room else None
         check(kernels.rlis_blocks_gemm_rows(x.data_ptr(), x.stride(0), code, scratch.data_ptr() if room else None, weight.data_ptr(), w.stride, w.scales.data_ptr(), out.data_ptr(), T, N, K,
-                                          out_code, _stream()), "linear_blocks")
+                                            out_code, int(early), _stream()), "linear_blocks")
         if room:
             _count("quantize_rows")
     else:

@@ -120,7 +120,7 @@ SIGNATURES = {
     "rlis_quantize_rows": [P, LL, P, LL, P, I, I, I, P],
     "rlis_quantize_matrix": [P, LL, LL, P, LL, P, I, I, I, I, P],
     "rlis_blocks_gemm_scratch": [I, I, I],
-    "rlis_blocks_gemm_rows": [P, LL, I, P, P, LL, P, P, I, I, I, I, P],
+    "rlis_blocks_gemm_rows": [P, LL, I, P, P, LL, P, P, I, I, I, I, I, P],
     "rlis_blocks_gemm": [P, LL, P, P, LL, P, P, I, I, I, I, I, P],
 }
 
