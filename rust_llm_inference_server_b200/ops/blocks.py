@@ -216,7 +216,8 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
               shared: tuple | None = None, shared_gate: bool = False, slope: float = 1.0, limit: float | None = None, up_shift: float = 0.0, interleave: int = 0,
               shared_interleave: int = 0, out: torch.Tensor | None = None) -> torch.Tensor:
     """A whole mixture of experts for up to `MOE_LAYER_TOKENS` tokens in two launches: what `moe_route`, `moe_up`, `moe_down`, a shared expert and `moe_combine`
-    compute, every weight read once.  x [T, W] bfloat16 (rows of a wider tensor if need be); the result [T, W] bfloat16 (`out`, or a new tensor).
+    compute, every weight read once.  x [T, W] bfloat16, rows that start at multiples of 16 bytes (of a wider tensor if need be); the result [T, W] bfloat16 (`out`, or
+    a new tensor).
 
     w_router float32 [experts + n_identity (+ 1), W] (with `shared_gate` its last row is the logit of the shared expert's gate), `correction`, `router_bias`,
     `scoring` ("sigmoid", "softmax" or "softmax_chosen"), `groups`, `normalize` and `n_identity` as `moe_route` takes them; `top` up to 16.
@@ -235,6 +236,8 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
                              normalize=normalize, n_identity=n_identity, shared=shared, shared_gate=shared_gate, slope=slope, limit=limit, up_shift=up_shift,
                              interleave=interleave, shared_interleave=shared_interleave, out=out)
     T, W = x.shape
+    if x.data_ptr() % 16 or (T > 1 and x.stride(0) % 8):
+        raise KernelError(f"moe_layer: rows of x start at multiples of 16 bytes, got an address of {x.data_ptr() % 16} beyond one and strides {x.stride()}")
     if T > MOE_LAYER_TOKENS:
         raise KernelError(f"moe_layer: takes up to {MOE_LAYER_TOKENS} tokens, got {T}; more go through moe_route, moe_up, moe_down and moe_combine")
     if scoring not in _SCORING:
