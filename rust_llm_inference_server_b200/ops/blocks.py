@@ -19,6 +19,10 @@ CODES = torch.float8_e4m3fn
 _device = torch._C._cuda_getDevice
 
 
+def _shape(t):
+    return tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__
+
+
 def _code_rows(values: torch.Tensor, what: str) -> int:
     """Bytes between the rows of a tensor of codes [.., N, K]."""
     if not isinstance(values, torch.Tensor) or values.dtype != CODES or not values.is_cuda:
@@ -39,8 +43,8 @@ class BlockRows:
     """Rows in blocks: `values` e4m3 [T, K] and `scales` float32 [ceil(K / 128), T], a block's scales of all rows side by side."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
-        if values.dim() != 2:
-            raise KernelError(f"BlockRows: expected rows [T, K], got {tuple(values.shape)}")
+        if not isinstance(values, torch.Tensor) or values.dim() != 2:
+            raise KernelError(f"BlockRows: expected rows [T, K], got {_shape(values)}")
         self.stride = _code_rows(values, "BlockRows")
         _scales(scales, values, (-(-values.shape[1] // BLOCK), values.shape[0]), "BlockRows")
         self.values, self.scales = values, scales
@@ -60,8 +64,8 @@ class BlockMatrix:
     """A matrix [N, K], or a stack of them [E, N, K], in blocks: `values` e4m3 and `scales` float32 [.., ceil(N / 128), ceil(K / 128)]."""
 
     def __init__(self, values: torch.Tensor, scales: torch.Tensor):
-        if values.dim() not in (2, 3):
-            raise KernelError(f"BlockMatrix: expected a matrix or a stack of them, got {tuple(values.shape)}")
+        if not isinstance(values, torch.Tensor) or values.dim() not in (2, 3):
+            raise KernelError(f"BlockMatrix: expected a matrix or a stack of them, got {_shape(values)}")
         self.stride = _code_rows(values, "BlockMatrix")
         N, K = values.shape[-2:]
         if values.dim() == 3 and values.shape[0] > 1 and values.stride(0) != N * self.stride:
@@ -195,7 +199,7 @@ def _layer_matrix(m, dims: int, rows, k, blocks: bool, device, name: str) -> _La
     t = m.values if blocks else m
     if not isinstance(t, torch.Tensor) or t.device != device or t.dim() != dims or (rows is not None and t.shape[-2] != rows) or (k is not None and t.shape[-1] != k):
         raise KernelError(f"moe_layer: {name}: expected {'a stack of matrices' if dims == 3 else 'a matrix'} of {rows} x {k} on {device}, "
-                          f"got {tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__}")
+                          f"got {_shape(t)}")
     if blocks:
         return _LayerMatrix(t.data_ptr(), m.scales.data_ptr(), m.stride, t.shape[-2] * m.stride)
     if t.dtype != torch.bfloat16 or not t.is_contiguous():
@@ -206,7 +210,7 @@ def _layer_matrix(m, dims: int, rows, k, blocks: bool, device, name: str) -> _La
 def _layer_vector(v, n: int, device, name: str):
     if v is None:
         return None
-    if v.dtype != torch.float32 or tuple(v.shape) != (n,) or not v.is_contiguous() or v.device != device:
+    if not isinstance(v, torch.Tensor) or v.dtype != torch.float32 or tuple(v.shape) != (n,) or not v.is_contiguous() or v.device != device:
         raise KernelError(f"moe_layer: {name}: expected contiguous float32 [{n}] on {device}")
     return v.data_ptr()
 
@@ -258,12 +262,12 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
     elif shared_gate:
         raise KernelError("moe_layer: a gate on the shared expert, and no shared expert")
     n_out = E + int(n_identity)
-    if w_router.dtype != torch.float32 or tuple(w_router.shape) != (n_out + (1 if shared_gate else 0), W) or not w_router.is_contiguous() or w_router.device != dev:
-        raise KernelError(f"moe_layer: expected a contiguous float32 router [{n_out + (1 if shared_gate else 0)}, {W}] on {dev}, got {w_router.dtype} {tuple(w_router.shape)}")
+    if not isinstance(w_router, torch.Tensor) or w_router.dtype != torch.float32 or tuple(w_router.shape) != (n_out + (1 if shared_gate else 0), W) or not w_router.is_contiguous() or w_router.device != dev:
+        raise KernelError(f"moe_layer: expected a contiguous float32 router [{n_out + (1 if shared_gate else 0)}, {W}] on {dev}, got {_shape(w_router)}")
     n_groups, keep = groups if groups is not None else (1, 1)
     if out is None:
         out = _empty((T, W), (W, 1), torch.bfloat16)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (T, W) or not out.is_contiguous() or out.device != dev:
+    elif not isinstance(out, torch.Tensor) or out.dtype != torch.bfloat16 or tuple(out.shape) != (T, W) or not out.is_contiguous() or out.device != dev:
         raise KernelError(f"moe_layer: out: expected contiguous bfloat16 {(T, W)} on {dev}")
     if T == 0:
         return out

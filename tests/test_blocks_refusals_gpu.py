@@ -25,3 +25,15 @@ def test_rows_of_the_layer_that_start_anywhere(T):
         assert bool((ops.moe_layer(uneven, m["router"], m["up"], m["down"], 2) == 0).all())
     wide[:, 8:136] = m["x"]
     assert torch.equal(ops.moe_layer(wide[:, 8:136], m["router"], m["up"], m["down"], 2), ops.moe_layer(m["x"], m["router"], m["up"], m["down"], 2))
+
+
+def test_what_is_no_tensor():
+    from rust_llm_inference_server_b200 import ops
+    from rust_llm_inference_server_b200.ops import KernelError
+    m = make(2, 128, 32, 4, 32)
+    layer = lambda **c: ops.moe_layer(m["x"], c.pop("router", m["router"]), m["up"], m["down"], 2, **c)
+    layer()
+    for call in (lambda: layer(router=[0.0] * 4), lambda: layer(correction=[0.0] * 4), lambda: layer(router_bias=0.5), lambda: layer(out=[]), lambda: layer(shared=([], m["shared_down"])),
+                 lambda: ops.linear_blocks([[1.0]], ops.quantize_matrix(m["router"])), lambda: ops.linear_blocks(m["x"], None), lambda: ops.quantize_matrix([1.0])):
+        with pytest.raises(KernelError):
+            call()
