@@ -1016,9 +1016,8 @@ extern "C" int rlis_moe_layer(const RlisMoeLayer* a, cudaStream_t stream) {
         a->inner_shared < 0 || (a->shared_gate && !shared) || a->interleave < 0 || (a->interleave > 0 && a->inner % a->interleave != 0) || a->interleave_shared < 0 ||
         (a->interleave_shared > 0 && a->inner_shared % a->interleave_shared != 0) || a->width > MOST_K || a->inner > MOST_K || a->inner_shared > MOST_K)
         return RLIS_ERR_UNSUPPORTED;
-    // codes: the eight rows that a load instruction takes lie in one block of rows
-    if (codes && ((a->interleave > 0 && a->interleave != 4 && a->interleave % 8 != 0) || (a->interleave_shared > 0 && a->interleave_shared != 4 && a->interleave_shared % 8 != 0)))
-        return RLIS_ERR_UNSUPPORTED;
+    // (every lane has the scales of its own rows, so any interleaving would do; beside codes groups of fewer than four rows are not offered, since no loader lays them out)
+    if (codes && (a->interleave % 4 != 0 || a->interleave_shared % 4 != 0)) return RLIS_ERR_UNSUPPORTED;
     if ((reinterpret_cast<uintptr_t>(a->x) & 15) != 0 || a->ldx % 8 != 0 || (reinterpret_cast<uintptr_t>(a->router) & 15) != 0 || (reinterpret_cast<uintptr_t>(a->workspace) & 15) != 0)
         return RLIS_ERR_UNSUPPORTED;
     const RlisLayerMatrix* all[4] = {&a->up, &a->down, &a->shared_up, &a->shared_down};

@@ -226,7 +226,7 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
     w_router float32 [experts + n_identity (+ 1), W] (with `shared_gate` its last row is the logit of the shared expert's gate), `correction`, `router_bias`,
     `scoring` ("sigmoid", "softmax" or "softmax_chosen"), `groups`, `normalize` and `n_identity` as `moe_route` takes them; `top` up to 16.
     w_gate_up [experts, 2 I, W] and w_down [experts, W, I], both contiguous bfloat16 or both stacks in blocks; `shared` = (gate|up [2 S, W], down [W, S]) of the
-    shared expert in the same form; `interleave` (`shared_interleave`) as `moe_up` takes it (in blocks 0, 4 or a multiple of 8); the gating of `glu_act` with
+    shared expert in the same form; `interleave` (`shared_interleave`) as `moe_up` takes it (in blocks a multiple of 4); the gating of `glu_act` with
     `slope`, `limit` and `up_shift`.  W, I and S are multiples of 8, in blocks of 16, and at most 16,384; the router has up to 512 outputs.
 
     Scores and sums are float32; the experts' gated results go into the second product to 2^-17 of each (beside codes to 2^-22, or 2^-39 of the largest of 128 of

@@ -38,3 +38,13 @@ def test_the_form_of_the_framework_s_layer_beside_its_parts(T):
     parts = ops.moe_combine(ops.moe_down(act, m["down"], plan, Step()), plan, None, torch.empty_like(m["x"]))
     want, size, _ = plain(m, 4, 2.5, **HOW)
     assert bool(((call(m, 4, 2.5, **HOW).double().cpu() - parts.double().cpu()).abs() <= 2.0 ** -7 * want.abs() + 2.0 ** -7 * size).all())
+
+
+# groups of rows that lie across the ends of blocks of 128, and that end inside the eight rows of a load
+@pytest.mark.parametrize("blocks", [False, True])
+@pytest.mark.parametrize("I,S,il,shared_il", [(240, 48, 12, 12), (240, 80, 20, 4), (144, 0, 36, 0), (240, 240, 60, 120)])
+def test_other_interleavings(blocks, I, S, il, shared_il):
+    for T in (3, 12):
+        m = make(T, 144, I, 5, S, blocks=blocks)
+        want, size, _ = plain(m, 2, interleave=il, shared_interleave=shared_il)
+        close(call(m, 2, interleave=il, shared_interleave=shared_il), m, want, size, 2)
