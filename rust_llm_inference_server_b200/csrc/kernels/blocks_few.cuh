@@ -209,12 +209,16 @@ void blocks_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
     }
     // The sums are in registers: tensor memory goes back before the cluster meets.  A CTA that held it there would wait for CTAs that may wait for tensor memory, which
     // another kernel's CTAs hold that wait for their own cluster in turn; so whoever holds some here waits for nothing but its own copies and products.
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    // (The takers only say that they have read theirs, and the warp that gives it back has arrived at the cluster's barrier before: 0.2 to 0.3 us less than a barrier of all.)
     __syncwarp();
-    __syncthreads();
     if (warp == 1) {
+        if (splits > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+        asm volatile("bar.sync 3, %0;" ::"n"(TAKERS + 32) : "memory");
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(COLS) : "memory");
+    } else if (taker) {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        asm volatile("bar.arrive 3, %0;" ::"n"(TAKERS + 32) : "memory");
     }
     const int f_local = (warp & 3) * 32 + lane, f = n0 + f_local, group = (warp - 2) / 4, t0 = group * C;
     if (splits == 1) {
@@ -237,7 +241,8 @@ void blocks_few_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_c
                 if (t0 + 2 * i + 1 < M) part[(t0 + 2 * i + 1) * BF_F + f_local] = v.y;
             }
         }
-        cluster_sync_all();
+        if (warp == 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else cluster_sync_all();
         if (taker) {
             for (int t = split + group * splits; t < M; t += GROUPS * splits) {
                 float v = 0.f;
