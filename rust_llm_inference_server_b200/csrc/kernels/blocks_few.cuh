@@ -10,8 +10,9 @@
 // Matrices with few features would fill few SMs, so k is split over the CTAs of a thread-block cluster (any number up to 16).  Their sums go to shared memory, and
 // after a cluster barrier CTA r adds the rows r, r + splits, .. of all CTAs in the order of the splits: the result does not depend on timing.  The number of
 // splits depends on N and K alone up to 64 rows (few_splits), so a row has the same bits whatever other rows there are.
-// 8 rows x 16,384 of K 2048 from rows in blocks 8.3 us (4.0 TB/s; plain rows, put into blocks by the product, 10.3), 64 x 4,096 of K 14336
-// 15.9, one row x 2,048 of K 2048 3.4 (plain 3.9): a launch, the first tiles' way from memory and the cluster's meeting before anything else.
+// 8 rows x 16,384 of K 2048 from rows in blocks 8.4 us (4.0 TB/s; plain rows, put into blocks by the product, 10.3), 64 x 4,096 of K 14336
+// 16.0, one row x 2,048 of K 2048, over weights that no cache holds, 4.1 (plain or not): a launch, the first tiles' way from memory and the cluster's meeting before
+// anything else.
 // (Included by blocks_gemm.cu, whose error word it shares.)
 #pragma once
 

@@ -2,7 +2,8 @@
 //
 //   y[m, n] = sum over blocks b of  sx[b, m] sw[n / 128, b] * (sum over k in b of cx[m, k] cw[n, k])
 //
-// A block's products are exact in the tensor cores' float32 sums, but two blocks' sums may not meet before they are scaled: a tile's sums of 128 k go to an
+// Two codes' product is exact and a block's sum of them float32 (they reach over more than its 24 bits: the instruction of each 32 k may cut a unit off it), but two blocks'
+// sums may not meet before they are scaled: a tile's sums of 128 k go to an
 // accumulator of their own in tensor memory, and the epilogue's warps take it from there, scale it and add it to the tile's float32 sums, which they keep in
 // registers.  So they work beside the tensor core all the time and not after a tile: for each 128 x 128 x 128 products of an SM (256 cycles) they read 16,384 sums
 // and add as many, by two in an instruction (fma.rn.f32x2), 64 cycles of the four schedulers.
@@ -14,7 +15,7 @@
 // epilogues; warps 4-11 are the epilogue, a quarter of the rows and half of the columns each, and tell CTA 0 when they have read an accumulator.
 // Few rows: blocks_few.cuh.
 //
-// What bounds it (2,048 x 16,384 of K 2048, 63.3 us, 2,172 TFLOP/s; the nominal e4m3 rate would be 31): the tiles' way from the second-level cache (what is left without
+// What bounds it (2,048 x 16,384 of K 2048, 63 to 64 us, 2,160 TFLOP/s; the nominal e4m3 rate would be 31): the tiles' way from the second-level cache (what is left without
 // products and sums takes 44 us, in tiles of 128 columns 73, 11 TB/s), the epilogue's sums (55 without them) and the products (55 with a quarter of them) are of one
 // size, and none hides the others whole.  (The hand-over of an accumulator by an arrive that releases waited for the loads of scales on their way, 1,050 to 1,300
 // cycles a block: 132 us; the widths of loads from tensor memory make no difference.)

@@ -140,8 +140,9 @@ def quantize_matrix(w: torch.Tensor) -> BlockMatrix:
 
 def linear_blocks(x, w: BlockMatrix, out_dtype=None, *, early: bool = False) -> torch.Tensor:
     """y = x @ w^T for a weight in blocks.  x [T, K]: plain rows (bfloat16 or float32; may be a column slice of wider rows), which are put into blocks as
-    `quantize_rows` does, or BlockRows, for rows that several products read.  Every block of 128 k is summed on its own, scaled by both scales and added in
-    float32; the result is rounded once, to `out_dtype` (bfloat16 or float32; None: x's, bfloat16 for BlockRows).
+    `quantize_rows` does, or BlockRows, for rows that several products read.  Every block of 128 k is summed on its own in float32, multiplied by the product of both
+    scales (which should be a normal float32) and added in float32; the result is rounded once, to `out_dtype` (bfloat16 or float32; None: x's, bfloat16 for
+    BlockRows).  Up to 64 rows a row's bits do not depend on the other rows of the call.
     `early`: w is a weight that no kernel still in flight writes, so that its first tiles may be asked for before the kernels before have finished."""
     if not isinstance(w, BlockMatrix) or w.values.dim() != 2:
         raise KernelError("linear_blocks: expected a BlockMatrix [N, K]")
@@ -230,7 +231,8 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
     `slope`, `limit` and `up_shift`.  W, I and S are multiples of 8, in blocks of 16, and at most 16,384; the router has up to 512 outputs.
 
     Scores and sums are float32; the experts' gated results go into the second product to 2^-17 of each (beside codes to 2^-22, or 2^-39 of the largest of 128 of
-    them); a token's result is rounded once."""
+    them); a token's result is rounded once.  Its last bits depend on the call's other tokens, whose experts decide how the sums are cut up, and on nothing else.
+    An expert's weight that is no number, or infinite, reaches only the tokens that chose it, and a token that is not finite only itself; the router's are finite."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
         raise KernelError("moe_layer: expected bfloat16 rows [T, W] with unit stride on the device; there is no CPU path")
     dev = x.device

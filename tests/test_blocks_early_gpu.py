@@ -43,3 +43,14 @@ def test_plain_rows_that_the_kernel_before_writes(T):
     again = ops.linear_blocks(ops.linear_blocks(xs[0], w)[:, :1024], w)
     assert all(torch.equal(y, want[i % 4]) for i, y in enumerate(got)) and torch.equal(first, again)
     ops.check_device_errors()
+
+
+@pytest.mark.parametrize("N,K", [(2048, 2048), (700, 4100), (300, 14336)])
+def test_a_row_s_bits_do_not_depend_on_the_rows_beside_it(N, K):
+    """Up to 64 rows, whoever puts them into blocks."""
+    from rust_llm_inference_server_b200 import ops
+    x, w = torch.randn(64, K, device="cuda").bfloat16(), ops.quantize_matrix(torch.randn(N, K, device="cuda"))
+    whole = ops.linear_blocks(x, w, torch.float32)
+    for first, last in ((0, 1), (5, 6), (0, 2), (3, 19), (60, 64), (10, 42), (0, 63)):
+        assert torch.equal(ops.linear_blocks(x[first:last], w, torch.float32), whole[first:last])
+        assert torch.equal(ops.linear_blocks(ops.quantize_rows(x[first:last]), w, torch.float32), whole[first:last])
