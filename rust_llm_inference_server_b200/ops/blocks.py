@@ -232,7 +232,7 @@ def moe_layer(x: torch.Tensor, w_router: torch.Tensor, w_gate_up, w_down, top: i
 
     Scores and sums are float32; the experts' gated results go into the second product to 2^-17 of each (beside codes to 2^-22, or 2^-39 of the largest of 128 of
     them); a token's result is rounded once.  Its last bits depend on the call's other tokens, whose experts decide how the sums are cut up, and on nothing else.
-    An expert's weight that is no number, or infinite, reaches only the tokens that chose it, and a token that is not finite only itself; the router's are finite."""
+    An expert's weight that is no number, or infinite, reaches only the tokens that chose it, and a token that is not finite only itself; the router's lie below 2^127."""
     if not isinstance(x, torch.Tensor) or not x.is_cuda or x.dtype != torch.bfloat16 or x.dim() != 2 or x.stride(1) != 1:
         raise KernelError("moe_layer: expected bfloat16 rows [T, W] with unit stride on the device; there is no CPU path")
     dev = x.device
