@@ -3,9 +3,8 @@
 //   y[m, n] = sum over blocks b of  sx[b, m] sw[n / 128, b] * (sum over k in b of cx[m, k] cw[n, k])
 //
 // Two codes' product is exact and a block's sum of them float32 (they reach over more than its 24 bits: the instruction of each 32 k may cut a unit off it), but two blocks'
-// sums may not meet before they are scaled: a tile's sums of 128 k go to an
-// accumulator of their own in tensor memory, and the epilogue's warps take it from there, scale it and add it to the tile's float32 sums, which they keep in
-// registers.  So they work beside the tensor core all the time and not after a tile: for each 128 x 128 x 128 products of an SM (256 cycles) they read 16,384 sums
+// sums may not meet before they are scaled: a tile's sums of 128 k go to an accumulator of their own in tensor memory, and the epilogue's warps take it from there,
+// scale it and add it to the tile's float32 sums, which they keep in registers.  So they work beside the tensor core all the time and not after a tile: for each 128 x 128 x 128 products of an SM (256 cycles) they read 16,384 sums
 // and add as many, by two in an instruction (fma.rn.f32x2), 64 cycles of the four schedulers.
 //
 // Many rows (this file): two SMs to a tile of 256 x BN, `tcgen05.mma.cta_group::2` of kind::f8f6f4.  A cluster of two CTAs; CTA r holds rows 128 r .. of x and

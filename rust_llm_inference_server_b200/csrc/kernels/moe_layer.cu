@@ -20,8 +20,8 @@
 //
 // The weights of the choice are multiplied into h in float32; the down product is then one long sum over the chosen experts' k, with the step's tokens as columns
 // whoever chose them.  Its CTAs bring the pieces of h that their chunks meet into shared memory first (read from the second-level cache chunk by chunk they took
-// more of the load units than the weights: 16 tokens, 83 of 128 experts of 768 in blocks 135 us, 111 so, each with one number of float16 for h).  Nothing but the result is rounded to the activations'
-// type: beside bfloat16 weights h is two bfloat16 numbers (their sum is h to 2^-17).  Codes become float16 by one instruction a pair (as bfloat16, which has none,
+// more of the load units than the weights: 16 tokens, 83 of 128 experts of 768 in blocks 135 us, 111 so, each with one number of float16 for h).
+// Nothing but the result is rounded to the activations' type: beside bfloat16 weights h is two bfloat16 numbers (their sum is h to 2^-17).  Codes become float16 by one instruction a pair (as bfloat16, which has none,
 // a word of four took 10 cycles of a scheduler instead of 5, and the products waited for it), so the tokens' rows and h's meet them as float16 of eleven bits, each
 // row (of h each piece of 128) times the power of two that brings its largest value to 2^14 .. 2^15: x is that exactly down to 2^-31 of the largest, h is two such
 // numbers, whose sum is h to 2^-22, or 2^-39 of the piece's largest.  (One of them is h to 2^-11 and takes 112 us for 121 in that layer, 41.3 for 43.6 with 8 tokens; but its
